@@ -343,6 +343,71 @@ typedef struct wnv_logmel_args {
 } wnv_logmel_args;
 WNV_API wnv_status wnv_logmel(wnv_mel_handle h, const wnv_logmel_args* args);
 
+/* ---- gated linear recurrence (added within ABI 6) -------------------------------------------------------
+ * The recurrent counterpart of the gated layer: with z = (f | v | o) along the channels,
+ *     h_t = sigmoid(f_t) h_{t-1} + (1 - sigmoid(f_t)) v_t        y_t = h_t sigmoid(o_t)        (gates == 2: no o, y = h)
+ * over (B, T, C), channels last, state and every sum in float32.  h_{t-1} reads as zero at a step that begins an utterance of a
+ * packed slot (seg_start[b][t] == t, the map of wnv_generate_args; a negative entry: begun before this call, h0 goes on), and rows
+ * of a padded batch end at lengths[b]: behind it z is not looked at, y and the gradients are zero and the state is handed on, so
+ * h_last is the state behind the last real step (h0 for an empty row).  lengths are taken as min(max(lengths[b], 0), T).
+ * The maps live in device memory and are not range-checked further: any value of seg_start other than t just does not begin one.
+ * No atomics on data: the same call gives the same bits.  Everything a call needs beyond its arguments is in `workspace`, which the
+ * call writes before it reads: calls that may run at the same time (other streams, graphs replayed side by side) each have their own. */
+typedef enum wnv_dtype { WNV_F32 = 0, WNV_BF16 = 1, WNV_F16 = 2 } wnv_dtype;
+struct wnv_recurrence_args {
+    int32_t B, C;
+    int64_t T;
+    int32_t gates;             /* 3: z = (f | v | o);  2: z = (f | v)                                          */
+    int32_t dtype;             /* wnv_dtype of z, y, dy and dz                                                 */
+    const void* z;             /* device (B, T, gates C): channels contiguous, the strides below >= 0          */
+    int64_t z_batch_stride, z_time_stride;      /* in elements; 0: broadcast                                   */
+    const float* h0;           /* device (B, C) float32 with a row stride, or NULL (zeros)                      */
+    int64_t h0_batch_stride;
+    const int32_t* lengths;    /* device (B), or NULL                                                          */
+    const int32_t* seg_start;  /* device (B, T), or NULL                                                       */
+    void* y;                   /* forward: device (B, T, C)                                                    */
+    float* h_last;             /* forward: device (B, C)                                                       */
+    void* saved;               /* forward: wnv_recurrence_saved_bytes for the backward pass to read, or NULL   */
+    void* workspace;           /* wnv_recurrence_workspace_bytes; may be NULL when that is 0                    */
+    const void* dy;            /* backward: device (B, T, C) with the strides below, or NULL (zeros)           */
+    int64_t dy_batch_stride, dy_time_stride;
+    const float* dh_last;      /* backward: device (B, C), or NULL (zeros)                                     */
+    void* dz;                  /* backward: device (B, T, gates C), contiguous                                 */
+    float* dh0;                /* backward: device (B, C), or NULL                                             */
+    void* stream;
+};
+typedef struct wnv_recurrence_args wnv_recurrence_args;
+/* Sizes of the two buffers (16-byte aligned device memory); -1 on bad arguments.  Host only. */
+WNV_API int64_t wnv_recurrence_saved_bytes(int32_t B, int64_t T, int32_t C, int32_t gates, int32_t dtype);
+WNV_API int64_t wnv_recurrence_workspace_bytes(int32_t B, int64_t T, int32_t C, int32_t gates, int32_t dtype);
+WNV_API wnv_status wnv_recurrence_forward(int32_t device, const wnv_recurrence_args* args);
+/* The same z, h0, lengths and seg_start as the forward call that filled `saved`. */
+WNV_API wnv_status wnv_recurrence_backward(int32_t device, const wnv_recurrence_args* args);
+/* One step: z device (B, gates C) with a row stride, state device (B, C) float32 updated in place, y device (B, C). */
+WNV_API wnv_status wnv_recurrence_step(int32_t device, const void* z, int64_t z_batch_stride, float* state, void* y, int32_t B, int32_t C,
+                               int32_t gates, int32_t dtype, void* stream);
+
+/* ---- 4-bit weights (added within ABI 6) ---------------------------------------------------------------
+ * The 1x1 convolution of one time step with weights of 4 bits: y = x W^T + bias,
+ *     W[n][k] = scale[n][k / group] (code[n][k] - zero[n][k / group]),    group 32, 64 or 128 inputs, the last one may be short.
+ * Scales are bf16; x and y have the call's dtype, sums are float32.  gates > 1: the outputs are that many gates of cout / gates
+ * channels, as the recurrence above takes them.  Setting weights waits for the device; after that a handle is only read, from any
+ * number of streams at once.  An infinite or NaN input makes the outputs of its own row NaN. */
+typedef struct wnv_q4* wnv_q4_handle;
+WNV_API wnv_status wnv_q4_create(int32_t cin, int32_t cout, int32_t gates, int32_t group, int32_t device, wnv_q4_handle* out);
+/* All device memory: codes (cout, cin) one per byte, scales bf16 (cout, ceil(cin / group)), zeros the same shape or NULL (8),
+ * bias float32 (cout) or NULL.  A code or zero point over 15: WNV_ERR_INVALID_ARG. */
+WNV_API wnv_status wnv_q4_set_codes(wnv_q4_handle h, const uint8_t* codes, const void* scales, const uint8_t* zeros, const float* bias,
+                            void* stream);
+/* weight device float32 (cout, cin), rounded here: asymmetric, a 15th of each group's range (widened to hold 0) as its scale. */
+WNV_API wnv_status wnv_q4_set_weights(wnv_q4_handle h, const float* weight, const float* bias, void* stream);
+WNV_API wnv_status wnv_q4_dequantise(wnv_q4_handle h, float* weight, void* stream);      /* device float32 (cout, cin) = W */
+WNV_API wnv_status wnv_q4_step(wnv_q4_handle h, const void* x, int64_t x_row_stride, void* y, int32_t B, int32_t dtype, void* stream);
+/* z = x W^T + bias kept in float32, then wnv_recurrence_step on it: x (B, cin), state (B, C) in place, y (B, C); C = cout / gates. */
+WNV_API wnv_status wnv_q4_recurrence_step(wnv_q4_handle h, const void* x, int64_t x_row_stride, float* state, void* y, int32_t B,
+                                  int32_t dtype, void* stream);
+WNV_API wnv_status wnv_q4_destroy(wnv_q4_handle h);
+
 /* ---- host helpers for a streamed replay tape (ABI 3) -------------------------------------------------
  * The reference draws its sampling noise from torch's CPU generator inside the loop (wavenet.py:334-335: OneHotCategorical ->
  * torch.multinomial's exponential race, B x 256 values per step); a replay of that stream is 49 M values for the benchmark batch

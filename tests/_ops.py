@@ -1,0 +1,132 @@
+"""Plain 64-bit forms of the gated recurrence and of the 4-bit products, and the error bounds that the tests hold the kernels to.
+
+Bounds, M = max(|v|, |h0|), S = max|dh|, u = 1 - sigmoid(f), eps = 2^-24 (half a step of float32):
+  * a gate is off by at most delta = (1.5 |f| + 8) eps of itself, next to 0 and next to 1: the exponent f log2(e) is rounded (|f| eps at
+    most, 1.5 with the change of base), exp2 and the reciprocal are within an ulp, and three more operations follow;
+  * h is a convex combination of the v and h0, so |h| <= M.  h_t = h + u (v - h) rounds three times (3 eps 2 M at most) and carries
+    u delta 2 M of the gate; an older error shrinks by 1 - u per step: at most 1 / u_min or T of them live at a time.  Maps of whole
+    stretches h -> h + (B - U h) round as often again when they are joined.  So |h - exact| <= k M with
+    k = 2 delta + 12 eps min(T, 1 / u_min) + 12 eps;
+  * dh_t = s, what goes back is s - u s: the same recursion with S in place of M, |dh - exact| <= k S;
+  * df = dh (h_{t-1} - v) sigmoid(f) u: k S 2 M + S k M + S 2 M (2 delta + 4 eps), times sigmoid(f) u <= 1/4: within k S M;
+    dv = dh u: (k + delta + eps) S <= 2 k S;  do = dy h sigmoid(o)(1 - sigmoid(o)): (k M + M (2 delta + 4 eps)) |dy| / 4 <= k M |dy|.
+  * the result's own type rounds by finfo.eps / 2 of the value (half a step of the smallest number near zero)."""
+import torch
+
+EPS = 2.0 ** -24
+DTYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+
+
+def oracle_scan(z, h0=None, output_gate=True, lengths=None, seg_start=None, dy=None, dh_last=None):
+    """float64 on the CPU, step by step.  -> dict(y, h_last, dz, dh0, h, dh) (gradients where dy is given)."""
+    z = z.detach().double().cpu()
+    B, T, n = z.shape
+    C = n // (3 if output_gate else 2)
+    live = torch.ones(B, T, dtype=torch.bool)
+    if lengths is not None:
+        live = torch.arange(T) < lengths.cpu().long()[:, None]
+    begins = torch.zeros(B, T, dtype=torch.bool)
+    if seg_start is not None:
+        begins = seg_start.cpu().long() == torch.arange(T)
+    begins &= live
+    z = torch.where(live[..., None], z, torch.zeros(()).double())
+    f, v = z[..., :C], z[..., C:2 * C]
+    a, u = torch.sigmoid(f), torch.sigmoid(-f)
+    so = torch.sigmoid(z[..., 2 * C:]) if output_gate else torch.ones(B, T, C).double()
+    h = torch.zeros(B, C).double() if h0 is None else h0.detach().double().cpu()
+    hs, before = [], []
+    for t in range(T):
+        p = torch.where(begins[:, t, None], torch.zeros(()).double(), h)
+        before.append(p)
+        h = torch.where(live[:, t, None], a[:, t] * p + u[:, t] * v[:, t], h)
+        hs.append(h)
+    hs, before = torch.stack(hs, 1), torch.stack(before, 1)
+    out = dict(y=torch.where(live[..., None], hs * so, torch.zeros(()).double()), h_last=h, h=hs)
+    if dy is None and dh_last is None:
+        return out
+    dy = torch.zeros(B, T, C).double() if dy is None else torch.where(live[..., None], dy.double().cpu(), torch.zeros(()).double())
+    r = torch.zeros(B, C).double() if dh_last is None else dh_last.double().cpu()
+    dhs = [None] * T
+    for t in reversed(range(T)):
+        d = dy[:, t] * so[:, t] + r
+        dhs[t] = torch.where(live[:, t, None], d, torch.zeros(()).double())
+        d = torch.where(begins[:, t, None], torch.zeros(()).double(), a[:, t] * d)
+        r = torch.where(live[:, t, None], d, r)
+    dh = torch.stack(dhs, 1)
+    dz = [dh * (before - v) * a * u, dh * u]
+    if output_gate:
+        dz.append(torch.where(live[..., None], dy * hs * so * torch.sigmoid(-z[..., 2 * C:]), torch.zeros(()).double()))
+    dz = torch.where(live[..., None], torch.cat(dz, -1), torch.zeros(()).double())
+    out.update(dz=dz, dh0=r, dh=dh)
+    return out
+
+
+def scan_bounds(z, want, h0=None, output_gate=True, lengths=None, dy=None, dh_last=None):
+    """k and the scales M, S, |dy| of the module's text, from the inputs and the exact result."""
+    z = z.detach().double().cpu()
+    T, C = z.shape[1], z.shape[2] // (3 if output_gate else 2)
+    if lengths is not None:
+        z = torch.where((torch.arange(T) < lengths.cpu().long()[:, None])[..., None], z, torch.zeros(()).double())
+    f, v, o = z[..., :C], z[..., C:2 * C], z[..., 2 * C:]
+    top = max(float(f.abs().max()), float(o.abs().max()) if output_gate else 0.0)
+    delta = (1.5 * top + 8) * EPS
+    k = 2 * delta + 12 * EPS * min(T, 1 / float(torch.sigmoid(-f).min())) + 12 * EPS
+    M = max(float(v.abs().max()), 0.0 if h0 is None else float(h0.abs().max()))
+    S = 0.0
+    if "dh" in want:
+        S = max(float(want["dh"].abs().max()), 0.0 if dh_last is None else float(dh_last.abs().max()))
+    D = 0.0 if dy is None else float(dy.double().abs().max())
+    return k, M, S, D
+
+
+def near(got, want, bound, what=""):
+    """|got - want| <= bound + the rounding to got's own type."""
+    info = torch.finfo(got.dtype)
+    got = got.detach().double().cpu()
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    assert bool(torch.isfinite(got).all()) == bool(torch.isfinite(want).all()), f"{what}: not finite"
+    allowed = bound + info.eps / 2 * (want.abs() + bound) + info.smallest_normal * info.eps / 2
+    over = (got - want).abs() / allowed
+    worst = float(over.max()) if over.numel() else 0.0
+    assert worst <= 1.0, f"{what}: {worst:.3g} times its bound (error {float((got - want).abs().max()):.3g}, bound {bound:.3g})"
+
+
+def check_scan(got, want, z, h0=None, output_gate=True, lengths=None, dy=None, dh_last=None):
+    """got: dict with y, h_last and, for gradients, dz, dh0."""
+    k, M, S, D = scan_bounds(z, want, h0, output_gate, lengths, dy, dh_last)
+    near(got["y"], want["y"], 2 * k * M, "y")       # the output gate multiplies once more: delta + eps
+    near(got["h_last"], want["h_last"], k * M, "h_last")
+    if "dz" in got:
+        C = want["h"].shape[-1]
+        near(got["dz"][..., :C], want["dz"][..., :C], 2 * k * S * M, "df")
+        near(got["dz"][..., C:2 * C], want["dz"][..., C:2 * C], 2 * k * S, "dv")
+        if output_gate:
+            near(got["dz"][..., 2 * C:], want["dz"][..., 2 * C:], k * M * D, "do")
+    if got.get("dh0") is not None:
+        near(got["dh0"], want["dh0"], k * S, "dh0")
+
+
+def q4_weight(codes, scales, zeros, group):
+    at = torch.arange(codes.shape[1]) // group
+    zp = torch.full_like(scales.double().cpu(), 8.0) if zeros is None else zeros.double().cpu()
+    return scales.double().cpu()[:, at] * (codes.double().cpu() - zp[:, at])
+
+
+def q4_bound(x, codes, scales, zeros, group, bias):
+    """Of the products' sums in float32, per output: the codes enter with an offset of up to 16 (24 with the zero point's own 16 + 15
+    against it), sums of 32 inputs are joined one after the other, then the groups: at most 64 + K / 32 roundings of a running sum of
+    the magnitudes, and the bias."""
+    K = codes.shape[1]
+    at = torch.arange(K) // group
+    s = scales.double().cpu().abs()[:, at]
+    mass = x.double().cpu().abs() @ (s * 62).t()
+    return (64 + K / 32) * EPS * mass + 2 * EPS * (0 if bias is None else bias.double().cpu().abs())
+
+
+def random_q4(n, k, group, seed, zeros=True):
+    g = torch.Generator().manual_seed(seed)
+    groups = -(-k // group)
+    codes = torch.randint(0, 16, (n, k), generator=g, dtype=torch.uint8)
+    scales = (torch.rand(n, groups, generator=g) * 0.1 + 0.01).to(torch.bfloat16)
+    zp = torch.randint(0, 16, (n, groups), generator=g, dtype=torch.uint8) if zeros else None
+    return codes, scales, zp

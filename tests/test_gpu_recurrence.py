@@ -1,0 +1,374 @@
+"""The gated recurrence on the GPU against its plain 64-bit form (tests/_ops.py, with the bounds' derivation)."""
+import pytest
+import torch
+
+from tests._ops import DTYPES, check_scan, near, oracle_scan
+from wavenet_vocoder_amd.recurrence import gated_recurrence, gated_recurrence_step
+
+pytestmark = pytest.mark.gpu
+
+
+def inputs(B, T, C, gates, dt, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    z = torch.randn(B, T, gates * C, generator=g)
+    z[..., :C] = z[..., :C] * 1.5 + 2.0
+    return (z.to(dt), torch.randn(B, C, generator=g), torch.randn(B, T, C, generator=g).to(dt), torch.randn(B, C, generator=g))
+
+
+def maps(kind, B, T, seed=0):
+    g = torch.Generator().manual_seed(seed + 77)
+    if kind == "lengths":
+        n = torch.randint(0, T + 1, (B,), generator=g)
+        n[0] = 0
+        n[-1] = T
+        if B > 2:
+            n[1] = 1
+        return dict(lengths=n.to(torch.int32))
+    if kind in ("packed", "both"):
+        first = torch.rand(B, T, generator=g) < 0.02
+        first[::2, 0] = True
+        at = torch.arange(T).expand(B, T)
+        m = dict(seg_start=torch.where(first, at, torch.tensor(-1)).cummax(1).values.to(torch.int32))
+        if kind == "both":
+            m["lengths"] = torch.randint(0, T + 1, (B,), generator=g).to(torch.int32)
+        return m
+    return {}
+
+
+def run(z, h0, dy, dh, gates, m, grads=True):
+    """One forward and backward pass through the public function; outputs as check_scan takes them."""
+    zc = z.cuda().requires_grad_(grads)
+    hc = None if h0 is None else h0.cuda().requires_grad_(grads)
+    mc = {k: v.cuda() for k, v in m.items()}
+    y, h_last = gated_recurrence(zc, hc, output_gate=gates == 3, **mc)
+    got = dict(y=y, h_last=h_last)
+    if grads:
+        leaves = (zc,) if hc is None else (zc, hc)
+        d = torch.autograd.grad((y, h_last), leaves, (dy.cuda(), dh.cuda()))
+        got.update(dz=d[0], dh0=d[1] if hc is not None else None)
+    torch.cuda.synchronize()
+    return got
+
+
+SHAPES = [(1, 1, 1), (2, 2, 3), (3, 7, 20), (2, 127, 64), (2, 128, 65), (3, 129, 33), (1, 300, 128), (2, 513, 17), (4, 1000, 72),
+          (1, 2500, 8), (2, 1025, 201), (1, 4097, 40)]
+
+
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+@pytest.mark.parametrize("gates", [2, 3])
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "x".join(map(str, s)))
+def test_scan_and_gradients(shape, gates, dtype):
+    B, T, C = shape
+    z, h0, dy, dh = inputs(B, T, C, gates, DTYPES[dtype], seed=T)
+    want = oracle_scan(z, h0, gates == 3, dy=dy, dh_last=dh)
+    check_scan(run(z, h0, dy, dh, gates, {}), want, z, h0, gates == 3, None, dy, dh)
+
+
+@pytest.mark.parametrize("kind", ["lengths", "packed", "both"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(5, 1, 8), (4, 130, 24), (3, 700, 129), (5, 2049, 16)], ids=lambda s: "x".join(map(str, s)))
+def test_padded_batches_and_packed_slots(shape, dtype, kind):
+    B, T, C = shape
+    z, h0, dy, dh = inputs(B, T, C, 3, DTYPES[dtype], seed=T + 1)
+    m = maps(kind, B, T, seed=T)
+    want = oracle_scan(z, h0, True, dy=dy, dh_last=dh, **m)
+    got = run(z, h0, dy, dh, 3, m)
+    check_scan(got, want, z, h0, True, m.get("lengths"), dy, dh)
+    if "lengths" in m:
+        behind = torch.arange(T) >= m["lengths"][:, None]
+        assert not got["y"].cpu()[behind].any() and not got["dz"].cpu()[behind].any()
+        empty = m["lengths"] == 0
+        assert torch.equal(got["h_last"].cpu()[empty], h0[empty]) and torch.equal(got["dh0"].cpu()[empty], dh[empty])
+
+
+@pytest.mark.parametrize("T", [40, 1500])
+@pytest.mark.parametrize("poison", [float("nan"), float("inf"), -float("inf")])
+def test_what_stands_behind_a_length_is_not_looked_at(poison, T):
+    B, C = 3, 40
+    z, h0, dy, dh = inputs(B, T, C, 3, torch.float32, seed=5)
+    n = torch.tensor([0, T // 2, T - 1], dtype=torch.int32)
+    clean = run(z, h0, dy, dh, 3, dict(lengths=n))
+    behind = torch.arange(T) >= n[:, None]
+    z[behind] = poison
+    dy[behind] = poison
+    got = run(z, h0, dy, dh, 3, dict(lengths=n))
+    for k in clean:
+        assert torch.equal(got[k], clean[k]), k
+
+
+@pytest.mark.parametrize("T", [60, 1500])
+def test_a_broken_utterance_stays_its_own(T):
+    """NaN and infinities of one utterance of a packed slot reach neither the next one's outputs nor the earlier one's gradients."""
+    z, h0, dy, dh = inputs(1, T, 16, 3, torch.float32, seed=6)
+    a, b = T // 3, 2 * T // 3
+    start = torch.zeros(1, T, dtype=torch.int32)
+    start[:, a:b], start[:, b:] = a, b
+    clean = run(z, h0, dy, dh, 3, dict(seg_start=start))
+    z[:, a + 2], z[:, b - 3] = float("nan"), float("inf")
+    dy[:, b - 2] = float("nan")
+    got = run(z, h0, dy, dh, 3, dict(seg_start=start))
+    for k in ("y", "dz"):
+        assert torch.equal(got[k][:, :a], clean[k][:, :a]) and torch.equal(got[k][:, b:], clean[k][:, b:]), k
+        assert torch.isnan(got[k][:, a:b]).any()
+    assert torch.equal(got["h_last"], clean["h_last"]) and torch.equal(got["dh0"], clean["dh0"])
+
+
+def test_a_nan_input_is_seen():
+    z, h0, dy, dh = inputs(1, 700, 4, 3, torch.float32)
+    z[0, 300, 1] = float("nan")                     # the gate of channel 1
+    got = run(z, h0, dy, dh, 3, {})
+    assert torch.isnan(got["y"][0, 300:, 1]).all() and torch.isnan(got["h_last"][0, 1])
+    assert torch.isfinite(got["y"][..., [0, 2, 3]]).all() and torch.isfinite(got["y"][0, :300]).all()
+    assert torch.isnan(got["dh0"][0, 1])
+
+
+@pytest.mark.parametrize("f", [-200.0, -30.0, 30.0, 200.0])
+@pytest.mark.parametrize("T", [5, 900])
+def test_gates_at_their_ends(f, T):
+    z, h0, dy, dh = inputs(2, T, 12, 3, torch.float32, seed=9)
+    z[..., :12] = f
+    want = oracle_scan(z, h0, True, dy=dy, dh_last=dh)
+    check_scan(run(z, h0, dy, dh, 3, {}), want, z, h0, True, None, dy, dh)
+
+
+def test_long_memory_keeps_its_precision():
+    """f = 9 remembers 8000 steps: a gate held only as sigmoid(f) in float32 would be 2e-4 off here."""
+    T, C = 12000, 8
+    z, h0, dy, dh = inputs(1, T, C, 2, torch.float32, seed=11)
+    z[..., :C] = 9.0
+    z[..., C:] += 1.0
+    want = oracle_scan(z, h0, False, dy=dy, dh_last=dh)
+    got = run(z, h0, dy, dh, 2, {})
+    check_scan(got, want, z, h0, False, None, dy, dh)
+    # random roundings: eps sqrt(8000) each way, far below the bound's sum of them and below 2e-4
+    assert float((got["h_last"].double().cpu() - want["h_last"]).abs().max()) < 2e-5 * float(z[..., C:].abs().max())
+
+
+def test_optional_arguments_and_partial_gradients():
+    z, h0, dy, dh = inputs(2, 333, 24, 3, torch.float32, seed=3)
+    want = oracle_scan(z, None, True, dy=dy)
+    zc = z.cuda().requires_grad_()
+    y, h_last = gated_recurrence(zc)
+    dz, = torch.autograd.grad(y, zc, dy.cuda(), retain_graph=True)
+    check_scan(dict(y=y, h_last=h_last, dz=dz), want, z, None, True, None, dy, None)
+    dz, = torch.autograd.grad(h_last, zc, dh.cuda())            # no gradient at y
+    want = oracle_scan(z, None, True, dh_last=dh)
+    check_scan(dict(y=y, h_last=h_last, dz=dz), want, z, None, True, None, None, dh)
+    hc = h0.cuda().requires_grad_()                             # the state alone
+    y, h_last = gated_recurrence(z.cuda(), hc)
+    d, = torch.autograd.grad((y, h_last), hc, (dy.cuda(), dh.cuda()))
+    near(d, oracle_scan(z, h0, True, dy=dy, dh_last=dh)["dh0"], 1e-3, "dh0")
+    with torch.no_grad():
+        assert torch.equal(gated_recurrence(zc)[0], gated_recurrence(z.cuda())[0])
+    assert not gated_recurrence(z.cuda())[0].requires_grad
+
+
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+@pytest.mark.parametrize("how", ["offset", "wide", "time", "broadcast_time", "broadcast_batch", "columns"])
+def test_strides(how, dtype):
+    """Views of other alignments and orders give the bits of the same values laid out densely."""
+    B, T, C, dt = 3, 300, 24, DTYPES[dtype]
+    z, h0, dy, dh = (t.cuda() for t in inputs(B, T, C, 3, dt, seed=13))
+    if how == "offset":                 # one element behind an aligned address
+        v = torch.empty(z.numel() + 1, dtype=dt, device="cuda")[1:].view(z.shape).copy_(z)
+    elif how == "wide":                 # a slice of wider rows
+        v = torch.zeros(B, T, 3 * C + 7, dtype=dt, device="cuda")[..., 3:3 + 3 * C].copy_(z)
+    elif how == "time":                 # time first in memory
+        v = torch.empty(T, B, 3 * C, dtype=dt, device="cuda").transpose(0, 1).copy_(z)
+    elif how == "broadcast_time":
+        z = z[:, :1].expand(B, T, 3 * C).contiguous()
+        v = z[:, :1].contiguous().expand(B, T, 3 * C)
+    elif how == "broadcast_batch":
+        z = z[:1].expand(B, T, 3 * C).contiguous()
+        v = z[:1].contiguous().expand(B, T, 3 * C)
+    else:                               # channels are not contiguous: copied once
+        v = torch.empty(B, 3 * C, T, dtype=dt, device="cuda").transpose(1, 2).copy_(z)
+    dyv = torch.empty(T, B, C, dtype=dt, device="cuda").transpose(0, 1).copy_(dy)
+    outs = []
+    for a, d in ((z, dy), (v, dyv)):
+        a = a.detach().requires_grad_()
+        y, h = gated_recurrence(a, h0)
+        outs.append((y, h, *torch.autograd.grad((y, h), a, (d, dh))))
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+
+
+def test_gradients_of_broadcast_inputs():
+    """One row of gates for the whole batch, one initial state for all rows: their gradients are the sums over the batch."""
+    B, T, C = 4, 150, 16
+    z, h0, dy, dh = inputs(B, T, C, 3, torch.float32, seed=17)
+    z, h0 = z[:1], h0[:1]
+    want = oracle_scan(z.expand(B, -1, -1), h0.expand(B, -1), True, dy=dy, dh_last=dh)
+    zc, hc = z.cuda().requires_grad_(), h0.cuda().requires_grad_()
+    y, h = gated_recurrence(zc.expand(B, -1, -1), hc.expand(B, -1))
+    dz, dh0 = torch.autograd.grad((y, h), (zc, hc), (dy.cuda(), dh.cuda()))
+    near(dz, want["dz"].sum(0, keepdim=True), 1e-3, "dz")
+    near(dh0, want["dh0"].sum(0, keepdim=True), 1e-3, "dh0")
+
+
+@pytest.mark.parametrize("gates", [2, 3])
+def test_gradient_against_differences(gates):
+    """<gradient, d> = (L(x + e d) - L(x - e d)) / 2 e of the exact forward pass, to e^2 and the gradient's own float32 error."""
+    B, T, C = 2, 200, 6
+    z, h0, dy, dh = inputs(B, T, C, gates, torch.float32, seed=19)
+    got = run(z, h0, dy, dh, gates, {})
+    g = torch.Generator().manual_seed(1)
+    for _ in range(4):
+        d, e = torch.randn(z.shape, generator=g).double(), 1e-4
+        d0 = torch.randn(h0.shape, generator=g).double()
+        L = []
+        for s in (e, -e):
+            o = oracle_scan(z.double() + s * d, h0.double() + s * d0, gates == 3)
+            L.append(float((o["y"] * dy.double()).sum() + (o["h_last"] * dh.double()).sum()))
+        diff = (L[0] - L[1]) / (2 * e)
+        dot = float((got["dz"].double().cpu() * d).sum() + (got["dh0"].double().cpu() * d0).sum())
+        mass = float((got["dz"].double().cpu() * d).abs().sum() + (got["dh0"].double().cpu() * d0).abs().sum())
+        assert abs(diff - dot) <= 1e-5 * mass, (diff, dot, mass)
+
+
+def test_batch_strides_over_32_bits():
+    C, T = 8, 40
+    z, h0, dy, dh = inputs(2, T, C, 3, torch.bfloat16, seed=23)
+    far = (1 << 31) + 8                 # elements between the two rows
+    buf = torch.empty(far + T * 3 * C, dtype=torch.bfloat16, device="cuda")
+    v = buf.as_strided((2, T, 3 * C), (far, 3 * C, 1))
+    v.copy_(z)
+    v.requires_grad_()
+    y, h = gated_recurrence(v, h0.cuda())
+    dz, = torch.autograd.grad((y, h), v, (dy.cuda(), dh.cuda()))
+    want = run(z, h0, dy, dh, 3, {})
+    assert torch.equal(y, want["y"]) and torch.equal(h, want["h_last"]) and torch.equal(dz, want["dz"])
+
+
+def test_outputs_over_32_bits():
+    """dz of 2.6e9 values: the last row and a middle one against the same rows alone."""
+    B, T, C = 18, 24064, 2000
+    g = torch.Generator(device="cuda").manual_seed(3)
+    z = torch.randn(B, T, 3 * C, generator=g, device="cuda", dtype=torch.bfloat16).requires_grad_()
+    dy = torch.randn(B, T, C, generator=g, device="cuda", dtype=torch.bfloat16)
+    y, h = gated_recurrence(z)
+    dz, = torch.autograd.grad(y, z, dy)
+    for b in (B // 2, B - 1):
+        zb = z[b:b + 1].detach().clone().requires_grad_()
+        yb, hb = gated_recurrence(zb)
+        dzb, = torch.autograd.grad(yb, zb, dy[b:b + 1])
+        # one row alone may be cut into stretches elsewhere: equal to the roundings of bf16 and of the sums behind them
+        for p, q in ((y[b], yb[0]), (dz[b], dzb[0]), (h[b], hb[0])):
+            assert float((p.float() - q.float()).abs().max()) <= 2.0 ** -8 * float(q.float().abs().max()) * 1.01
+
+
+def test_the_same_call_gives_the_same_bits():
+    z, h0, dy, dh = inputs(3, 2000, 96, 3, torch.bfloat16, seed=29)
+    first = run(z, h0, dy, dh, 3, {})
+    for _ in range(5):
+        again = run(z, h0, dy, dh, 3, {})
+        for k in first:
+            assert torch.equal(first[k], again[k]), k
+
+
+def test_two_streams_at_once():
+    args = [inputs(2, 3000, 64, 3, torch.float32, seed=s) for s in (31, 37)]
+    want = [run(*a, 3, {}) for a in args]
+    dev = [[t.cuda() for t in a] for a in args]
+    streams = [torch.cuda.Stream() for _ in args]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(10):
+        got = []
+        for (z, h0, dy, dh), s in zip(dev, streams):
+            with torch.cuda.stream(s):
+                a, b = z.detach().requires_grad_(), h0.detach().requires_grad_()
+                y, h = gated_recurrence(a, b)
+                got.append((y, h, *torch.autograd.grad((y, h), (a, b), (dy, dh))))
+        torch.cuda.synchronize()
+        for g, w in zip(got, want):
+            for x, k in zip(g, ("y", "h_last", "dz", "dh0")):
+                assert torch.equal(x, w[k]), k
+
+
+@pytest.mark.parametrize("T", [50, 3000])
+def test_captured_and_replayed(T):
+    """Forward and backward of two graphs with inputs of their own, replayed in turn and side by side with eager work between."""
+    args = [inputs(2, T, 48, 3, torch.bfloat16, seed=s) for s in (41, 43)]
+    start = maps("packed", 2, T)["seg_start"].cuda()
+    graphs, bufs, outs = [], [], []
+    for a in args:
+        z, h0, dy, dh = (t.cuda() for t in a)
+        z, h0 = z.requires_grad_(), h0.requires_grad_()
+
+        def once(z=z, h0=h0, dy=dy, dh=dh):
+            y, h = gated_recurrence(z, h0, seg_start=start)
+            return (y, h, *torch.autograd.grad((y, h), (z, h0), (dy, dh)))
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            once()
+        torch.cuda.current_stream().wait_stream(side)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(once())
+        graphs.append(g)
+        bufs.append((z, h0, dy, dh, once))
+    other = torch.cuda.Stream()
+    for rep in range(4):
+        with torch.no_grad():
+            for z, h0, dy, dh, _ in bufs:
+                z.copy_(torch.randn_like(z) + 1)
+                h0.copy_(torch.randn_like(h0))
+        want = [b[4]() for b in bufs]
+        for o in outs:
+            for t in o:
+                t.detach().zero_()
+        torch.cuda.synchronize()
+        if rep % 2:
+            with torch.cuda.stream(other):
+                graphs[1].replay()
+            graphs[0].replay()
+        else:
+            graphs[0].replay()
+            graphs[1].replay()
+        torch.cuda.synchronize()
+        for o, w in zip(outs, want):
+            for x, y in zip(o, w):
+                assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+@pytest.mark.parametrize("gates", [2, 3])
+@pytest.mark.parametrize("shape", [(1, 1), (8, 128), (3, 17), (65, 130), (1, 2049)], ids=lambda s: "x".join(map(str, s)))
+def test_step_is_the_scan(shape, gates, dtype):
+    B, C = shape
+    T, dt = 5, DTYPES[dtype]
+    z, h0, _, _ = inputs(B, T, C, gates, dt, seed=47)
+    want = oracle_scan(z, h0, gates == 3)
+    state, ys = h0.cuda(), []
+    for t in range(T):
+        at = state.data_ptr()
+        ys.append(gated_recurrence_step(z.cuda()[:, t], state, output_gate=gates == 3))       # a strided view of the sequence
+        assert state.data_ptr() == at
+    check_scan(dict(y=torch.stack(ys, 1), h_last=state), want, z, h0, gates == 3)
+
+
+def test_step_captured():
+    z, h0, _, _ = inputs(4, 6, 40, 3, torch.float32, seed=53)
+    want = oracle_scan(z, h0, True)
+    zt, state = z[:, 0].cuda(), h0.cuda()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = gated_recurrence_step(zt, state)
+    state.copy_(h0)
+    ys = []
+    for t in range(6):
+        zt.copy_(z[:, t])
+        g.replay()
+        ys.append(y.clone())
+    check_scan(dict(y=torch.stack(ys, 1), h_last=state), want, z, h0, True)
+
+
+def test_offsets_of_the_step_over_32_bits():
+    far = (1 << 31) + 8
+    z, h0, _, _ = inputs(2, 1, 8, 3, torch.bfloat16, seed=59)
+    v = torch.empty(far + 24, dtype=torch.bfloat16, device="cuda").as_strided((2, 24), (far, 1))
+    v.copy_(z[:, 0])
+    a, b = h0.cuda(), h0.cuda()
+    assert torch.equal(gated_recurrence_step(v, a), gated_recurrence_step(z[:, 0].cuda(), b)) and torch.equal(a, b)

@@ -10,8 +10,8 @@ import ctypes as C
 import os
 from typing import Optional
 
-__all__ = ["lib", "WnvError", "check", "Config", "Tensor", "GenerateArgs", "GluConfig", "PostArgs", "ForwardArgs", "MelConfig", "LogmelArgs", "LIB_PATH",
-           "WNV_ABI_VERSION", "DIST", "UPSAMPLE"]
+__all__ = ["lib", "WnvError", "check", "Config", "Tensor", "GenerateArgs", "GluConfig", "PostArgs", "ForwardArgs", "MelConfig", "LogmelArgs", "RecurrenceArgs", "LIB_PATH",
+           "WNV_ABI_VERSION", "DIST", "DTYPE", "UPSAMPLE"]
 
 WNV_ABI_VERSION = 6
 WNV_MAX_UPSAMPLE_STAGES = 8
@@ -22,6 +22,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("WNV_LIB") or os.path.join(_HERE, "libwnv_hip.so")
 TEST_LIB_PATH = os.path.join(_HERE, "libwnv_test.so")
 
+DTYPE = {"float32": 0, "bfloat16": 1, "float16": 2}          # wnv_dtype
 DIST = {"categorical": 0, "Logistic": 1, "Normal": 2}
 UPSAMPLE = {None: 0, "none": 0, "ConvInUpsampleNetwork": 1, "UpsampleNetwork": 2}
 # upsample_activation (upsample.py:30,47-49: getattr(nn, name)(**params)) -> (wnv_upsample_act, the keyword of its one parameter)
@@ -112,6 +113,16 @@ class GluConfig(C.Structure):
                                          "bias")]
 
 
+class RecurrenceArgs(C.Structure):
+    _fields_ = [
+        ("B", C.c_int32), ("C", C.c_int32), ("T", C.c_int64), ("gates", C.c_int32), ("dtype", C.c_int32), ("z", C.c_void_p),
+        ("z_batch_stride", C.c_int64), ("z_time_stride", C.c_int64), ("h0", C.c_void_p), ("h0_batch_stride", C.c_int64),
+        ("lengths", C.c_void_p), ("seg_start", C.c_void_p), ("y", C.c_void_p), ("h_last", C.c_void_p), ("saved", C.c_void_p),
+        ("workspace", C.c_void_p), ("dy", C.c_void_p), ("dy_batch_stride", C.c_int64), ("dy_time_stride", C.c_int64),
+        ("dh_last", C.c_void_p), ("dz", C.c_void_p), ("dh0", C.c_void_p), ("stream", C.c_void_p),
+    ]
+
+
 _PROTOS = {
     # name: (restype, argtypes)
     "wnv_abi_version": (C.c_int32, []),
@@ -150,6 +161,19 @@ _PROTOS = {
     "wnv_mel_frames": (C.c_int64, [C.POINTER(MelConfig), C.c_int64]),
     "wnv_mel_basis": (C.c_int, [C.c_void_p, C.c_void_p]),
     "wnv_logmel": (C.c_int, [C.c_void_p, C.POINTER(LogmelArgs)]),
+    "wnv_recurrence_saved_bytes": (C.c_int64, [C.c_int32, C.c_int64, C.c_int32, C.c_int32, C.c_int32]),
+    "wnv_recurrence_workspace_bytes": (C.c_int64, [C.c_int32, C.c_int64, C.c_int32, C.c_int32, C.c_int32]),
+    "wnv_recurrence_forward": (C.c_int, [C.c_int32, C.POINTER(RecurrenceArgs)]),
+    "wnv_recurrence_backward": (C.c_int, [C.c_int32, C.POINTER(RecurrenceArgs)]),
+    "wnv_recurrence_step": (C.c_int, [C.c_int32, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int32,
+                                      C.c_int32, C.c_void_p]),
+    "wnv_q4_create": (C.c_int, [C.c_int32] * 5 + [C.POINTER(C.c_void_p)]),
+    "wnv_q4_set_codes": (C.c_int, [C.c_void_p] * 6),
+    "wnv_q4_set_weights": (C.c_int, [C.c_void_p] * 4),
+    "wnv_q4_dequantise": (C.c_int, [C.c_void_p] * 3),
+    "wnv_q4_step": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_int32, C.c_int32, C.c_void_p]),
+    "wnv_q4_recurrence_step": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_void_p]),
+    "wnv_q4_destroy": (C.c_int, [C.c_void_p]),
     "wnv_bytes_per_step": (C.c_int64, [C.c_void_p, C.c_int32]),
     "wnv_macs_per_sample": (C.c_int64, [C.c_void_p]),
 }

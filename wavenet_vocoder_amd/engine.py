@@ -1,5 +1,6 @@
 """Thin object wrappers over the C ABI handles (``include/wnv.h``): ``Engine`` (whole network),
-``QueueConv`` (conv.Conv1d.incremental_forward) and ``GluLayer`` (ResidualConv1dGLU.incremental_forward).
+``QueueConv`` (conv.Conv1d.incremental_forward), ``GluLayer`` (ResidualConv1dGLU.incremental_forward) and ``Q4Linear`` (a 1x1
+convolution of one time step with 4-bit weights).
 
 torch is used here for exactly three things: owning device memory (``tensor.data_ptr()``), naming the
 HIP stream to launch on, and moving weights to the host once.  All arithmetic happens in libwnv_hip.so.
@@ -14,7 +15,7 @@ import torch
 from . import _lib
 from ._lib import Config, GenerateArgs, GluConfig, Tensor, check
 
-__all__ = ["Engine", "QueueConv", "GluLayer", "make_config", "require_gpu_tensor", "check_checkpoint"]
+__all__ = ["Engine", "QueueConv", "GluLayer", "Q4Linear", "make_config", "require_gpu_tensor", "check_checkpoint"]
 
 
 def require_gpu_tensor(t: torch.Tensor, what: str) -> None:
@@ -412,5 +413,110 @@ class GluLayer:
         try:
             if self._h.value:
                 _lib.lib().wnv_glu_destroy(self._h)
+        except Exception:
+            pass
+
+
+class Q4Linear:
+    """y = x W^T + bias of a few rows with weights of 4 bits, W[n, k] = scale[n, k / group] (code[n, k] - zero[n, k / group]).
+
+    ``gates`` 2 or 3: the outputs are that many gates of ``cout / gates`` channels, and ``recurrence_step`` hands them to the step of
+    the gated recurrence (``recurrence.gated_recurrence_step``) within the same launch.  Setting the weights waits for the device;
+    after that the handle is only read, on any number of streams at once."""
+
+    _DTYPES = {getattr(torch, name): code for name, code in _lib.DTYPE.items()}
+
+    def __deepcopy__(self, memo):          # (as Engine: the handle stays with the original, the copy builds its own on first use)
+        return None
+
+    def __reduce__(self):
+        return (type(None), ())
+
+    def __init__(self, cin: int, cout: int, device: torch.device, *, group_size: int = 64, gates: int = 1):
+        self._h = C.c_void_p()
+        device = torch.device(device)
+        if device.type != "cuda":
+            raise RuntimeError(f"Q4Linear on {device}: the MI355X engine only runs on a HIP device; there is no CPU fallback")
+        idx = device.index if device.index is not None else torch.cuda.current_device()
+        self.device = torch.device("cuda", idx)
+        self.cin, self.cout, self.group_size, self.gates = int(cin), int(cout), int(group_size), int(gates)
+        check(_lib.lib().wnv_q4_create(self.cin, self.cout, self.gates, self.group_size, idx, C.byref(self._h)))
+        self.channels = self.cout // self.gates
+
+    def _given(self, t: torch.Tensor, what: str, shape, dtype: torch.dtype) -> torch.Tensor:
+        if tuple(t.shape) != tuple(shape):
+            raise ValueError(f"{what} is {tuple(t.shape)}, expected {tuple(shape)}")
+        if t.dtype != dtype:
+            raise TypeError(f"{what} is {t.dtype}, expected {dtype}")
+        return t.detach().to(self.device).contiguous()
+
+    def _bias(self, bias: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+        return None if bias is None else self._given(bias.float(), "bias", (self.cout,), torch.float32)
+
+    def set_weights(self, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> None:
+        """weight (cout, cin) or (cout, cin, 1), any float type: rounded to 4 bits, asymmetric, with bf16 scales."""
+        w = weight.reshape(self.cout, self.cin) if tuple(weight.shape) == (self.cout, self.cin, 1) else weight
+        w, b = self._given(w.float(), "weight", (self.cout, self.cin), torch.float32), self._bias(bias)
+        check(_lib.lib().wnv_q4_set_weights(self._h, w.data_ptr(), _ptr(b), _stream(self.device)))
+
+    def set_codes(self, codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None,
+                  bias: Optional[torch.Tensor] = None) -> None:
+        """Weights that are rounded already: codes (cout, cin) uint8 0..15, scales (cout, groups) bfloat16, zeros (cout, groups) uint8
+        0..15 (None: 8)."""
+        groups = -(-self.cin // self.group_size)
+        q = self._given(codes, "codes", (self.cout, self.cin), torch.uint8)
+        s = self._given(scales, "scales", (self.cout, groups), torch.bfloat16)
+        zp = None if zeros is None else self._given(zeros, "zeros", (self.cout, groups), torch.uint8)
+        b = self._bias(bias)
+        check(_lib.lib().wnv_q4_set_codes(self._h, q.data_ptr(), s.data_ptr(), _ptr(zp), _ptr(b), _stream(self.device)))
+
+    def weight(self) -> torch.Tensor:
+        """W (cout, cin) float32, as the products use it."""
+        w = torch.empty(self.cout, self.cin, device=self.device)
+        check(_lib.lib().wnv_q4_dequantise(self._h, w.data_ptr(), _stream(self.device)))
+        return w
+
+    def _x(self, x: torch.Tensor) -> int:
+        if not x.is_cuda:
+            require_gpu_tensor(x, "x")
+        if x.device != self.device:
+            raise ValueError(f"x lives on {x.device}, the weights on {self.device}")
+        if x.dim() != 2 or x.shape[1] != self.cin or x.shape[0] == 0:
+            raise ValueError(f"x is {tuple(x.shape)}, expected (B, {self.cin})")
+        if torch.is_grad_enabled() and x.requires_grad:
+            raise RuntimeError("4-bit products are not differentiable: use torch.no_grad()")
+        code = self._DTYPES.get(x.dtype)
+        if code is None:
+            raise TypeError(f"x is {x.dtype}: float32, bfloat16 and float16 are implemented")
+        return code
+
+    def step(self, x: torch.Tensor) -> torch.Tensor:
+        """x (B, cin) float32, bfloat16 or float16 -> (B, cout) of the same type."""
+        code = self._x(x)
+        if x.stride(1) != 1:
+            x = x.contiguous()
+        y = torch.empty(x.shape[0], self.cout, device=x.device, dtype=x.dtype)
+        check(_lib.lib().wnv_q4_step(self._h, x.data_ptr(), x.stride(0), y.data_ptr(), x.shape[0], code,
+                                     torch._C._cuda_getCurrentRawStream(self.device.index)))
+        return y
+
+    def recurrence_step(self, x: torch.Tensor, state: torch.Tensor) -> torch.Tensor:
+        """x (B, cin), ``state`` (B, channels) float32 contiguous, updated in place -> y (B, channels) of x's type."""
+        code = self._x(x)
+        if tuple(state.shape) != (x.shape[0], self.channels):
+            raise ValueError(f"state is {tuple(state.shape)}, expected {(x.shape[0], self.channels)}")
+        if state.dtype != torch.float32 or state.device != x.device or not state.is_contiguous():
+            raise ValueError("state is updated in place: it has to be float32, contiguous and on x's device")
+        if x.stride(1) != 1:
+            x = x.contiguous()
+        y = torch.empty(x.shape[0], self.channels, device=x.device, dtype=x.dtype)
+        check(_lib.lib().wnv_q4_recurrence_step(self._h, x.data_ptr(), x.stride(0), state.data_ptr(), y.data_ptr(), x.shape[0], code,
+                                                torch._C._cuda_getCurrentRawStream(self.device.index)))
+        return y
+
+    def __del__(self):  # pragma: no cover
+        try:
+            if self._h.value:
+                _lib.lib().wnv_q4_destroy(self._h)
         except Exception:
             pass

@@ -1,0 +1,170 @@
+"""The gated linear recurrence: the scan over a sequence, with its gradients, and the step of one sample.
+
+    z = (f | v | o) along the channels
+    h_t = sigmoid(f_t) h_{t-1} + (1 - sigmoid(f_t)) v_t        y_t = h_t sigmoid(o_t)        (no output gate: y = h)
+
+The recurrent counterpart of the gated convolution of ``modules.ResidualConv1dGLU`` (reference modules.py:112-169): its whole past is
+one state of C float32 numbers instead of a history ring.  All arithmetic happens in libwnv_hip.so (``wnv_recurrence_*`` in
+include/wnv.h); there is no CPU path.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional, Tuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from ._lib import DTYPE, RecurrenceArgs, check
+from .engine import require_gpu_tensor
+
+__all__ = ["gated_recurrence", "gated_recurrence_step"]
+
+_DTYPES = {getattr(torch, name): code for name, code in DTYPE.items()}
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _dtype(z: torch.Tensor) -> int:
+    code = _DTYPES.get(z.dtype)
+    if code is None:
+        raise TypeError(f"z is {z.dtype}: float32, bfloat16 and float16 are implemented")
+    return code
+
+
+def _channels(z: torch.Tensor, gates: int) -> int:
+    if z.shape[-1] == 0 or z.shape[-1] % gates:
+        raise ValueError(f"z has {z.shape[-1]} channels, which are not {gates} gates of the same size")
+    return z.shape[-1] // gates
+
+
+def _state(h: torch.Tensor, name: str, B: int, n: int, z: torch.Tensor) -> torch.Tensor:
+    if tuple(h.shape) != (B, n):
+        raise ValueError(f"{name} is {tuple(h.shape)}, expected {(B, n)}")
+    if h.dtype != torch.float32:
+        raise TypeError(f"{name} is {h.dtype}: the state is float32")
+    if h.device != z.device:
+        raise ValueError(f"{name} lives on {h.device}, z on {z.device}")
+    return h
+
+
+def _map(m: Optional[torch.Tensor], name: str, shape: Tuple[int, ...], z: torch.Tensor) -> Optional[torch.Tensor]:
+    if m is None:
+        return None
+    if tuple(m.shape) != shape:
+        raise ValueError(f"{name} is {tuple(m.shape)}, expected {shape}")
+    if m.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"{name} is {m.dtype}: int32 or int64")
+    if m.device != z.device:
+        raise ValueError(f"{name} lives on {m.device}, z on {z.device}")
+    if m.dtype == torch.int64:
+        m = m.clamp(-1, 2 ** 31 - 1).to(torch.int32)
+    return m.contiguous()
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """``t`` with its last dimension contiguous (a copy only where it is not: any batch and time stride is taken, 0 too)."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _call(fn, z, gates, h0, lengths, seg_start, *, y=None, h_last=None, saved=None, dy=None, dh_last=None, dz=None, dh0=None):
+    B, T, n = z.shape[0], z.shape[1], z.shape[2] // gates
+    code = _DTYPES[z.dtype]
+    dev = z.device.index
+    ws = None
+    nbytes = _lib.lib().wnv_recurrence_workspace_bytes(B, T, n, gates, code)
+    if nbytes > 0:          # of the stream that runs the call: torch's allocator hands it out again behind the call's own work only
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=z.device)
+    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    a = RecurrenceArgs(B, n, T, gates, code, z.data_ptr(), z.stride(0), z.stride(1), ptr(h0), 0 if h0 is None else h0.stride(0),
+                       ptr(lengths), ptr(seg_start), ptr(y), ptr(h_last), ptr(saved), ptr(ws), ptr(dy),
+                       0 if dy is None else dy.stride(0), 0 if dy is None else dy.stride(1), ptr(dh_last), ptr(dz), ptr(dh0),
+                       _raw_stream(dev))
+    check(fn(dev, C.byref(a)))
+
+
+def _forward(z, h0, gates, lengths, seg_start, keep: bool):
+    B, T, n = z.shape[0], z.shape[1], z.shape[2] // gates
+    y = torch.empty(B, T, n, dtype=z.dtype, device=z.device)
+    h_last = torch.empty(B, n, dtype=torch.float32, device=z.device)
+    saved = None
+    if keep:
+        nbytes = _lib.lib().wnv_recurrence_saved_bytes(B, T, n, gates, _DTYPES[z.dtype])
+        saved = torch.empty(nbytes, dtype=torch.uint8, device=z.device)
+    _call(_lib.lib().wnv_recurrence_forward, z, gates, h0, lengths, seg_start, y=y, h_last=h_last, saved=saved)
+    return y, h_last, saved
+
+
+class _GatedRecurrence(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, z, h0, gates, lengths, seg_start):
+        ctx.set_materialize_grads(False)
+        y, h_last, saved = _forward(z, h0, gates, lengths, seg_start, True)
+        ctx.gates, ctx.optional = gates, (h0 is not None, lengths is not None, seg_start is not None)
+        ctx.save_for_backward(z, saved, *(t for t in (h0, lengths, seg_start) if t is not None))
+        return y, h_last
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dh_last):
+        z, saved, *rest = ctx.saved_tensors
+        h0, lengths, seg_start = ((rest.pop(0) if there else None) for there in ctx.optional)
+        dz = torch.empty(z.shape, dtype=z.dtype, device=z.device)
+        dh0 = torch.empty(h0.shape, dtype=torch.float32, device=z.device) if h0 is not None and ctx.needs_input_grad[1] else None
+        dy = None if dy is None else _rows(dy)
+        dh_last = None if dh_last is None else dh_last.contiguous()
+        _call(_lib.lib().wnv_recurrence_backward, z, ctx.gates, h0, lengths, seg_start, saved=saved, dy=dy, dh_last=dh_last, dz=dz, dh0=dh0)
+        return (dz if ctx.needs_input_grad[0] else None), dh0, None, None, None
+
+
+def gated_recurrence(z: torch.Tensor, h0: Optional[torch.Tensor] = None, *, output_gate: bool = True,
+                     lengths: Optional[torch.Tensor] = None, seg_start: Optional[torch.Tensor] = None
+                     ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """z (B, T, 3 C) -> y (B, T, C) of z's type and the state behind the last step (B, C) float32; ``output_gate=False``: z (B, T, 2 C).
+
+    ``h0`` (B, C) float32: the state before the first step (zeros).  ``lengths`` (B,): rows of a padded batch end there -- behind it z
+    is not looked at, y and the gradients are zero, and the state is handed on (an empty row's is ``h0``).  ``seg_start`` (B, T): the
+    map of a packed slot (``wnv_generate_args``) -- the state reads as zero at each step t with ``seg_start[b, t] == t``; a negative
+    entry is an utterance begun before this call, which goes on from ``h0``.  Differentiable (once) in z and h0.  Runs on the current
+    stream of z's device and is capturable; the same call gives the same bits."""
+    require_gpu_tensor(z, "z")
+    if z.dim() != 3:
+        raise ValueError(f"z is {tuple(z.shape)}, expected (B, T, channels)")
+    _dtype(z)
+    gates = 3 if output_gate else 2
+    B, T = z.shape[0], z.shape[1]
+    n = _channels(z, gates)
+    if B == 0 or T == 0:
+        raise ValueError(f"z is {tuple(z.shape)}: an empty batch or sequence")
+    if h0 is not None:
+        h0 = _rows(_state(h0, "h0", B, n, z))
+    lengths = _map(lengths, "lengths", (B,), z)
+    seg_start = _map(seg_start, "seg_start", (B, T), z)
+    z = _rows(z)
+    if torch.is_grad_enabled() and (z.requires_grad or (h0 is not None and h0.requires_grad)):
+        return _GatedRecurrence.apply(z, h0, gates, lengths, seg_start)
+    y, h_last, _ = _forward(z, h0, gates, lengths, seg_start, False)
+    return y, h_last
+
+
+def gated_recurrence_step(z: torch.Tensor, state: torch.Tensor, *, output_gate: bool = True) -> torch.Tensor:
+    """One step: z (B, 3 C) (``output_gate=False``: (B, 2 C)), ``state`` (B, C) float32 contiguous, updated in place -> y (B, C) of z's
+    type.  Not differentiable: the training form is ``gated_recurrence``."""
+    require_gpu_tensor(z, "z")
+    if z.dim() != 2:
+        raise ValueError(f"z is {tuple(z.shape)}, expected (B, channels)")
+    code = _dtype(z)
+    gates = 3 if output_gate else 2
+    B, n = z.shape[0], _channels(z, gates)
+    if B == 0:
+        raise ValueError("z is an empty batch")
+    if not _state(state, "state", B, n, z).is_contiguous():
+        raise ValueError("state is updated in place: it has to be contiguous")
+    if torch.is_grad_enabled() and (z.requires_grad or state.requires_grad):
+        raise RuntimeError("gated_recurrence_step is not differentiable: use gated_recurrence, or torch.no_grad()")
+    z = _rows(z)
+    y = torch.empty(B, n, dtype=z.dtype, device=z.device)
+    dev = z.device.index
+    check(_lib.lib().wnv_recurrence_step(dev, z.data_ptr(), z.stride(0), state.data_ptr(), y.data_ptr(), B, n, gates, code,
+                                         _raw_stream(dev)))
+    return y
