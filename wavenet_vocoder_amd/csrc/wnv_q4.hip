@@ -193,7 +193,8 @@ extern "C" wnv_status wnv_q4_create(int32_t cin, int32_t cout, int32_t gates, in
         return fail(WNV_ERR_INVALID_ARG, "wnv_q4_create: bad geometry (cin %d, cout %d, gates %d)", cin, cout, gates);
     if (group != 32 && group != 64 && group != 128)
         return fail(WNV_ERR_UNSUPPORTED, "wnv_q4_create: groups of %d inputs (32, 64 and 128 are implemented)", group);
-    if (cin > (1 << 20) || cout > (1 << 20)) return fail(WNV_ERR_UNSUPPORTED, "wnv_q4_create: at most 2^20 inputs and outputs");
+    if (cin > (1 << 20) || cout > (1 << 20) || (int64_t)cin * cout > INT32_MAX)
+        return fail(WNV_ERR_UNSUPPORTED, "wnv_q4_create: at most 2^20 inputs, 2^20 outputs and 2^31 - 1 weights");
     wnv_q4* h = new wnv_q4();
     h->device = device;
     Q4Dev& q = h->q;

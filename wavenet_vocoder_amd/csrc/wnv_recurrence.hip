@@ -15,15 +15,16 @@
 namespace {
 
 struct RecArgs {
-    int B, C, gates;
-    long long T, zb, zt;            // batch and time stride of z, in elements
+    int B, C, T, tiles, chunks;     // tiles of the channels, chunks of the time
+    long long zb, zt;               // batch and time stride of z, in elements
     long long h0b;
     const void* z;
     const float* h0;
     const int *lengths, *seg_start;
     void* y;
     float* h_last;
-    float* saved;                   // (B, T, C) states, for the backward pass
+    float* saved;                   // [row][chunk of the backward pass][tile width]: the state before the chunk's first step
+    unsigned long long* slots;      // workspace: a counter in 256 bytes of its own, then each row's maps
     const void* dy;
     long long dyb, dyt;
     const float* dh_last;
@@ -31,75 +32,405 @@ struct RecArgs {
     float* dh0;
 };
 
-constexpr int RT = 64;
+// ---- maps of the state --------------------------------------------------------------------------------------------------------
+// A stretch of steps maps the state before it to the state behind it: h -> h + (b - u h), with 1 - u the product of its gates; u < 0
+// says that the state behind it is b whatever stood before.  The backward pass maps what flows back by the same form.
+struct Map { float u, b; };
 
-template <typename E>
-__global__ void __launch_bounds__(RT) wnv_recurrence_fwd(RecArgs a) {
-    const int c = blockIdx.x * RT + threadIdx.x, b = blockIdx.y;
-    if (c >= a.C) return;
-    const E* z = (const E*)a.z + (long long)b * a.zb + c;
-    E* y = (E*)a.y + (long long)b * a.T * a.C + c;
-    const long long n = a.lengths ? min((long long)a.lengths[b], a.T) : a.T;
-    float h = a.h0 ? a.h0[(long long)b * a.h0b + c] : 0.f;
-    for (long long t = 0; t < a.T; ++t) {
-        float out = 0.f;
-        if (t < n) {
-            float keep, u;
-            wnv_gate(wnv_up(z[t * a.zt]), keep, u);
-            if (a.seg_start && a.seg_start[(long long)b * a.T + t] == t) h = 0.f;
-            h = fmaf(u, wnv_up(z[t * a.zt + a.C]) - h, h);
-            out = h;
-            if (a.gates == 3) {
-                float so, uo;
-                wnv_gate(wnv_up(z[t * a.zt + 2 * a.C]), so, uo);
-                out = h * so;
-            }
-        }
-        y[t * a.C] = wnv_down<E>(out);
-        if (a.saved) a.saved[((long long)b * a.T + t) * a.C + c] = h;
-    }
-    a.h_last[(long long)b * a.C + c] = h;
+__device__ __forceinline__ float apply(Map m, float h) { return m.u < 0.f ? m.b : h + fmaf(-m.u, h, m.b); }
+__device__ __forceinline__ Map join(Map first, Map then) {
+    Map r;
+    r.u = then.u < 0.f || first.u < 0.f ? -1.f : fmaf(-first.u, then.u, first.u + then.u);
+    r.b = apply(then, first.b);
+    return r;
 }
 
-// g_t = dy_t sigmoid(o_t);  dh_t = g_t + (what step t+1 hands back);  hands back dh_t sigmoid(f_t), nothing over a beginning
+// A map is handed to the other workgroups as one 8-byte store that carries its own "valid": the workspace is filled with ones, and u
+// is never that pattern (a NaN is rewritten to the usual one).  No fence is needed: nothing else is read on the strength of it.
+constexpr unsigned EMPTY = 0xffffffffu;
+__device__ __forceinline__ void publish(unsigned long long* slot, Map m) {
+    const unsigned u = m.u != m.u ? 0x7fc00000u : __float_as_uint(m.u);
+    __hip_atomic_store(slot, ((unsigned long long)__float_as_uint(m.b) << 32) | u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ unsigned long long peek(const unsigned long long* slot) {
+    return __hip_atomic_load(slot, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// The wait ends: a workgroup draws its chunk from a counter, so the chunks before that of one that runs have all been started, and
+// the lowest of them waits for nobody.  Should a slot stay empty for some seconds all the same, its map is NaN: the launch ends, and
+// says so in its results.
+__device__ __forceinline__ Map taken(const unsigned long long* slot, unsigned long long v) {
+    for (int tries = 0; (unsigned)v == EMPTY; ++tries) {
+        if (tries > (1 << 22)) return {__uint_as_float(0x7fc00000u), __uint_as_float(0x7fc00000u)};
+        __builtin_amdgcn_s_sleep(1);
+        v = peek(slot);
+    }
+    return {__uint_as_float((unsigned)v), __uint_as_float((unsigned)(v >> 32))};
+}
+
+// How a chunk learns the state before it, without a chain through all chunks and in one order of arithmetic whatever the timing:
+// 16 chunks are a group, 16 groups a section.  Every chunk hands out its map; the last one of a group joins the 16 and hands out the
+// group's; the last one of a section hands out the state behind it.  A chunk takes the section's state, runs it through the maps
+// of the groups before its own and of the chunks before it in its group: two waits behind its own loads for 256 chunks (32768 steps
+// forward), and one more for each further section.
+constexpr int GROUP = 16;
+struct Slots {                      // of one row of tiles, a thread's own channel
+    unsigned long long *chunk, *group, *section;
+};
+__device__ __forceinline__ long long slots_of_row(int chunks, int W) {
+    return (long long)W * (chunks + chunks / GROUP + chunks / (GROUP * GROUP));
+}
+__device__ __forceinline__ Slots slots_at(unsigned long long* all, int row, int chunks, int W, int ch) {
+    unsigned long long* p = all + 32 + row * slots_of_row(chunks, W) + ch;
+    return {p, p + (long long)W * chunks, p + (long long)W * (chunks + chunks / GROUP)};
+}
+
+// Joins `own` to what stands before it in the group of chunk k (counted in the order in which the chunks are drawn) and hands out what
+// others wait for; `before`: the maps, still to be applied.
+template <int W>
+__device__ __forceinline__ int maps_in_group(const Slots& s, int k, int chunks, Map own, Map (&before)[GROUP - 1]) {
+    const int at = k % GROUP;
+    const bool more = k + 1 < chunks, last = at == GROUP - 1;
+    if (more && !last) publish(s.chunk + (long long)k * W, own);
+    unsigned long long v[GROUP - 1];
+#pragma unroll
+    for (int i = 0; i < GROUP - 1; ++i)
+        if (i < at) v[i] = peek(s.chunk + (long long)(k - at + i) * W);
+    Map all{0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < GROUP - 1; ++i)
+        if (i < at) {
+            before[i] = taken(s.chunk + (long long)(k - at + i) * W, v[i]);
+            all = join(all, before[i]);
+        }
+    if (more && last && k / GROUP % GROUP != GROUP - 1) publish(s.group + (long long)(k / GROUP) * W, join(all, own));
+    return at;
+}
+// The state before the group of chunk k; `first` before chunk 0.
+template <int W> __device__ __forceinline__ float state_before_group(const Slots& s, int k, float first) {
+    const int section = k / (GROUP * GROUP), g0 = section * GROUP, n = k / GROUP - g0;
+    unsigned long long v[GROUP - 1];
+#pragma unroll
+    for (int i = 0; i < GROUP - 1; ++i)
+        if (i < n) v[i] = peek(s.group + (long long)(g0 + i) * W);
+    float h = first;
+    if (section) {
+        const unsigned long long* at = s.section + (long long)(section - 1) * W;
+        h = taken(at, peek(at)).b;
+    }
+#pragma unroll
+    for (int i = 0; i < GROUP - 1; ++i)
+        if (i < n) h = apply(taken(s.group + (long long)(g0 + i) * W, v[i]), h);
+    return h;
+}
+template <int W> __device__ __forceinline__ void state_behind(const Slots& s, int k, int chunks, float h) {
+    if ((k + 1) % (GROUP * GROUP) == 0 && k + 1 < chunks) publish(s.section + (long long)(k / (GROUP * GROUP)) * W, {-1.f, h});
+}
+
+// ---- the shape of a workgroup -------------------------------------------------------------------------------------------------
+// 256 threads = 16 lanes along the channels x 16 stretches of L steps.  A lane holds V channels, so that a row of a tile is 64
+// channels: 128 bytes of a 16-bit type, 256 of float32.  The last lane of a row that is no multiple of V starts earlier and shares
+// channels with its neighbour (both compute and write the same); V = 1 is for rows narrower than 4.
+constexpr int THREADS = 256, LANES = 16, STRETCHES = THREADS / LANES;
+constexpr int FWD_L = 8, BWD_L = 4;
+
+template <typename E, int V> struct Vec { E e[V]; };
+template <typename E, int V> __device__ __forceinline__ Vec<E, V> load(const E* p) {      // at any alignment
+    Vec<E, V> v;
+    __builtin_memcpy(&v, p, sizeof v);
+    return v;
+}
+template <typename E, int V> __device__ __forceinline__ void store(E* p, const Vec<E, V>& v) { __builtin_memcpy(p, &v, sizeof v); }
+
+struct Place { int b, tile, chunk, row; };
+
+// Chunks are drawn from a counter, all rows' first ones first: the order that the waits rely on.
+template <bool BACK> __device__ __forceinline__ Place draw_place(const RecArgs& a) {
+    __shared__ int drawn;
+    int i = blockIdx.x;
+    if (a.chunks > 1) {
+        if (threadIdx.x == 0) drawn = atomicAdd((int*)a.slots, 1) + 1;      // filled with ones: it starts at -1
+        __syncthreads();
+        i = drawn;
+    }
+    const int rows = a.B * a.tiles;
+    Place p;
+    p.row = i % rows;
+    p.chunk = i / rows;
+    if (BACK) p.chunk = a.chunks - 1 - p.chunk;
+    p.b = p.row / a.tiles;
+    p.tile = p.row % a.tiles;
+    return p;
+}
+
+// What stands in a thread's stretch: live steps from its first, and which of them begin an utterance.
+struct Stretch { int t0, live, begins; };
+template <int L> __device__ __forceinline__ Stretch stretch_of(const RecArgs& a, int b, int t0) {
+    Stretch s{t0, 0, 0};
+    const int n = a.lengths ? min(a.lengths[b], a.T) : a.T;
+    s.live = max(0, min(L, n - t0));
+    if (a.seg_start) {
+        const int* m = a.seg_start + (long long)b * a.T;
+#pragma unroll
+        for (int l = 0; l < L; ++l)
+            if (l < s.live && m[t0 + l] == t0 + l) s.begins |= 1 << l;
+    }
+    return s;
+}
+
+// One chunk of one tile.  Each thread reduces its stretch to a map, 64 threads (one a channel) join the stretches' maps, find the
+// state before the chunk and walk it through, and each thread runs over its stretch again, out of its registers.  z is read once.
+template <typename E, int G, int V>
+__global__ void __launch_bounds__(THREADS) wnv_recurrence_fwd(RecArgs a) {
+    constexpr int L = FWD_L, W = LANES * V;
+    __shared__ Map maps[STRETCHES][W];
+    __shared__ float starts[STRETCHES][W], base[W];
+    const int tid = threadIdx.x, lane = tid % LANES, st = tid / LANES;
+    const Place p = draw_place<false>(a);
+    const int first = p.tile * W + lane * V;
+    const bool on = first < a.C;
+    const int c = min(first, a.C - V);
+    const Stretch s = stretch_of<L>(a, p.b, p.chunk * (STRETCHES * L) + st * L);
+    const int live = on ? s.live : 0;
+    const E* z = (const E*)a.z + (long long)p.b * a.zb + (long long)s.t0 * a.zt + c;
+
+    Vec<E, V> f[L], v[L], o[L];
+#pragma unroll
+    for (int l = 0; l < L; ++l)
+        if (l < live) {
+            f[l] = load<E, V>(z + l * a.zt);
+            v[l] = load<E, V>(z + l * a.zt + a.C);
+            if (G == 3) o[l] = load<E, V>(z + l * a.zt + 2 * a.C);
+        }
+    float u[L][V];
+    Map m[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) m[i] = {0.f, 0.f};
+#pragma unroll
+    for (int l = 0; l < L; ++l)
+        if (l < live) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                float keep;
+                wnv_gate(wnv_up(f[l].e[i]), keep, u[l][i]);
+                if (s.begins >> l & 1) m[i].b = 0.f;
+                m[i].u = fmaf(-u[l][i], m[i].u, m[i].u + u[l][i]);
+                m[i].b = fmaf(u[l][i], wnv_up(v[l].e[i]) - m[i].b, m[i].b);
+            }
+        }
+#pragma unroll
+    for (int i = 0; i < V; ++i) maps[st][lane * V + i] = {s.begins ? -1.f : m[i].u, m[i].b};
+    __syncthreads();
+
+    // wave 0: the chunk's map, and the chunks of its group; wave 1: what stands before the group
+    const int wave = tid / 64, ch = tid % 64, chan = min(p.tile * W + ch / V * V, a.C - V) + ch % V;
+    const bool there = ch < W && p.tile * W + ch / V * V < a.C;
+    const Slots slots = slots_at(a.slots, p.row, a.chunks, W, ch);
+    Map before[GROUP - 1];
+    int n = 0;
+    if (wave == 0 && ch < W) {
+        Map all{0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < STRETCHES; ++k) all = join(all, maps[k][ch]);
+        n = maps_in_group<W>(slots, p.chunk, a.chunks, all, before);
+    } else if (wave == 1 && ch < W) {
+        base[ch] = state_before_group<W>(slots, p.chunk, a.h0 && there ? a.h0[p.b * a.h0b + chan] : 0.f);
+    }
+    __syncthreads();
+    if (wave == 0 && ch < W) {
+        float h = base[ch];
+#pragma unroll
+        for (int i = 0; i < GROUP - 1; ++i)
+            if (i < n) h = apply(before[i], h);
+        constexpr int EVERY = BWD_L * STRETCHES / L;        // stretches between two states that the backward pass starts from
+        const int saves = (a.T + BWD_L * STRETCHES - 1) / (BWD_L * STRETCHES), left = (a.T - p.chunk * (STRETCHES * L) + L - 1) / L;
+        float* save = a.saved ? a.saved + ((long long)p.row * saves + p.chunk * (STRETCHES / EVERY)) * W + ch : nullptr;
+#pragma unroll
+        for (int k = 0; k < STRETCHES; ++k) {
+            starts[k][ch] = h;
+            if (k % EVERY == 0 && save && k < left) save[k / EVERY * W] = h;
+            h = apply(maps[k][ch], h);
+        }
+        state_behind<W>(slots, p.chunk, a.chunks, h);
+        if (p.chunk + 1 == a.chunks && there) a.h_last[(long long)p.b * a.C + chan] = h;
+    }
+    __syncthreads();
+
+    float h[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) h[i] = starts[st][lane * V + i];
+    E* y = (E*)a.y + ((long long)p.b * a.T + s.t0) * a.C + c;
+#pragma unroll
+    for (int l = 0; l < L; ++l)
+        if (on && s.t0 + l < a.T) {
+            Vec<E, V> out;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                float q = 0.f;
+                if (l < live) {
+                    if (s.begins >> l & 1) h[i] = 0.f;
+                    h[i] = fmaf(u[l][i], wnv_up(v[l].e[i]) - h[i], h[i]);
+                    q = h[i];
+                    if (G == 3) {
+                        float so, uo;
+                        wnv_gate(wnv_up(o[l].e[i]), so, uo);
+                        q *= so;
+                    }
+                }
+                out.e[i] = wnv_down<E>(q);
+            }
+            store<E, V>(y + (long long)l * a.C, out);
+        }
+}
+
+// g_t = dy_t sigmoid(o_t);  dh_t = g_t + (what step t+1 hands back);  hands back r = dh_t - u_t dh_t, nothing over a beginning
 // df = dh (h_{t-1} - v) sigmoid(f) u;  dv = dh u;  do = dy h sigmoid(o) (1 - sigmoid(o))
-template <typename E>
-__global__ void __launch_bounds__(RT) wnv_recurrence_bwd(RecArgs a) {
-    const int c = blockIdx.x * RT + threadIdx.x, b = blockIdx.y;
-    if (c >= a.C) return;
-    const E* z = (const E*)a.z + (long long)b * a.zb + c;
-    const E* dy = a.dy ? (const E*)a.dy + (long long)b * a.dyb + c : nullptr;
-    E* dz = (E*)a.dz + (long long)b * a.T * a.gates * a.C + c;
-    const float* hs = a.saved + (long long)b * a.T * a.C + c;
-    const long long n = a.lengths ? min((long long)a.lengths[b], a.T) : a.T;
-    float r = a.dh_last ? a.dh_last[(long long)b * a.C + c] : 0.f;
-    const float h0 = a.h0 ? a.h0[(long long)b * a.h0b + c] : 0.f;
-    for (long long t = a.T - 1; t >= 0; --t) {
-        float df = 0.f, dv = 0.f, dgo = 0.f;
-        if (t < n) {
-            float keep, u;
-            wnv_gate(wnv_up(z[t * a.zt]), keep, u);
-            const bool begins = a.seg_start && a.seg_start[(long long)b * a.T + t] == t;
-            const float before = begins ? 0.f : t ? hs[(t - 1) * a.C] : h0, v = wnv_up(z[t * a.zt + a.C]);
-            float g = dy ? wnv_up(dy[t * a.dyt]) : 0.f;
-            if (a.gates == 3) {
-                float so, uo;
-                wnv_gate(wnv_up(z[t * a.zt + 2 * a.C]), so, uo);
-                dgo = g * hs[t * a.C] * so * uo;
-                g *= so;
-            }
-            const float dh = g + r;
-            df = dh * (before - v) * keep * u;
-            dv = dh * u;
-            r = begins ? 0.f : fmaf(-u, dh, dh);
+// The chunks run from the last to the first, r is found the way the forward pass finds h; h itself starts from the state that the
+// forward pass saved before each chunk and is run through again.
+template <typename E, int G, int V>
+__global__ void __launch_bounds__(THREADS) wnv_recurrence_bwd(RecArgs a) {
+    constexpr int L = BWD_L, W = LANES * V;
+    __shared__ Map ahead[STRETCHES][W], back[STRETCHES][W];         // of h and of r
+    __shared__ float hs[STRETCHES][W], rs[STRETCHES][W], base[W];
+    const int tid = threadIdx.x, lane = tid % LANES, st = tid / LANES;
+    const Place p = draw_place<true>(a);
+    const int first = p.tile * W + lane * V;
+    const bool on = first < a.C;
+    const int c = min(first, a.C - V);
+    const Stretch s = stretch_of<L>(a, p.b, p.chunk * (STRETCHES * L) + st * L);
+    const int live = on ? s.live : 0;
+    const E* z = (const E*)a.z + (long long)p.b * a.zb + (long long)s.t0 * a.zt + c;
+    const E* dy = (const E*)a.dy + (long long)p.b * a.dyb + (long long)s.t0 * a.dyt + c;
+
+    Vec<E, V> f[L], v[L], o[L], d[L];
+#pragma unroll
+    for (int l = 0; l < L; ++l)
+        if (l < live) {
+            f[l] = load<E, V>(z + l * a.zt);
+            v[l] = load<E, V>(z + l * a.zt + a.C);
+            if (G == 3) o[l] = load<E, V>(z + l * a.zt + 2 * a.C);
+            if (a.dy) d[l] = load<E, V>(dy + l * a.dyt);
         }
-        E* d = dz + t * a.gates * a.C;
-        d[0] = wnv_down<E>(df);
-        d[a.C] = wnv_down<E>(dv);
-        if (a.gates == 3) d[2 * a.C] = wnv_down<E>(dgo);
+    float u[L][V], uk[L][V], g[L][V], q[L][V];          // u sigmoid(f); dy sigmoid(o); dy sigmoid(o) (1 - sigmoid(o))
+    Map m[V], r[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) m[i] = r[i] = {0.f, 0.f};
+#pragma unroll
+    for (int l = 0; l < L; ++l)
+        if (l < live) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                float keep;
+                wnv_gate(wnv_up(f[l].e[i]), keep, u[l][i]);
+                uk[l][i] = u[l][i] * keep;
+                if (s.begins >> l & 1) m[i].b = 0.f;
+                m[i].u = fmaf(-u[l][i], m[i].u, m[i].u + u[l][i]);
+                m[i].b = fmaf(u[l][i], wnv_up(v[l].e[i]) - m[i].b, m[i].b);
+                g[l][i] = a.dy ? wnv_up(d[l].e[i]) : 0.f;
+                if (G == 3) {
+                    float so, uo;
+                    wnv_gate(wnv_up(o[l].e[i]), so, uo);
+                    g[l][i] *= so;
+                    q[l][i] = g[l][i] * uo;
+                }
+            }
+        }
+#pragma unroll
+    for (int l = L - 1; l >= 0; --l)
+        if (l < live) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float dh = g[l][i] + r[i].b;
+                r[i].b = s.begins >> l & 1 ? 0.f : fmaf(-u[l][i], dh, dh);
+            }
+        }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        ahead[st][lane * V + i] = {s.begins ? -1.f : m[i].u, m[i].b};
+        back[st][lane * V + i] = {s.begins ? -1.f : m[i].u, r[i].b};
     }
-    if (a.dh0) a.dh0[(long long)b * a.C + c] = r;
+    __syncthreads();
+
+    // waves 0 and 1 as in the forward pass, on the chunks from behind; wave 2: h through the chunk
+    const int wave = tid / 64, ch = tid % 64, chan = min(p.tile * W + ch / V * V, a.C - V) + ch % V, order = a.chunks - 1 - p.chunk;
+    const bool there = ch < W && p.tile * W + ch / V * V < a.C;
+    const Slots slots = slots_at(a.slots, p.row, a.chunks, W, ch);
+    Map behind[GROUP - 1];
+    int n = 0;
+    if (wave == 0 && ch < W) {
+        Map all{0.f, 0.f};
+#pragma unroll
+        for (int k = STRETCHES - 1; k >= 0; --k) all = join(all, back[k][ch]);
+        n = maps_in_group<W>(slots, order, a.chunks, all, behind);
+    } else if (wave == 1 && ch < W) {
+        base[ch] = state_before_group<W>(slots, order, a.dh_last && there ? a.dh_last[(long long)p.b * a.C + chan] : 0.f);
+    } else if (wave == 2 && ch < W) {
+        float h = a.saved[((long long)p.row * a.chunks + p.chunk) * W + ch];
+#pragma unroll
+        for (int k = 0; k < STRETCHES; ++k) {
+            hs[k][ch] = h;
+            h = apply(ahead[k][ch], h);
+        }
+    }
+    __syncthreads();
+    if (wave == 0 && ch < W) {
+        float x = base[ch];
+#pragma unroll
+        for (int i = 0; i < GROUP - 1; ++i)
+            if (i < n) x = apply(behind[i], x);
+#pragma unroll
+        for (int k = STRETCHES - 1; k >= 0; --k) {
+            rs[k][ch] = x;
+            x = apply(back[k][ch], x);
+        }
+        state_behind<W>(slots, order, a.chunks, x);
+        if (p.chunk == 0 && a.dh0 && there) a.dh0[(long long)p.b * a.C + chan] = x;
+    }
+    __syncthreads();
+
+    float before[L][V], x[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        float h = hs[st][lane * V + i];
+        x[i] = rs[st][lane * V + i];
+#pragma unroll
+        for (int l = 0; l < L; ++l)
+            if (l < live) {
+                before[l][i] = s.begins >> l & 1 ? 0.f : h;
+                h = fmaf(u[l][i], wnv_up(v[l].e[i]) - before[l][i], before[l][i]);
+            }
+    }
+    E* dz = (E*)a.dz + ((long long)p.b * a.T + s.t0) * (G * (long long)a.C) + c;
+#pragma unroll
+    for (int l = L - 1; l >= 0; --l)
+        if (on && s.t0 + l < a.T) {
+            Vec<E, V> df, dv, dg;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                float xf = 0.f, xv = 0.f, xo = 0.f;
+                if (l < live) {
+                    const float w = wnv_up(v[l].e[i]) - before[l][i], dh = g[l][i] + x[i];
+                    xf = -dh * w * uk[l][i];
+                    xv = dh * u[l][i];
+                    if (G == 3) xo = q[l][i] * fmaf(u[l][i], w, before[l][i]);
+                    x[i] = s.begins >> l & 1 ? 0.f : fmaf(-u[l][i], dh, dh);
+                }
+                df.e[i] = wnv_down<E>(xf);
+                dv.e[i] = wnv_down<E>(xv);
+                dg.e[i] = wnv_down<E>(xo);
+            }
+            E* to = dz + (long long)l * G * a.C;
+            store<E, V>(to, df);
+            store<E, V>(to + a.C, dv);
+            if (G == 3) store<E, V>(to + 2 * (long long)a.C, dg);
+        }
 }
+
+__global__ void __launch_bounds__(256) wnv_recurrence_fill(uint4* p, long long n) {
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i < n) p[i] = uint4{EMPTY, EMPTY, EMPTY, EMPTY};
+}
+
+constexpr int RT = 64;
 
 template <typename E>
 __global__ void __launch_bounds__(RT) wnv_recurrence_one(const E* z, long long zb, float* state, E* y, int C, int gates) {
@@ -128,7 +459,7 @@ __global__ void __launch_bounds__(RT) wnv_recurrence_one(const E* z, long long z
 wnv_status check_shape(const char* who, int device, int64_t B, int64_t T, int64_t C, int gates, int dtype) {
     if (device < 0) return fail(WNV_ERR_INVALID_ARG, "%s: device must be >= 0", who);
     if (B <= 0 || T <= 0 || C <= 0) return fail(WNV_ERR_INVALID_ARG, "%s: B, T and C must be positive", who);
-    if (T > INT32_MAX) return fail(WNV_ERR_UNSUPPORTED, "%s: at most 2^31 - 1 steps", who);
+    if (T > (1 << 30)) return fail(WNV_ERR_UNSUPPORTED, "%s: at most 2^30 steps", who);
     if (B > 65535 || C > (1 << 20)) return fail(WNV_ERR_UNSUPPORTED, "%s: at most 65535 rows and 2^20 channels", who);
     if (gates != 2 && gates != 3) return fail(WNV_ERR_INVALID_ARG, "%s: gates must be 2 (f, v) or 3 (f, v, o)", who);
     if (!wnv_dtype_size(dtype)) return fail(WNV_ERR_INVALID_ARG, "%s: unknown dtype %d", who, dtype);
@@ -147,28 +478,57 @@ wnv_status check_strides(const char* who, const wnv_recurrence_args* a) {
     return WNV_OK;
 }
 
-RecArgs device_args(const wnv_recurrence_args* a) {
-    RecArgs k{};
-    k.B = a->B; k.C = a->C; k.gates = a->gates; k.T = a->T;
+int width_of(int C) { return C < 4 ? LANES : LANES * 4; }
+int chunks_of(int64_t T, int L) { return (int)((T + STRETCHES * L - 1) / (STRETCHES * L)); }
+int64_t slot_bytes(int64_t B, int64_t T, int C, int L) {       // the counter in 256 bytes of its own, then the maps
+    const int64_t n = chunks_of(T, L), W = width_of(C), tiles = (C + W - 1) / W;
+    return n > 1 ? 256 + B * tiles * W * (n + n / GROUP + n / (GROUP * GROUP)) * 8 : 0;
+}
+
+// The kernel's arguments for chunks of STRETCHES * L steps; the workspace is filled on the way.
+wnv_status prepare(const char* who, const wnv_recurrence_args* a, int L, RecArgs& k) {
+    k.B = a->B; k.C = a->C; k.T = (int)a->T;
+    k.tiles = (a->C + width_of(a->C) - 1) / width_of(a->C);
+    k.chunks = chunks_of(a->T, L);
     k.zb = a->z_batch_stride; k.zt = a->z_time_stride; k.h0b = a->h0_batch_stride;
     k.z = a->z; k.h0 = a->h0; k.lengths = a->lengths; k.seg_start = a->seg_start;
-    k.y = a->y; k.h_last = a->h_last; k.saved = (float*)a->saved;
+    k.y = a->y; k.h_last = a->h_last; k.saved = (float*)a->saved; k.slots = (unsigned long long*)a->workspace;
     k.dy = a->dy; k.dyb = a->dy_batch_stride; k.dyt = a->dy_time_stride;
     k.dh_last = a->dh_last; k.dz = a->dz; k.dh0 = a->dh0;
-    return k;
+    const int64_t blocks = (int64_t)k.B * k.tiles * k.chunks, bytes = slot_bytes(a->B, a->T, a->C, L);
+    if (blocks >= (1 << 24)) return fail(WNV_ERR_UNSUPPORTED, "%s: B x T x C is too large", who);
+    if (bytes) {
+        if (!a->workspace) return fail(WNV_ERR_INVALID_ARG, "%s: workspace is NULL", who);
+        hipLaunchKernelGGL(wnv_recurrence_fill, dim3((unsigned)((bytes / 16 + 255) / 256)), dim3(256), 0, (hipStream_t)a->stream,
+                           (uint4*)a->workspace, (long long)(bytes / 16));
+    }
+    return WNV_OK;
 }
 
 }  // namespace
 
 extern "C" int64_t wnv_recurrence_saved_bytes(int32_t B, int64_t T, int32_t C, int32_t gates, int32_t dtype) {
     if (check_shape("wnv_recurrence_saved_bytes", 0, B, T, C, gates, dtype) != WNV_OK) return -1;
-    return (int64_t)B * T * C * 4;
+    const int W = width_of(C);
+    return (int64_t)B * ((C + W - 1) / W) * chunks_of(T, BWD_L) * W * 4;
 }
 
 extern "C" int64_t wnv_recurrence_workspace_bytes(int32_t B, int64_t T, int32_t C, int32_t gates, int32_t dtype) {
     if (check_shape("wnv_recurrence_workspace_bytes", 0, B, T, C, gates, dtype) != WNV_OK) return -1;
-    return 0;
+    return std::max(slot_bytes(B, T, C, FWD_L), slot_bytes(B, T, C, BWD_L));
 }
+
+#define WNV_LAUNCH_BY_SHAPE(kernel, a, k)                                                                                       \
+    do {                                                                                                                        \
+        const dim3 grid((unsigned)((int64_t)k.B * k.tiles * k.chunks));                                                         \
+        hipStream_t s = (hipStream_t)a->stream;                                                                                 \
+        WNV_BY_TYPE(a->dtype, {                                                                                                 \
+            if (a->gates == 3 && a->C >= 4) hipLaunchKernelGGL((kernel<E, 3, 4>), grid, dim3(THREADS), 0, s, k);                 \
+            else if (a->gates == 3) hipLaunchKernelGGL((kernel<E, 3, 1>), grid, dim3(THREADS), 0, s, k);                         \
+            else if (a->C >= 4) hipLaunchKernelGGL((kernel<E, 2, 4>), grid, dim3(THREADS), 0, s, k);                             \
+            else hipLaunchKernelGGL((kernel<E, 2, 1>), grid, dim3(THREADS), 0, s, k);                                            \
+        });                                                                                                                     \
+    } while (0)
 
 extern "C" wnv_status wnv_recurrence_forward(int32_t device, const wnv_recurrence_args* a) {
     if (!a || !a->z || !a->y || !a->h_last) return fail(WNV_ERR_INVALID_ARG, "wnv_recurrence_forward: NULL argument");
@@ -176,9 +536,9 @@ extern "C" wnv_status wnv_recurrence_forward(int32_t device, const wnv_recurrenc
     if (wnv_status st = check_strides("wnv_recurrence_forward", a)) return st;
     DeviceGuard guard(device);
     if (!guard.ok) return fail(WNV_ERR_HIP, "wnv_recurrence_forward: cannot select device %d", device);
-    const RecArgs k = device_args(a);
-    const dim3 grid((a->C + RT - 1) / RT, a->B);
-    WNV_BY_TYPE(a->dtype, hipLaunchKernelGGL(wnv_recurrence_fwd<E>, grid, dim3(RT), 0, (hipStream_t)a->stream, k));
+    RecArgs k{};
+    if (wnv_status st = prepare("wnv_recurrence_forward", a, FWD_L, k)) return st;
+    WNV_LAUNCH_BY_SHAPE(wnv_recurrence_fwd, a, k);
     return launched("wnv_recurrence_forward");
 }
 
@@ -188,9 +548,9 @@ extern "C" wnv_status wnv_recurrence_backward(int32_t device, const wnv_recurren
     if (wnv_status st = check_strides("wnv_recurrence_backward", a)) return st;
     DeviceGuard guard(device);
     if (!guard.ok) return fail(WNV_ERR_HIP, "wnv_recurrence_backward: cannot select device %d", device);
-    const RecArgs k = device_args(a);
-    const dim3 grid((a->C + RT - 1) / RT, a->B);
-    WNV_BY_TYPE(a->dtype, hipLaunchKernelGGL(wnv_recurrence_bwd<E>, grid, dim3(RT), 0, (hipStream_t)a->stream, k));
+    RecArgs k{};
+    if (wnv_status st = prepare("wnv_recurrence_backward", a, BWD_L, k)) return st;
+    WNV_LAUNCH_BY_SHAPE(wnv_recurrence_bwd, a, k);
     return launched("wnv_recurrence_backward");
 }
 
