@@ -372,3 +372,12 @@ def test_offsets_of_the_step_over_32_bits():
     v.copy_(z[:, 0])
     a, b = h0.cuda(), h0.cuda()
     assert torch.equal(gated_recurrence_step(v, a), gated_recurrence_step(z[:, 0].cuda(), b)) and torch.equal(a, b)
+
+
+def test_steps_far_apart():
+    """Time strides of 2^22 elements and more are copied once."""
+    z, h0, dy, dh = inputs(1, 3, 8, 3, torch.bfloat16, seed=61)
+    far = (1 << 22) + 16
+    v = torch.empty(2 * far + 24, dtype=torch.bfloat16, device="cuda").as_strided((1, 3, 24), (3 * far, far, 1))
+    v.copy_(z)
+    assert torch.equal(gated_recurrence(v, h0.cuda())[0], gated_recurrence(z.cuda(), h0.cuda())[0])

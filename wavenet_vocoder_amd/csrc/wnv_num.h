@@ -14,14 +14,16 @@ template <typename E> __device__ __forceinline__ float wnv_up(E x) { return (flo
 // one rounding to nearest even, of a value computed in 32 bits
 template <typename E> __device__ __forceinline__ E wnv_down(float x) { return (E)x; }
 
-// keep = sigmoid(x) and its complement 1 - keep = e / (1 + e), e = exp(-x), both from one exponential and one reciprocal; the
-// complement is exact to a few ulps where keep is next to 1 (1 - keep would leave it 2^-24 absolute: at x = 9, 5e-4 of it).
-// The exponent stops at 126, so that 1 + e is finite and its reciprocal normal: keep <= 2^-126 and 1 - keep = 1 there, in
-// place of inf * 0.  A NaN passes (the comparison is false).
-__device__ __forceinline__ void wnv_gate(float x, float& keep, float& drop) {
-    float p = x * -1.44269504088896340736f;
-    p = p > 126.0f ? 126.0f : p;
-    const float e = __builtin_amdgcn_exp2f(p);
-    keep = __builtin_amdgcn_rcpf(1.0f + e);
-    drop = e * keep;
+// sigmoid(x) = 1 / (1 + exp(-x)), by the hardware's base-2 exponential and reciprocal (an ulp each): to a few ulps of itself at both
+// ends, so that 1 - sigmoid(f), taken as sigmoid(-f), is as exact next to 0 as sigmoid(f) (1 - sigmoid(f) would leave it 2^-24
+// absolute: at f = 9, 5e-4 of it).  exp overflows to infinity, whose reciprocal is the right 0; a NaN passes.
+__device__ __forceinline__ float wnv_gate(float x) {
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -1.44269504088896340736f));
+}
+// The same, and sigmoid(x) (1 - sigmoid(x)) = e / (1 + e)^2 with e = exp(-|x|) <= 1: exact at both ends too, no overflow.
+__device__ __forceinline__ float wnv_gate(float x, float& slope) {
+    const float e = __builtin_amdgcn_exp2f(fabsf(x) * -1.44269504088896340736f);
+    const float r = __builtin_amdgcn_rcpf(1.0f + e), er = e * r;
+    slope = er * r;
+    return x >= 0.f ? r : er;
 }

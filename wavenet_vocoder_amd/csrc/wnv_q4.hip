@@ -147,15 +147,10 @@ __global__ void __launch_bounds__(64) wnv_q4_rows(Q4Dev q, Q4Call a) {
     }
     const int row = blockIdx.x * 16 + r;
     if (row >= q.rows) return;
-    float keep, u, h = a.state[(long long)b * q.rows + row];
-    wnv_gate(z[0], keep, u);
-    h = fmaf(u, z[GATES > 1 ? 1 : 0] - h, h);
+    float h = a.state[(long long)b * q.rows + row];
+    h = fmaf(wnv_gate(-z[0]), z[GATES > 1 ? 1 : 0] - h, h);
     a.state[(long long)b * q.rows + row] = h;
-    if (GATES == 3) {
-        float so, uo;
-        wnv_gate(z[GATES > 2 ? 2 : 0], so, uo);
-        h *= so;
-    }
+    if (GATES == 3) h *= wnv_gate(z[GATES > 2 ? 2 : 0]);
     ((E*)a.y)[(long long)b * q.rows + row] = wnv_down<E>(h);
 }
 

@@ -24,7 +24,7 @@ struct RecArgs {
     void* y;
     float* h_last;
     float* saved;                   // [row][chunk of the backward pass][tile width]: the state before the chunk's first step
-    unsigned long long* slots;      // workspace: a counter in 256 bytes of its own, then each row's maps
+    unsigned long long* slots;      // workspace: of each row a counter, then its maps
     const void* dy;
     long long dyb, dyt;
     const float* dh_last;
@@ -72,22 +72,21 @@ __device__ __forceinline__ Map taken(const unsigned long long* slot, unsigned lo
 // group's; the last one of a section hands out the state behind it.  A chunk takes the section's state, runs it through the maps
 // of the groups before its own and of the chunks before it in its group: two waits behind its own loads for 256 chunks (32768 steps
 // forward), and one more for each further section.
-constexpr int GROUP = 16;
-struct Slots {                      // of one row of tiles, a thread's own channel
+constexpr int GROUP = 16, COUNTER = 16;      // a row's counter has 128 bytes of its own
+struct Slots {                      // of one row of tiles, one channel
     unsigned long long *chunk, *group, *section;
 };
-__device__ __forceinline__ long long slots_of_row(int chunks, int W) {
-    return (long long)W * (chunks + chunks / GROUP + chunks / (GROUP * GROUP));
+__host__ __device__ __forceinline__ long long slots_of_row(int chunks, int W) {
+    return COUNTER + (long long)W * (chunks + chunks / GROUP + chunks / (GROUP * GROUP));
 }
 __device__ __forceinline__ Slots slots_at(unsigned long long* all, int row, int chunks, int W, int ch) {
-    unsigned long long* p = all + 32 + row * slots_of_row(chunks, W) + ch;
+    unsigned long long* p = all + row * slots_of_row(chunks, W) + COUNTER + ch;
     return {p, p + (long long)W * chunks, p + (long long)W * (chunks + chunks / GROUP)};
 }
 
-// Joins `own` to what stands before it in the group of chunk k (counted in the order in which the chunks are drawn) and hands out what
-// others wait for; `before`: the maps, still to be applied.
-template <int W>
-__device__ __forceinline__ int maps_in_group(const Slots& s, int k, int chunks, Map own, Map (&before)[GROUP - 1]) {
+// Hands out what others wait for of chunk k (counted in the order in which the chunks are drawn), and returns the map of the chunks
+// before it in its group.
+template <int W> __device__ __forceinline__ Map map_in_group(const Slots& s, int k, int chunks, Map own) {
     const int at = k % GROUP;
     const bool more = k + 1 < chunks, last = at == GROUP - 1;
     if (more && !last) publish(s.chunk + (long long)k * W, own);
@@ -98,12 +97,9 @@ __device__ __forceinline__ int maps_in_group(const Slots& s, int k, int chunks, 
     Map all{0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < GROUP - 1; ++i)
-        if (i < at) {
-            before[i] = taken(s.chunk + (long long)(k - at + i) * W, v[i]);
-            all = join(all, before[i]);
-        }
+        if (i < at) all = join(all, taken(s.chunk + (long long)(k - at + i) * W, v[i]));
     if (more && last && k / GROUP % GROUP != GROUP - 1) publish(s.group + (long long)(k / GROUP) * W, join(all, own));
-    return at;
+    return all;
 }
 // The state before the group of chunk k; `first` before chunk 0.
 template <int W> __device__ __forceinline__ float state_before_group(const Slots& s, int k, float first) {
@@ -122,43 +118,81 @@ template <int W> __device__ __forceinline__ float state_before_group(const Slots
         if (i < n) h = apply(taken(s.group + (long long)(g0 + i) * W, v[i]), h);
     return h;
 }
-template <int W> __device__ __forceinline__ void state_behind(const Slots& s, int k, int chunks, float h) {
-    if ((k + 1) % (GROUP * GROUP) == 0 && k + 1 < chunks) publish(s.section + (long long)(k / (GROUP * GROUP)) * W, {-1.f, h});
-}
+__device__ __forceinline__ bool ends_section(int k, int chunks) { return (k + 1) % (GROUP * GROUP) == 0 && k + 1 < chunks; }
 
 // ---- the shape of a workgroup -------------------------------------------------------------------------------------------------
-// 256 threads = 16 lanes along the channels x 16 stretches of L steps.  A lane holds V channels, so that a row of a tile is 64
-// channels: 128 bytes of a 16-bit type, 256 of float32.  The last lane of a row that is no multiple of V starts earlier and shares
-// channels with its neighbour (both compute and write the same); V = 1 is for rows narrower than 4.
-constexpr int THREADS = 256, LANES = 16, STRETCHES = THREADS / LANES;
+// 4 waves of 4 stretches of L steps; a stretch is 16 lanes, a row of the wave, along the channels.  A lane holds V channels, so that
+// a tile is 64 channels wide: 128 bytes of a 16-bit type, 256 of float32.  The last lane of a tile that ends in no multiple of V
+// starts earlier and shares channels with its neighbour (both compute and write the same); V = 1 is for rows narrower than 4.
+constexpr int WAVES = 4, THREADS = 64 * WAVES, LANES = 16, STRETCHES = THREADS / LANES;
 constexpr int FWD_L = 8, BWD_L = 4;
 
-template <typename E, int V> struct Vec { E e[V]; };
-template <typename E, int V> __device__ __forceinline__ Vec<E, V> load(const E* p) {      // at any alignment
-    Vec<E, V> v;
-    __builtin_memcpy(&v, p, sizeof v);
+// V elements as they stand in memory, packed in as few registers; addresses are a uniform base and 32 bits of a lane's own.
+template <typename E, int V> struct Vec {
+    static constexpr int N = (V * (int)sizeof(E) + 3) / 4;
+    uint32_t w[N];
+    __device__ __forceinline__ float get(int i) const {
+        if (sizeof(E) == 4) return __uint_as_float(w[i]);
+        if (__is_same(E, wnv_bf16)) return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+        return (float)__builtin_bit_cast(wnv_f16, (uint16_t)(w[i / 2] >> (16 * (i & 1))));
+    }
+};
+// Data goes past the caches: it is read and written once (bf16 8 x 24064 x 512 forward: 213 us without, 188 with the hint).
+template <int BYTES> struct Raw { typedef uint32_t T __attribute__((ext_vector_type(BYTES / 4), aligned(1))); };
+template <> struct Raw<2> { typedef uint16_t T __attribute__((aligned(1))); };
+template <> struct Raw<4> { typedef uint32_t T __attribute__((aligned(1))); };
+template <typename E, int V> __device__ __forceinline__ Vec<E, V> load(const E* base, uint32_t bytes) {        // at any alignment
+    typedef typename Raw<V * sizeof(E)>::T R;
+    const R r = __builtin_nontemporal_load((const R*)((const char*)base + bytes));
+    Vec<E, V> v{};
+    __builtin_memcpy(v.w, &r, sizeof r);
     return v;
 }
-template <typename E, int V> __device__ __forceinline__ void store(E* p, const Vec<E, V>& v) { __builtin_memcpy(p, &v, sizeof v); }
+template <typename E, int V> __device__ __forceinline__ void store(E* base, uint32_t bytes, const float (&x)[V]) {
+    typedef typename Raw<V * sizeof(E)>::T R;
+    E e[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) e[i] = wnv_down<E>(x[i]);
+    R r;
+    __builtin_memcpy(&r, e, sizeof r);
+    __builtin_nontemporal_store(r, (R*)((char*)base + bytes));
+}
+
+// The maps of a wave's four rows joined in time (BACK: the last row first): of all four, and of those before the own row.
+template <bool BACK> __device__ __forceinline__ void join_rows(Map x, Map& all, Map& before) {
+    const auto u = __builtin_amdgcn_permlane16_swap(__float_as_uint(x.u), __float_as_uint(x.u), false, false);     // rows 0 0 2 2 | 1 1 3 3
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x.b), __float_as_uint(x.b), false, false);
+    const Map even{__uint_as_float(u[0]), __uint_as_float(b[0])}, odd{__uint_as_float(u[1]), __uint_as_float(b[1])};
+    const Map pair = BACK ? join(odd, even) : join(even, odd);
+    const auto pu = __builtin_amdgcn_permlane32_swap(__float_as_uint(pair.u), __float_as_uint(pair.u), false, false);  // rows 0 1 0 1 | 2 3 2 3
+    const auto pb = __builtin_amdgcn_permlane32_swap(__float_as_uint(pair.b), __float_as_uint(pair.b), false, false);
+    const Map low{__uint_as_float(pu[0]), __uint_as_float(pb[0])}, high{__uint_as_float(pu[1]), __uint_as_float(pb[1])};
+    const int row = (threadIdx.x / LANES) & 3;
+    all = BACK ? join(high, low) : join(low, high);
+    before = (row & 1) != BACK ? (BACK ? odd : even) : Map{0.f, 0.f};
+    if ((row >> 1) != BACK) before = join(BACK ? high : low, before);
+}
 
 struct Place { int b, tile, chunk, row; };
 
-// Chunks are drawn from a counter, all rows' first ones first: the order that the waits rely on.
-template <bool BACK> __device__ __forceinline__ Place draw_place(const RecArgs& a) {
+// Chunks are drawn from a counter, one for all tiles of a batch row, all tiles' first chunks first: the order that the waits rely on.
+// Workgroup i runs on XCD i % 8, so that for a batch of 8 a row's maps stay within one L2, which also reads whole rows of z: a
+// counter for each tile instead keeps an XCD to one column of tiles and to few of its L2's channels (float32 8 x 24064 x 512
+// backward: 562 us against 491), and one for all workgroups is drawn from by 700 at once (bf16 8 x 7680 x 128 forward: 28 against 18).
+template <bool BACK> __device__ __forceinline__ Place draw_place(const RecArgs& a, int W) {
     __shared__ int drawn;
-    int i = blockIdx.x;
-    if (a.chunks > 1) {
-        if (threadIdx.x == 0) drawn = atomicAdd((int*)a.slots, 1) + 1;      // filled with ones: it starts at -1
-        __syncthreads();
-        i = drawn;
-    }
-    const int rows = a.B * a.tiles;
     Place p;
-    p.row = i % rows;
-    p.chunk = i / rows;
+    p.b = blockIdx.x % a.B;
+    int i = blockIdx.x / a.B;
+    if (a.chunks > 1) {
+        if (threadIdx.x == 0) drawn = atomicAdd((int*)(a.slots + (long long)p.b * a.tiles * slots_of_row(a.chunks, W)), 1) + 1;     // it starts at -1
+        __syncthreads();
+        i = __builtin_amdgcn_readfirstlane(drawn);
+    }
+    p.tile = i % a.tiles;
+    p.chunk = i / a.tiles;
     if (BACK) p.chunk = a.chunks - 1 - p.chunk;
-    p.b = p.row / a.tiles;
-    p.tile = p.row % a.tiles;
+    p.row = p.b * a.tiles + p.tile;
     return p;
 }
 
@@ -177,32 +211,33 @@ template <int L> __device__ __forceinline__ Stretch stretch_of(const RecArgs& a,
     return s;
 }
 
-// One chunk of one tile.  Each thread reduces its stretch to a map, 64 threads (one a channel) join the stretches' maps, find the
-// state before the chunk and walk it through, and each thread runs over its stretch again, out of its registers.  z is read once.
+// One chunk of one tile.  Each thread reduces its stretch to a map, the wave joins its four, wave 0 the chunk's and its group's while
+// wave 1 finds the state before the group; then each thread knows the state before its stretch and runs over it again, out of its
+// registers.  z is read once.
 template <typename E, int G, int V>
-__global__ void __launch_bounds__(THREADS) wnv_recurrence_fwd(RecArgs a) {
+__global__ void __launch_bounds__(THREADS, sizeof(E) == 4 ? 3 : 4) wnv_recurrence_fwd(RecArgs a) {
     constexpr int L = FWD_L, W = LANES * V;
-    __shared__ Map maps[STRETCHES][W];
-    __shared__ float starts[STRETCHES][W], base[W];
-    const int tid = threadIdx.x, lane = tid % LANES, st = tid / LANES;
-    const Place p = draw_place<false>(a);
-    const int first = p.tile * W + lane * V;
-    const bool on = first < a.C;
-    const int c = min(first, a.C - V);
-    const Stretch s = stretch_of<L>(a, p.b, p.chunk * (STRETCHES * L) + st * L);
+    __shared__ Map totals[WAVES][W], prev[W];
+    __shared__ float base[W];
+    const int tid = threadIdx.x, lane = tid % LANES, wave = tid / 64, at = lane * V;
+    const Place p = draw_place<false>(a, W);
+    const bool on = p.tile * W + at < a.C;
+    const int c = min(p.tile * W + at, a.C - V);
+    const Stretch s = stretch_of<L>(a, p.b, p.chunk * (STRETCHES * L) + tid / LANES * L);
     const int live = on ? s.live : 0;
-    const E* z = (const E*)a.z + (long long)p.b * a.zb + (long long)s.t0 * a.zt + c;
+    const E* z = (const E*)a.z + (long long)p.b * a.zb + (long long)p.chunk * (STRETCHES * L) * a.zt;
+    const uint32_t from = (uint32_t)(tid / LANES * L * a.zt + c) * (uint32_t)sizeof(E);
 
     Vec<E, V> f[L], v[L], o[L];
 #pragma unroll
     for (int l = 0; l < L; ++l)
         if (l < live) {
-            f[l] = load<E, V>(z + l * a.zt);
-            v[l] = load<E, V>(z + l * a.zt + a.C);
-            if (G == 3) o[l] = load<E, V>(z + l * a.zt + 2 * a.C);
+            f[l] = load<E, V>(z + l * a.zt, from);
+            v[l] = load<E, V>(z + l * a.zt + a.C, from);
+            if (G == 3) o[l] = load<E, V>(z + l * a.zt + 2 * a.C, from);
         }
     float u[L][V];
-    Map m[V];
+    Map m[V], before[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) m[i] = {0.f, 0.f};
 #pragma unroll
@@ -210,75 +245,69 @@ __global__ void __launch_bounds__(THREADS) wnv_recurrence_fwd(RecArgs a) {
         if (l < live) {
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                float keep;
-                wnv_gate(wnv_up(f[l].e[i]), keep, u[l][i]);
+                u[l][i] = wnv_gate(-f[l].get(i));
                 if (s.begins >> l & 1) m[i].b = 0.f;
                 m[i].u = fmaf(-u[l][i], m[i].u, m[i].u + u[l][i]);
-                m[i].b = fmaf(u[l][i], wnv_up(v[l].e[i]) - m[i].b, m[i].b);
+                m[i].b = fmaf(u[l][i], v[l].get(i) - m[i].b, m[i].b);
             }
         }
 #pragma unroll
-    for (int i = 0; i < V; ++i) maps[st][lane * V + i] = {s.begins ? -1.f : m[i].u, m[i].b};
-    __syncthreads();
-
-    // wave 0: the chunk's map, and the chunks of its group; wave 1: what stands before the group
-    const int wave = tid / 64, ch = tid % 64, chan = min(p.tile * W + ch / V * V, a.C - V) + ch % V;
-    const bool there = ch < W && p.tile * W + ch / V * V < a.C;
-    const Slots slots = slots_at(a.slots, p.row, a.chunks, W, ch);
-    Map before[GROUP - 1];
-    int n = 0;
-    if (wave == 0 && ch < W) {
-        Map all{0.f, 0.f};
-#pragma unroll
-        for (int k = 0; k < STRETCHES; ++k) all = join(all, maps[k][ch]);
-        n = maps_in_group<W>(slots, p.chunk, a.chunks, all, before);
-    } else if (wave == 1 && ch < W) {
-        base[ch] = state_before_group<W>(slots, p.chunk, a.h0 && there ? a.h0[p.b * a.h0b + chan] : 0.f);
+    for (int i = 0; i < V; ++i) {
+        if (s.begins) m[i].u = -1.f;
+        Map all;
+        join_rows<false>(m[i], all, before[i]);
+        if (tid % 64 < LANES) totals[wave][at + i] = all;
     }
     __syncthreads();
-    if (wave == 0 && ch < W) {
-        float h = base[ch];
+    const int ch = tid % 64;
+    if (wave < 2 && ch < W) {
+        const Slots slots = slots_at(a.slots, p.row, a.chunks, W, ch);
+        if (wave == 0) {
+            Map all = totals[0][ch];
 #pragma unroll
-        for (int i = 0; i < GROUP - 1; ++i)
-            if (i < n) h = apply(before[i], h);
-        constexpr int EVERY = BWD_L * STRETCHES / L;        // stretches between two states that the backward pass starts from
-        const int saves = (a.T + BWD_L * STRETCHES - 1) / (BWD_L * STRETCHES), left = (a.T - p.chunk * (STRETCHES * L) + L - 1) / L;
-        float* save = a.saved ? a.saved + ((long long)p.row * saves + p.chunk * (STRETCHES / EVERY)) * W + ch : nullptr;
-#pragma unroll
-        for (int k = 0; k < STRETCHES; ++k) {
-            starts[k][ch] = h;
-            if (k % EVERY == 0 && save && k < left) save[k / EVERY * W] = h;
-            h = apply(maps[k][ch], h);
+            for (int w = 1; w < WAVES; ++w) all = join(all, totals[w][ch]);
+            prev[ch] = map_in_group<W>(slots, p.chunk, a.chunks, all);
+        } else {
+            const bool there = p.tile * W + ch / V * V < a.C;
+            base[ch] = state_before_group<W>(slots, p.chunk, a.h0 && there ? a.h0[p.b * a.h0b + min(p.tile * W + ch / V * V, a.C - V) + ch % V] : 0.f);
         }
-        state_behind<W>(slots, p.chunk, a.chunks, h);
-        if (p.chunk + 1 == a.chunks && there) a.h_last[(long long)p.b * a.C + chan] = h;
     }
     __syncthreads();
 
+    constexpr int EVERY = BWD_L * WAVES / L;            // waves between two states that the backward pass starts from
+    const int saves = (a.T + BWD_L * STRETCHES - 1) / (BWD_L * STRETCHES), save = p.chunk * (WAVES / EVERY) + wave / EVERY;
     float h[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) h[i] = starts[st][lane * V + i];
-    E* y = (E*)a.y + ((long long)p.b * a.T + s.t0) * a.C + c;
+    for (int i = 0; i < V; ++i) {
+        h[i] = apply(prev[at + i], base[at + i]);
+        for (int w = 0; w < wave; ++w) h[i] = apply(totals[w][at + i], h[i]);
+        if (a.saved && tid % (64 * EVERY) < LANES && save < saves) a.saved[((long long)p.row * saves + save) * W + at + i] = h[i];
+        h[i] = apply(before[i], h[i]);
+        if (tid >= THREADS - LANES) {                   // the chunk's last stretch: the state behind it
+            const float last = apply(m[i], h[i]);
+            if (ends_section(p.chunk, a.chunks))
+                publish(slots_at(a.slots, p.row, a.chunks, W, at + i).section + (long long)(p.chunk / (GROUP * GROUP)) * W, {-1.f, last});
+            if (p.chunk + 1 == a.chunks && on) a.h_last[(long long)p.b * a.C + c + i] = last;
+        }
+    }
+    E* y = (E*)a.y + ((long long)p.b * a.T + (long long)p.chunk * (STRETCHES * L)) * a.C;
+    const uint32_t to = (uint32_t)(tid / LANES * L * a.C + c) * (uint32_t)sizeof(E);
 #pragma unroll
     for (int l = 0; l < L; ++l)
         if (on && s.t0 + l < a.T) {
-            Vec<E, V> out;
+            float out[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 float q = 0.f;
                 if (l < live) {
                     if (s.begins >> l & 1) h[i] = 0.f;
-                    h[i] = fmaf(u[l][i], wnv_up(v[l].e[i]) - h[i], h[i]);
+                    h[i] = fmaf(u[l][i], v[l].get(i) - h[i], h[i]);
                     q = h[i];
-                    if (G == 3) {
-                        float so, uo;
-                        wnv_gate(wnv_up(o[l].e[i]), so, uo);
-                        q *= so;
-                    }
+                    if (G == 3) q *= wnv_gate(o[l].get(i));
                 }
-                out.e[i] = wnv_down<E>(q);
+                out[i] = q;
             }
-            store<E, V>(y + (long long)l * a.C, out);
+            store<E, V>(y + (long long)l * a.C, to, out);
         }
 }
 
@@ -287,29 +316,32 @@ __global__ void __launch_bounds__(THREADS) wnv_recurrence_fwd(RecArgs a) {
 // The chunks run from the last to the first, r is found the way the forward pass finds h; h itself starts from the state that the
 // forward pass saved before each chunk and is run through again.
 template <typename E, int G, int V>
-__global__ void __launch_bounds__(THREADS) wnv_recurrence_bwd(RecArgs a) {
+__global__ void __launch_bounds__(THREADS, 3) wnv_recurrence_bwd(RecArgs a) {
     constexpr int L = BWD_L, W = LANES * V;
-    __shared__ Map ahead[STRETCHES][W], back[STRETCHES][W];         // of h and of r
-    __shared__ float hs[STRETCHES][W], rs[STRETCHES][W], base[W];
-    const int tid = threadIdx.x, lane = tid % LANES, st = tid / LANES;
-    const Place p = draw_place<true>(a);
-    const int first = p.tile * W + lane * V;
-    const bool on = first < a.C;
-    const int c = min(first, a.C - V);
-    const Stretch s = stretch_of<L>(a, p.b, p.chunk * (STRETCHES * L) + st * L);
+    __shared__ Map ahead[WAVES][W], back[WAVES][W], prev[W];        // of h and of r
+    __shared__ float base[W];
+    const int tid = threadIdx.x, lane = tid % LANES, wave = tid / 64, at = lane * V;
+    const Place p = draw_place<true>(a, W);
+    const int order = a.chunks - 1 - p.chunk;
+    const bool on = p.tile * W + at < a.C;
+    const int c = min(p.tile * W + at, a.C - V);
+    const Stretch s = stretch_of<L>(a, p.b, p.chunk * (STRETCHES * L) + tid / LANES * L);
     const int live = on ? s.live : 0;
-    const E* z = (const E*)a.z + (long long)p.b * a.zb + (long long)s.t0 * a.zt + c;
-    const E* dy = (const E*)a.dy + (long long)p.b * a.dyb + (long long)s.t0 * a.dyt + c;
+    const E* z = (const E*)a.z + (long long)p.b * a.zb + (long long)p.chunk * (STRETCHES * L) * a.zt;
+    const E* dy = (const E*)a.dy + (long long)p.b * a.dyb + (long long)p.chunk * (STRETCHES * L) * a.dyt;
+    const uint32_t from = (uint32_t)(tid / LANES * L * a.zt + c) * (uint32_t)sizeof(E);
+    const uint32_t dfrom = (uint32_t)(tid / LANES * L * a.dyt + c) * (uint32_t)sizeof(E);
 
     Vec<E, V> f[L], v[L], o[L], d[L];
 #pragma unroll
     for (int l = 0; l < L; ++l)
         if (l < live) {
-            f[l] = load<E, V>(z + l * a.zt);
-            v[l] = load<E, V>(z + l * a.zt + a.C);
-            if (G == 3) o[l] = load<E, V>(z + l * a.zt + 2 * a.C);
-            if (a.dy) d[l] = load<E, V>(dy + l * a.dyt);
+            f[l] = load<E, V>(z + l * a.zt, from);
+            v[l] = load<E, V>(z + l * a.zt + a.C, from);
+            if (G == 3) o[l] = load<E, V>(z + l * a.zt + 2 * a.C, from);
+            if (a.dy) d[l] = load<E, V>(dy + l * a.dyt, dfrom);
         }
+    const Vec<float, V> saved = load<float, V>(a.saved + ((long long)p.row * a.chunks + p.chunk) * W, at * 4);
     float u[L][V], uk[L][V], g[L][V], q[L][V];          // u sigmoid(f); dy sigmoid(o); dy sigmoid(o) (1 - sigmoid(o))
     Map m[V], r[V];
 #pragma unroll
@@ -319,18 +351,15 @@ __global__ void __launch_bounds__(THREADS) wnv_recurrence_bwd(RecArgs a) {
         if (l < live) {
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                float keep;
-                wnv_gate(wnv_up(f[l].e[i]), keep, u[l][i]);
-                uk[l][i] = u[l][i] * keep;
+                u[l][i] = wnv_gate(-f[l].get(i), uk[l][i]);
                 if (s.begins >> l & 1) m[i].b = 0.f;
                 m[i].u = fmaf(-u[l][i], m[i].u, m[i].u + u[l][i]);
-                m[i].b = fmaf(u[l][i], wnv_up(v[l].e[i]) - m[i].b, m[i].b);
-                g[l][i] = a.dy ? wnv_up(d[l].e[i]) : 0.f;
+                m[i].b = fmaf(u[l][i], v[l].get(i) - m[i].b, m[i].b);
+                g[l][i] = a.dy ? d[l].get(i) : 0.f;
                 if (G == 3) {
-                    float so, uo;
-                    wnv_gate(wnv_up(o[l].e[i]), so, uo);
+                    const float so = wnv_gate(o[l].get(i), q[l][i]);
+                    q[l][i] *= g[l][i];
                     g[l][i] *= so;
-                    q[l][i] = g[l][i] * uo;
                 }
             }
         }
@@ -343,85 +372,78 @@ __global__ void __launch_bounds__(THREADS) wnv_recurrence_bwd(RecArgs a) {
                 r[i].b = s.begins >> l & 1 ? 0.f : fmaf(-u[l][i], dh, dh);
             }
         }
+    Map h_before[V], r_before[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        ahead[st][lane * V + i] = {s.begins ? -1.f : m[i].u, m[i].b};
-        back[st][lane * V + i] = {s.begins ? -1.f : m[i].u, r[i].b};
+        if (s.begins) m[i].u = -1.f;
+        r[i].u = m[i].u;
+        Map all, all_back;
+        join_rows<false>(m[i], all, h_before[i]);
+        join_rows<true>(r[i], all_back, r_before[i]);
+        if (tid % 64 < LANES) ahead[wave][at + i] = all, back[wave][at + i] = all_back;
     }
     __syncthreads();
-
-    // waves 0 and 1 as in the forward pass, on the chunks from behind; wave 2: h through the chunk
-    const int wave = tid / 64, ch = tid % 64, chan = min(p.tile * W + ch / V * V, a.C - V) + ch % V, order = a.chunks - 1 - p.chunk;
-    const bool there = ch < W && p.tile * W + ch / V * V < a.C;
-    const Slots slots = slots_at(a.slots, p.row, a.chunks, W, ch);
-    Map behind[GROUP - 1];
-    int n = 0;
-    if (wave == 0 && ch < W) {
-        Map all{0.f, 0.f};
+    const int ch = tid % 64;
+    if (wave < 2 && ch < W) {
+        const Slots slots = slots_at(a.slots, p.row, a.chunks, W, ch);
+        if (wave == 0) {
+            Map all = back[WAVES - 1][ch];
 #pragma unroll
-        for (int k = STRETCHES - 1; k >= 0; --k) all = join(all, back[k][ch]);
-        n = maps_in_group<W>(slots, order, a.chunks, all, behind);
-    } else if (wave == 1 && ch < W) {
-        base[ch] = state_before_group<W>(slots, order, a.dh_last && there ? a.dh_last[(long long)p.b * a.C + chan] : 0.f);
-    } else if (wave == 2 && ch < W) {
-        float h = a.saved[((long long)p.row * a.chunks + p.chunk) * W + ch];
-#pragma unroll
-        for (int k = 0; k < STRETCHES; ++k) {
-            hs[k][ch] = h;
-            h = apply(ahead[k][ch], h);
+            for (int w = WAVES - 2; w >= 0; --w) all = join(all, back[w][ch]);
+            prev[ch] = map_in_group<W>(slots, order, a.chunks, all);
+        } else {
+            const bool there = p.tile * W + ch / V * V < a.C;
+            base[ch] = state_before_group<W>(slots, order, a.dh_last && there ? a.dh_last[(long long)p.b * a.C + min(p.tile * W + ch / V * V, a.C - V) + ch % V] : 0.f);
         }
-    }
-    __syncthreads();
-    if (wave == 0 && ch < W) {
-        float x = base[ch];
-#pragma unroll
-        for (int i = 0; i < GROUP - 1; ++i)
-            if (i < n) x = apply(behind[i], x);
-#pragma unroll
-        for (int k = STRETCHES - 1; k >= 0; --k) {
-            rs[k][ch] = x;
-            x = apply(back[k][ch], x);
-        }
-        state_behind<W>(slots, order, a.chunks, x);
-        if (p.chunk == 0 && a.dh0 && there) a.dh0[(long long)p.b * a.C + chan] = x;
     }
     __syncthreads();
 
     float before[L][V], x[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        float h = hs[st][lane * V + i];
-        x[i] = rs[st][lane * V + i];
+        float h = saved.get(i);
+        x[i] = apply(prev[at + i], base[at + i]);
+        for (int w = 0; w < wave; ++w) h = apply(ahead[w][at + i], h);
+        for (int w = WAVES - 1; w > wave; --w) x[i] = apply(back[w][at + i], x[i]);
+        h = apply(h_before[i], h);
+        x[i] = apply(r_before[i], x[i]);
+        if (tid < LANES) {                              // the chunk's first stretch: what flows out of it
+            const float out = apply(r[i], x[i]);
+            if (ends_section(order, a.chunks))
+                publish(slots_at(a.slots, p.row, a.chunks, W, at + i).section + (long long)(order / (GROUP * GROUP)) * W, {-1.f, out});
+            if (p.chunk == 0 && a.dh0 && on) a.dh0[(long long)p.b * a.C + c + i] = out;
+        }
 #pragma unroll
         for (int l = 0; l < L; ++l)
             if (l < live) {
                 before[l][i] = s.begins >> l & 1 ? 0.f : h;
-                h = fmaf(u[l][i], wnv_up(v[l].e[i]) - before[l][i], before[l][i]);
+                h = fmaf(u[l][i], v[l].get(i) - before[l][i], before[l][i]);
             }
     }
-    E* dz = (E*)a.dz + ((long long)p.b * a.T + s.t0) * (G * (long long)a.C) + c;
+    E* dz = (E*)a.dz + ((long long)p.b * a.T + (long long)p.chunk * (STRETCHES * L)) * (G * (long long)a.C);
+    const uint32_t to = (uint32_t)(tid / LANES * L * G * a.C + c) * (uint32_t)sizeof(E);
 #pragma unroll
     for (int l = L - 1; l >= 0; --l)
         if (on && s.t0 + l < a.T) {
-            Vec<E, V> df, dv, dg;
+            float df[V], dv[V], dg[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 float xf = 0.f, xv = 0.f, xo = 0.f;
                 if (l < live) {
-                    const float w = wnv_up(v[l].e[i]) - before[l][i], dh = g[l][i] + x[i];
+                    const float w = v[l].get(i) - before[l][i], dh = g[l][i] + x[i];
                     xf = -dh * w * uk[l][i];
                     xv = dh * u[l][i];
                     if (G == 3) xo = q[l][i] * fmaf(u[l][i], w, before[l][i]);
                     x[i] = s.begins >> l & 1 ? 0.f : fmaf(-u[l][i], dh, dh);
                 }
-                df.e[i] = wnv_down<E>(xf);
-                dv.e[i] = wnv_down<E>(xv);
-                dg.e[i] = wnv_down<E>(xo);
+                df[i] = xf;
+                dv[i] = xv;
+                dg[i] = xo;
             }
-            E* to = dz + (long long)l * G * a.C;
-            store<E, V>(to, df);
-            store<E, V>(to + a.C, dv);
-            if (G == 3) store<E, V>(to + 2 * (long long)a.C, dg);
+            E* row = dz + (long long)l * G * a.C;
+            store<E, V>(row, to, df);
+            store<E, V>(row + a.C, to, dv);
+            if (G == 3) store<E, V>(row + 2 * (long long)a.C, to, dg);
         }
 }
 
@@ -437,15 +459,10 @@ __global__ void __launch_bounds__(RT) wnv_recurrence_one(const E* z, long long z
     const int c = blockIdx.x * RT + threadIdx.x, b = blockIdx.y;
     if (c >= C) return;
     z += (long long)b * zb + c;
-    float keep, u, h = state[(long long)b * C + c];
-    wnv_gate(wnv_up(z[0]), keep, u);
-    h = fmaf(u, wnv_up(z[C]) - h, h);
+    float h = state[(long long)b * C + c];
+    h = fmaf(wnv_gate(-wnv_up(z[0])), wnv_up(z[C]) - h, h);
     state[(long long)b * C + c] = h;
-    if (gates == 3) {
-        float so, uo;
-        wnv_gate(wnv_up(z[2 * C]), so, uo);
-        h *= so;
-    }
+    if (gates == 3) h *= wnv_gate(wnv_up(z[2 * C]));
     y[(long long)b * C + c] = wnv_down<E>(h);
 }
 
@@ -475,14 +492,16 @@ wnv_status check_strides(const char* who, const wnv_recurrence_args* a) {
     if (a->z_batch_stride < 0 || a->z_time_stride < 0 || (a->h0 && a->h0_batch_stride < 0) ||
         (a->dy && (a->dy_batch_stride < 0 || a->dy_time_stride < 0)))
         return fail(WNV_ERR_INVALID_ARG, "%s: negative stride", who);
+    if (a->T > 1 && (a->z_time_stride >= (1 << 22) || (a->dy && a->dy_time_stride >= (1 << 22))))
+        return fail(WNV_ERR_UNSUPPORTED, "%s: time strides of 2^22 elements and more", who);
     return WNV_OK;
 }
 
 int width_of(int C) { return C < 4 ? LANES : LANES * 4; }
 int chunks_of(int64_t T, int L) { return (int)((T + STRETCHES * L - 1) / (STRETCHES * L)); }
-int64_t slot_bytes(int64_t B, int64_t T, int C, int L) {       // the counter in 256 bytes of its own, then the maps
-    const int64_t n = chunks_of(T, L), W = width_of(C), tiles = (C + W - 1) / W;
-    return n > 1 ? 256 + B * tiles * W * (n + n / GROUP + n / (GROUP * GROUP)) * 8 : 0;
+int64_t slot_bytes(int64_t B, int64_t T, int C, int L) {
+    const int n = chunks_of(T, L), W = width_of(C);
+    return n > 1 ? B * ((C + W - 1) / W) * slots_of_row(n, W) * 8 : 0;
 }
 
 // The kernel's arguments for chunks of STRETCHES * L steps; the workspace is filled on the way.
@@ -490,10 +509,10 @@ wnv_status prepare(const char* who, const wnv_recurrence_args* a, int L, RecArgs
     k.B = a->B; k.C = a->C; k.T = (int)a->T;
     k.tiles = (a->C + width_of(a->C) - 1) / width_of(a->C);
     k.chunks = chunks_of(a->T, L);
-    k.zb = a->z_batch_stride; k.zt = a->z_time_stride; k.h0b = a->h0_batch_stride;
+    k.zb = a->z_batch_stride; k.zt = a->T > 1 ? a->z_time_stride : 0; k.h0b = a->h0_batch_stride;
     k.z = a->z; k.h0 = a->h0; k.lengths = a->lengths; k.seg_start = a->seg_start;
     k.y = a->y; k.h_last = a->h_last; k.saved = (float*)a->saved; k.slots = (unsigned long long*)a->workspace;
-    k.dy = a->dy; k.dyb = a->dy_batch_stride; k.dyt = a->dy_time_stride;
+    k.dy = a->dy; k.dyb = a->dy_batch_stride; k.dyt = a->T > 1 ? a->dy_time_stride : 0;
     k.dh_last = a->dh_last; k.dz = a->dz; k.dh0 = a->dh0;
     const int64_t blocks = (int64_t)k.B * k.tiles * k.chunks, bytes = slot_bytes(a->B, a->T, a->C, L);
     if (blocks >= (1 << 24)) return fail(WNV_ERR_UNSUPPORTED, "%s: B x T x C is too large", who);

@@ -63,8 +63,8 @@ def _map(m: Optional[torch.Tensor], name: str, shape: Tuple[int, ...], z: torch.
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
-    """``t`` with its last dimension contiguous (a copy only where it is not: any batch and time stride is taken, 0 too)."""
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+    """``t`` with its last dimension contiguous: a copy only where it is not, or where steps lie 2^22 elements and more apart."""
+    return t if (t.stride(-1) == 1 or t.shape[-1] == 1) and (t.dim() < 3 or t.stride(1) < 1 << 22) else t.contiguous()
 
 
 def _call(fn, z, gates, h0, lengths, seg_start, *, y=None, h_last=None, saved=None, dy=None, dh_last=None, dz=None, dh0=None):
