@@ -23,7 +23,7 @@ struct RecArgs {
     const int *lengths, *seg_start;
     void* y;
     float* h_last;
-    float* saved;                   // [row][chunk of the backward pass][tile width]: the state before the chunk's first step
+    float* saved;                   // [row][chunk][tile width]: the state before the chunk's first step
     unsigned long long* slots;      // workspace: of each row a counter, then its maps
     const void* dy;
     long long dyb, dyt;
@@ -34,14 +34,19 @@ struct RecArgs {
 
 // ---- maps of the state --------------------------------------------------------------------------------------------------------
 // A stretch of steps maps the state before it to the state behind it: h -> h + (b - u h), with 1 - u the product of its gates; u < 0
-// says that the state behind it is b whatever stood before.  The backward pass maps what flows back by the same form.
+// says that the state behind it is b whatever stood before, which only happens where utterances begin (SEG; without the test a join
+// is 4 operations in place of 8, and the kernels a fifth shorter).  The backward pass maps what flows back by the same form.
 struct Map { float u, b; };
 
-__device__ __forceinline__ float apply(Map m, float h) { return m.u < 0.f ? m.b : h + fmaf(-m.u, h, m.b); }
-__device__ __forceinline__ Map join(Map first, Map then) {
+template <bool SEG> __device__ __forceinline__ float apply(Map m, float h) {
+    const float r = h + fmaf(-m.u, h, m.b);
+    return SEG && m.u < 0.f ? m.b : r;
+}
+template <bool SEG> __device__ __forceinline__ Map join(Map first, Map then) {
     Map r;
-    r.u = then.u < 0.f || first.u < 0.f ? -1.f : fmaf(-first.u, then.u, first.u + then.u);
-    r.b = apply(then, first.b);
+    r.u = fmaf(-first.u, then.u, first.u + then.u);
+    if (SEG && (then.u < 0.f || first.u < 0.f)) r.u = -1.f;
+    r.b = apply<SEG>(then, first.b);
     return r;
 }
 
@@ -55,16 +60,28 @@ __device__ __forceinline__ void publish(unsigned long long* slot, Map m) {
 __device__ __forceinline__ unsigned long long peek(const unsigned long long* slot) {
     return __hip_atomic_load(slot, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
+__device__ __forceinline__ Map unpacked(unsigned long long v) { return {__uint_as_float((unsigned)v), __uint_as_float((unsigned)(v >> 32))}; }
+
+// Waits until the first n (uniform, N at most) of the slots that lie W apart hold maps, and hands them to `take` in their order.
 // The wait ends: a workgroup draws its chunk from a counter, so the chunks before that of one that runs have all been started, and
 // the lowest of them waits for nobody.  Should a slot stay empty for some seconds all the same, its map is NaN: the launch ends, and
 // says so in its results.
-__device__ __forceinline__ Map taken(const unsigned long long* slot, unsigned long long v) {
-    for (int tries = 0; (unsigned)v == EMPTY; ++tries) {
-        if (tries > (1 << 22)) return {__uint_as_float(0x7fc00000u), __uint_as_float(0x7fc00000u)};
+template <int N, typename F> __device__ __forceinline__ void take_maps(const unsigned long long* slots, int W, int n, F take) {
+    unsigned long long v[N];
+    for (int tries = 0;; ++tries) {
+        bool holds = true;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (i < n) v[i] = peek(slots + (long long)i * W);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (i < n && (unsigned)v[i] == EMPTY) holds = false;
+        if (holds || tries > (1 << 22)) break;
         __builtin_amdgcn_s_sleep(1);
-        v = peek(slot);
     }
-    return {__uint_as_float((unsigned)v), __uint_as_float((unsigned)(v >> 32))};
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        if (i < n) take(unpacked(v[i]));        // the empty pattern itself is a NaN
 }
 
 // How a chunk learns the state before it, without a chain through all chunks and in one order of arithmetic whatever the timing:
@@ -86,46 +103,42 @@ __device__ __forceinline__ Slots slots_at(unsigned long long* all, int row, int 
 
 // Hands out what others wait for of chunk k (counted in the order in which the chunks are drawn), and returns the map of the chunks
 // before it in its group.
-template <int W> __device__ __forceinline__ Map map_in_group(const Slots& s, int k, int chunks, Map own) {
+template <int W, bool SEG> __device__ __forceinline__ Map map_in_group(const Slots& s, int k, int chunks, Map own) {
     const int at = k % GROUP;
     const bool more = k + 1 < chunks, last = at == GROUP - 1;
     if (more && !last) publish(s.chunk + (long long)k * W, own);
-    unsigned long long v[GROUP - 1];
-#pragma unroll
-    for (int i = 0; i < GROUP - 1; ++i)
-        if (i < at) v[i] = peek(s.chunk + (long long)(k - at + i) * W);
     Map all{0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < GROUP - 1; ++i)
-        if (i < at) all = join(all, taken(s.chunk + (long long)(k - at + i) * W, v[i]));
-    if (more && last && k / GROUP % GROUP != GROUP - 1) publish(s.group + (long long)(k / GROUP) * W, join(all, own));
+    for (int i = 0; i < at; i += GROUP / 2)         // 8 at a time: 15 at once cost 14 registers more, and a wave per SIMD with them
+        take_maps<GROUP / 2>(s.chunk + (long long)(k - at + i) * W, W, min(at - i, GROUP / 2), [&](Map m) { all = join<SEG>(all, m); });
+    if (more && last && k / GROUP % GROUP != GROUP - 1) publish(s.group + (long long)(k / GROUP) * W, join<SEG>(all, own));
     return all;
 }
-// The state before the group of chunk k; `first` before chunk 0.
-template <int W> __device__ __forceinline__ float state_before_group(const Slots& s, int k, float first) {
-    const int section = k / (GROUP * GROUP), g0 = section * GROUP, n = k / GROUP - g0;
-    unsigned long long v[GROUP - 1];
-#pragma unroll
-    for (int i = 0; i < GROUP - 1; ++i)
-        if (i < n) v[i] = peek(s.group + (long long)(g0 + i) * W);
+// The state before the group of chunk k as far as the first 8 groups of its section lead, `first` before chunk 0, and the map of
+// the section's other groups before it.
+template <int W, bool SEG> __device__ __forceinline__ float state_before_groups(const Slots& s, int k, float first) {
+    const int section = k / (GROUP * GROUP), g0 = section * GROUP, n = min(k / GROUP - g0, GROUP / 2);
     float h = first;
-    if (section) {
-        const unsigned long long* at = s.section + (long long)(section - 1) * W;
-        h = taken(at, peek(at)).b;
-    }
-#pragma unroll
-    for (int i = 0; i < GROUP - 1; ++i)
-        if (i < n) h = apply(taken(s.group + (long long)(g0 + i) * W, v[i]), h);
+    if (section) take_maps<1>(s.section + (long long)(section - 1) * W, W, 1, [&](Map m) { h = m.b; });
+    take_maps<GROUP / 2>(s.group + (long long)g0 * W, W, n, [&](Map m) { h = apply<SEG>(m, h); });
     return h;
+}
+template <int W, bool SEG> __device__ __forceinline__ Map map_of_groups(const Slots& s, int k) {
+    const int g0 = k / (GROUP * GROUP) * GROUP + GROUP / 2, n = k / GROUP - g0;
+    Map all{0.f, 0.f};
+    take_maps<GROUP / 2 - 1>(s.group + (long long)g0 * W, W, n, [&](Map m) { all = join<SEG>(all, m); });
+    return all;
 }
 __device__ __forceinline__ bool ends_section(int k, int chunks) { return (k + 1) % (GROUP * GROUP) == 0 && k + 1 < chunks; }
 
 // ---- the shape of a workgroup -------------------------------------------------------------------------------------------------
-// 4 waves of 4 stretches of L steps; a stretch is 16 lanes, a row of the wave, along the channels.  A lane holds V channels, so that
-// a tile is 64 channels wide: 128 bytes of a 16-bit type, 256 of float32.  The last lane of a tile that ends in no multiple of V
+// 4 waves of 4 stretches of L steps; a stretch is 16 lanes, a row of the wave, along the channels.  A lane holds V = 4 channels, so
+// that a tile is 64 channels wide: 128 bytes of a 16-bit type, 256 of float32 (8 channels a lane and 4 steps, for rows of 256 bytes
+// of a 16-bit type too, took 213 us for 185 forward and 506 for 316 backward, bf16 8 x 24064 x 512: more maps to join per step).
+// Registers decide how many workgroups share a CU: 3 forward and 2 backward, each with 32 steps x channels a thread.  Half the steps
+// and 3 workgroups backward took 356 us for 316.  The last lane of a tile that ends in no multiple of V
 // starts earlier and shares channels with its neighbour (both compute and write the same); V = 1 is for rows narrower than 4.
 constexpr int WAVES = 4, THREADS = 64 * WAVES, LANES = 16, STRETCHES = THREADS / LANES;
-constexpr int FWD_L = 8, BWD_L = 4;
+constexpr int L = 8;
 
 // V elements as they stand in memory, packed in as few registers; addresses are a uniform base and 32 bits of a lane's own.
 template <typename E, int V> struct Vec {
@@ -159,18 +172,18 @@ template <typename E, int V> __device__ __forceinline__ void store(E* base, uint
 }
 
 // The maps of a wave's four rows joined in time (BACK: the last row first): of all four, and of those before the own row.
-template <bool BACK> __device__ __forceinline__ void join_rows(Map x, Map& all, Map& before) {
+template <bool BACK, bool SEG> __device__ __forceinline__ void join_rows(Map x, Map& all, Map& before) {
     const auto u = __builtin_amdgcn_permlane16_swap(__float_as_uint(x.u), __float_as_uint(x.u), false, false);     // rows 0 0 2 2 | 1 1 3 3
     const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x.b), __float_as_uint(x.b), false, false);
     const Map even{__uint_as_float(u[0]), __uint_as_float(b[0])}, odd{__uint_as_float(u[1]), __uint_as_float(b[1])};
-    const Map pair = BACK ? join(odd, even) : join(even, odd);
+    const Map pair = BACK ? join<SEG>(odd, even) : join<SEG>(even, odd);
     const auto pu = __builtin_amdgcn_permlane32_swap(__float_as_uint(pair.u), __float_as_uint(pair.u), false, false);  // rows 0 1 0 1 | 2 3 2 3
     const auto pb = __builtin_amdgcn_permlane32_swap(__float_as_uint(pair.b), __float_as_uint(pair.b), false, false);
     const Map low{__uint_as_float(pu[0]), __uint_as_float(pb[0])}, high{__uint_as_float(pu[1]), __uint_as_float(pb[1])};
     const int row = (threadIdx.x / LANES) & 3;
-    all = BACK ? join(high, low) : join(low, high);
+    all = BACK ? join<SEG>(high, low) : join<SEG>(low, high);
     before = (row & 1) != BACK ? (BACK ? odd : even) : Map{0.f, 0.f};
-    if ((row >> 1) != BACK) before = join(BACK ? high : low, before);
+    if ((row >> 1) != BACK) before = join<SEG>(BACK ? high : low, before);
 }
 
 struct Place { int b, tile, chunk, row; };
@@ -196,35 +209,34 @@ template <bool BACK> __device__ __forceinline__ Place draw_place(const RecArgs& 
     return p;
 }
 
-// What stands in a thread's stretch: live steps from its first, and which of them begin an utterance.
-struct Stretch { int t0, live, begins; };
-template <int L> __device__ __forceinline__ Stretch stretch_of(const RecArgs& a, int b, int t0) {
-    Stretch s{t0, 0, 0};
-    const int n = a.lengths ? min(a.lengths[b], a.T) : a.T;
-    s.live = max(0, min(L, n - t0));
-    if (a.seg_start) {
-        const int* m = a.seg_start + (long long)b * a.T;
-#pragma unroll
-        for (int l = 0; l < L; ++l)
-            if (l < s.live && m[t0 + l] == t0 + l) s.begins |= 1 << l;
-    }
-    return s;
+// Of a thread's stretch from step t0 on: how many of its steps are live, and which of them begin an utterance.
+__device__ __forceinline__ int live_steps(const RecArgs& a, int b, int t0) {
+    return max(0, min(L, (a.lengths ? min(a.lengths[b], a.T) : a.T) - t0));
+}
+// The wave's 32 entries of the map in one load (asked for ahead of the data), a lane each; a stretch takes its 8 bits of the ballot.
+template <bool SEG> __device__ __forceinline__ int map_entry(const RecArgs& a, int b, int chunk) {
+    const int t = chunk * (STRETCHES * L) + threadIdx.x / 64 * (4 * L) + threadIdx.x % 64;
+    return SEG && threadIdx.x % 64 < 4 * L && t < a.T ? a.seg_start[(long long)b * a.T + t] - t : 1;
+}
+template <bool SEG> __device__ __forceinline__ int begins_in(int entry, int live) {
+    static_assert(L == 8, "a stretch is a byte of the ballot");
+    return SEG ? (int)(__ballot(entry == 0) >> (threadIdx.x / LANES % 4 * L)) & ((1 << live) - 1) : 0;
 }
 
 // One chunk of one tile.  Each thread reduces its stretch to a map, the wave joins its four, wave 0 the chunk's and its group's while
-// wave 1 finds the state before the group; then each thread knows the state before its stretch and runs over it again, out of its
+// waves 1 and 2 find the state before the group; then each thread knows the state before its stretch and runs over it again, out of its
 // registers.  z is read once.
-template <typename E, int G, int V>
-__global__ void __launch_bounds__(THREADS, sizeof(E) == 4 ? 3 : 4) wnv_recurrence_fwd(RecArgs a) {
-    constexpr int L = FWD_L, W = LANES * V;
-    __shared__ Map totals[WAVES][W], prev[W];
+template <typename E, int G, int V, bool SEG>
+__global__ void __launch_bounds__(THREADS, SEG && sizeof(E) == 2 ? 4 : 3) wnv_recurrence_fwd(RecArgs a) {
+    constexpr int W = LANES * V;
+    __shared__ Map totals[WAVES][W], prev[W], groups[W];
     __shared__ float base[W];
     const int tid = threadIdx.x, lane = tid % LANES, wave = tid / 64, at = lane * V;
     const Place p = draw_place<false>(a, W);
     const bool on = p.tile * W + at < a.C;
     const int c = min(p.tile * W + at, a.C - V);
-    const Stretch s = stretch_of<L>(a, p.b, p.chunk * (STRETCHES * L) + tid / LANES * L);
-    const int live = on ? s.live : 0;
+    const int t0 = p.chunk * (STRETCHES * L) + tid / LANES * L, steps = live_steps(a, p.b, t0), live = on ? steps : 0;
+    const int entry = map_entry<SEG>(a, p.b, p.chunk);
     const E* z = (const E*)a.z + (long long)p.b * a.zb + (long long)p.chunk * (STRETCHES * L) * a.zt;
     const uint32_t from = (uint32_t)(tid / LANES * L * a.zt + c) * (uint32_t)sizeof(E);
 
@@ -236,6 +248,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(E) == 4 ? 3 : 4) wnv_recurrenc
             v[l] = load<E, V>(z + l * a.zt + a.C, from);
             if (G == 3) o[l] = load<E, V>(z + l * a.zt + 2 * a.C, from);
         }
+    const int begins = begins_in<SEG>(entry, steps);
     float u[L][V];
     Map m[V], before[V];
 #pragma unroll
@@ -246,45 +259,45 @@ __global__ void __launch_bounds__(THREADS, sizeof(E) == 4 ? 3 : 4) wnv_recurrenc
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 u[l][i] = wnv_gate(-f[l].get(i));
-                if (s.begins >> l & 1) m[i].b = 0.f;
+                if (SEG && begins >> l & 1) m[i].b = 0.f;
                 m[i].u = fmaf(-u[l][i], m[i].u, m[i].u + u[l][i]);
                 m[i].b = fmaf(u[l][i], v[l].get(i) - m[i].b, m[i].b);
             }
         }
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        if (s.begins) m[i].u = -1.f;
+        if (SEG && begins) m[i].u = -1.f;
         Map all;
-        join_rows<false>(m[i], all, before[i]);
+        join_rows<false, SEG>(m[i], all, before[i]);
         if (tid % 64 < LANES) totals[wave][at + i] = all;
     }
     __syncthreads();
     const int ch = tid % 64;
-    if (wave < 2 && ch < W) {
+    if (wave < 3 && ch < W) {
         const Slots slots = slots_at(a.slots, p.row, a.chunks, W, ch);
         if (wave == 0) {
             Map all = totals[0][ch];
 #pragma unroll
-            for (int w = 1; w < WAVES; ++w) all = join(all, totals[w][ch]);
-            prev[ch] = map_in_group<W>(slots, p.chunk, a.chunks, all);
-        } else {
+            for (int w = 1; w < WAVES; ++w) all = join<SEG>(all, totals[w][ch]);
+            prev[ch] = map_in_group<W, SEG>(slots, p.chunk, a.chunks, all);
+        } else if (wave == 1) {
             const bool there = p.tile * W + ch / V * V < a.C;
-            base[ch] = state_before_group<W>(slots, p.chunk, a.h0 && there ? a.h0[p.b * a.h0b + min(p.tile * W + ch / V * V, a.C - V) + ch % V] : 0.f);
+            base[ch] = state_before_groups<W, SEG>(slots, p.chunk, a.h0 && there ? a.h0[p.b * a.h0b + min(p.tile * W + ch / V * V, a.C - V) + ch % V] : 0.f);
+        } else {
+            groups[ch] = map_of_groups<W, SEG>(slots, p.chunk);
         }
     }
     __syncthreads();
 
-    constexpr int EVERY = BWD_L * WAVES / L;            // waves between two states that the backward pass starts from
-    const int saves = (a.T + BWD_L * STRETCHES - 1) / (BWD_L * STRETCHES), save = p.chunk * (WAVES / EVERY) + wave / EVERY;
     float h[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        h[i] = apply(prev[at + i], base[at + i]);
-        for (int w = 0; w < wave; ++w) h[i] = apply(totals[w][at + i], h[i]);
-        if (a.saved && tid % (64 * EVERY) < LANES && save < saves) a.saved[((long long)p.row * saves + save) * W + at + i] = h[i];
-        h[i] = apply(before[i], h[i]);
+        h[i] = apply<SEG>(prev[at + i], apply<SEG>(groups[at + i], base[at + i]));
+        if (a.saved && tid < LANES) a.saved[((long long)p.row * a.chunks + p.chunk) * W + at + i] = h[i];
+        for (int w = 0; w < wave; ++w) h[i] = apply<SEG>(totals[w][at + i], h[i]);
+        h[i] = apply<SEG>(before[i], h[i]);
         if (tid >= THREADS - LANES) {                   // the chunk's last stretch: the state behind it
-            const float last = apply(m[i], h[i]);
+            const float last = apply<SEG>(m[i], h[i]);
             if (ends_section(p.chunk, a.chunks))
                 publish(slots_at(a.slots, p.row, a.chunks, W, at + i).section + (long long)(p.chunk / (GROUP * GROUP)) * W, {-1.f, last});
             if (p.chunk + 1 == a.chunks && on) a.h_last[(long long)p.b * a.C + c + i] = last;
@@ -294,13 +307,13 @@ __global__ void __launch_bounds__(THREADS, sizeof(E) == 4 ? 3 : 4) wnv_recurrenc
     const uint32_t to = (uint32_t)(tid / LANES * L * a.C + c) * (uint32_t)sizeof(E);
 #pragma unroll
     for (int l = 0; l < L; ++l)
-        if (on && s.t0 + l < a.T) {
+        if (on && t0 + l < a.T) {
             float out[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 float q = 0.f;
                 if (l < live) {
-                    if (s.begins >> l & 1) h[i] = 0.f;
+                    if (SEG && begins >> l & 1) h[i] = 0.f;
                     h[i] = fmaf(u[l][i], v[l].get(i) - h[i], h[i]);
                     q = h[i];
                     if (G == 3) q *= wnv_gate(o[l].get(i));
@@ -315,18 +328,18 @@ __global__ void __launch_bounds__(THREADS, sizeof(E) == 4 ? 3 : 4) wnv_recurrenc
 // df = dh (h_{t-1} - v) sigmoid(f) u;  dv = dh u;  do = dy h sigmoid(o) (1 - sigmoid(o))
 // The chunks run from the last to the first, r is found the way the forward pass finds h; h itself starts from the state that the
 // forward pass saved before each chunk and is run through again.
-template <typename E, int G, int V>
-__global__ void __launch_bounds__(THREADS, 3) wnv_recurrence_bwd(RecArgs a) {
-    constexpr int L = BWD_L, W = LANES * V;
-    __shared__ Map ahead[WAVES][W], back[WAVES][W], prev[W];        // of h and of r
+template <typename E, int G, int V, bool SEG>
+__global__ void __launch_bounds__(THREADS, 2) wnv_recurrence_bwd(RecArgs a) {
+    constexpr int W = LANES * V;
+    __shared__ Map ahead[WAVES][W], back[WAVES][W], prev[W], groups[W];        // of h and of r
     __shared__ float base[W];
     const int tid = threadIdx.x, lane = tid % LANES, wave = tid / 64, at = lane * V;
     const Place p = draw_place<true>(a, W);
     const int order = a.chunks - 1 - p.chunk;
     const bool on = p.tile * W + at < a.C;
     const int c = min(p.tile * W + at, a.C - V);
-    const Stretch s = stretch_of<L>(a, p.b, p.chunk * (STRETCHES * L) + tid / LANES * L);
-    const int live = on ? s.live : 0;
+    const int t0 = p.chunk * (STRETCHES * L) + tid / LANES * L, steps = live_steps(a, p.b, t0), live = on ? steps : 0;
+    const int entry = map_entry<SEG>(a, p.b, p.chunk);
     const E* z = (const E*)a.z + (long long)p.b * a.zb + (long long)p.chunk * (STRETCHES * L) * a.zt;
     const E* dy = (const E*)a.dy + (long long)p.b * a.dyb + (long long)p.chunk * (STRETCHES * L) * a.dyt;
     const uint32_t from = (uint32_t)(tid / LANES * L * a.zt + c) * (uint32_t)sizeof(E);
@@ -342,6 +355,7 @@ __global__ void __launch_bounds__(THREADS, 3) wnv_recurrence_bwd(RecArgs a) {
             if (a.dy) d[l] = load<E, V>(dy + l * a.dyt, dfrom);
         }
     const Vec<float, V> saved = load<float, V>(a.saved + ((long long)p.row * a.chunks + p.chunk) * W, at * 4);
+    const int begins = begins_in<SEG>(entry, steps);
     float u[L][V], uk[L][V], g[L][V], q[L][V];          // u sigmoid(f); dy sigmoid(o); dy sigmoid(o) (1 - sigmoid(o))
     Map m[V], r[V];
 #pragma unroll
@@ -352,7 +366,7 @@ __global__ void __launch_bounds__(THREADS, 3) wnv_recurrence_bwd(RecArgs a) {
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 u[l][i] = wnv_gate(-f[l].get(i), uk[l][i]);
-                if (s.begins >> l & 1) m[i].b = 0.f;
+                if (SEG && begins >> l & 1) m[i].b = 0.f;
                 m[i].u = fmaf(-u[l][i], m[i].u, m[i].u + u[l][i]);
                 m[i].b = fmaf(u[l][i], v[l].get(i) - m[i].b, m[i].b);
                 g[l][i] = a.dy ? d[l].get(i) : 0.f;
@@ -369,31 +383,33 @@ __global__ void __launch_bounds__(THREADS, 3) wnv_recurrence_bwd(RecArgs a) {
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 const float dh = g[l][i] + r[i].b;
-                r[i].b = s.begins >> l & 1 ? 0.f : fmaf(-u[l][i], dh, dh);
+                r[i].b = SEG && begins >> l & 1 ? 0.f : fmaf(-u[l][i], dh, dh);
             }
         }
     Map h_before[V], r_before[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        if (s.begins) m[i].u = -1.f;
+        if (SEG && begins) m[i].u = -1.f;
         r[i].u = m[i].u;
         Map all, all_back;
-        join_rows<false>(m[i], all, h_before[i]);
-        join_rows<true>(r[i], all_back, r_before[i]);
+        join_rows<false, SEG>(m[i], all, h_before[i]);
+        join_rows<true, SEG>(r[i], all_back, r_before[i]);
         if (tid % 64 < LANES) ahead[wave][at + i] = all, back[wave][at + i] = all_back;
     }
     __syncthreads();
     const int ch = tid % 64;
-    if (wave < 2 && ch < W) {
+    if (wave < 3 && ch < W) {
         const Slots slots = slots_at(a.slots, p.row, a.chunks, W, ch);
         if (wave == 0) {
             Map all = back[WAVES - 1][ch];
 #pragma unroll
-            for (int w = WAVES - 2; w >= 0; --w) all = join(all, back[w][ch]);
-            prev[ch] = map_in_group<W>(slots, order, a.chunks, all);
-        } else {
+            for (int w = WAVES - 2; w >= 0; --w) all = join<SEG>(all, back[w][ch]);
+            prev[ch] = map_in_group<W, SEG>(slots, order, a.chunks, all);
+        } else if (wave == 1) {
             const bool there = p.tile * W + ch / V * V < a.C;
-            base[ch] = state_before_group<W>(slots, order, a.dh_last && there ? a.dh_last[(long long)p.b * a.C + min(p.tile * W + ch / V * V, a.C - V) + ch % V] : 0.f);
+            base[ch] = state_before_groups<W, SEG>(slots, order, a.dh_last && there ? a.dh_last[(long long)p.b * a.C + min(p.tile * W + ch / V * V, a.C - V) + ch % V] : 0.f);
+        } else {
+            groups[ch] = map_of_groups<W, SEG>(slots, order);
         }
     }
     __syncthreads();
@@ -402,13 +418,13 @@ __global__ void __launch_bounds__(THREADS, 3) wnv_recurrence_bwd(RecArgs a) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         float h = saved.get(i);
-        x[i] = apply(prev[at + i], base[at + i]);
-        for (int w = 0; w < wave; ++w) h = apply(ahead[w][at + i], h);
-        for (int w = WAVES - 1; w > wave; --w) x[i] = apply(back[w][at + i], x[i]);
-        h = apply(h_before[i], h);
-        x[i] = apply(r_before[i], x[i]);
+        x[i] = apply<SEG>(prev[at + i], apply<SEG>(groups[at + i], base[at + i]));
+        for (int w = 0; w < wave; ++w) h = apply<SEG>(ahead[w][at + i], h);
+        for (int w = WAVES - 1; w > wave; --w) x[i] = apply<SEG>(back[w][at + i], x[i]);
+        h = apply<SEG>(h_before[i], h);
+        x[i] = apply<SEG>(r_before[i], x[i]);
         if (tid < LANES) {                              // the chunk's first stretch: what flows out of it
-            const float out = apply(r[i], x[i]);
+            const float out = apply<SEG>(r[i], x[i]);
             if (ends_section(order, a.chunks))
                 publish(slots_at(a.slots, p.row, a.chunks, W, at + i).section + (long long)(order / (GROUP * GROUP)) * W, {-1.f, out});
             if (p.chunk == 0 && a.dh0 && on) a.dh0[(long long)p.b * a.C + c + i] = out;
@@ -416,7 +432,7 @@ __global__ void __launch_bounds__(THREADS, 3) wnv_recurrence_bwd(RecArgs a) {
 #pragma unroll
         for (int l = 0; l < L; ++l)
             if (l < live) {
-                before[l][i] = s.begins >> l & 1 ? 0.f : h;
+                before[l][i] = SEG && begins >> l & 1 ? 0.f : h;
                 h = fmaf(u[l][i], v[l].get(i) - before[l][i], before[l][i]);
             }
     }
@@ -424,7 +440,7 @@ __global__ void __launch_bounds__(THREADS, 3) wnv_recurrence_bwd(RecArgs a) {
     const uint32_t to = (uint32_t)(tid / LANES * L * G * a.C + c) * (uint32_t)sizeof(E);
 #pragma unroll
     for (int l = L - 1; l >= 0; --l)
-        if (on && s.t0 + l < a.T) {
+        if (on && t0 + l < a.T) {
             float df[V], dv[V], dg[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) {
@@ -434,7 +450,7 @@ __global__ void __launch_bounds__(THREADS, 3) wnv_recurrence_bwd(RecArgs a) {
                     xf = -dh * w * uk[l][i];
                     xv = dh * u[l][i];
                     if (G == 3) xo = q[l][i] * fmaf(u[l][i], w, before[l][i]);
-                    x[i] = s.begins >> l & 1 ? 0.f : fmaf(-u[l][i], dh, dh);
+                    x[i] = SEG && begins >> l & 1 ? 0.f : fmaf(-u[l][i], dh, dh);
                 }
                 df[i] = xf;
                 dv[i] = xv;
@@ -497,24 +513,26 @@ wnv_status check_strides(const char* who, const wnv_recurrence_args* a) {
     return WNV_OK;
 }
 
-int width_of(int C) { return C < 4 ? LANES : LANES * 4; }
-int chunks_of(int64_t T, int L) { return (int)((T + STRETCHES * L - 1) / (STRETCHES * L)); }
-int64_t slot_bytes(int64_t B, int64_t T, int C, int L) {
-    const int n = chunks_of(T, L), W = width_of(C);
-    return n > 1 ? B * ((C + W - 1) / W) * slots_of_row(n, W) * 8 : 0;
+struct Cut { int W, tiles, chunks; };
+Cut cut_of(int64_t T, int C) {
+    Cut c;
+    c.W = LANES * (C < 4 ? 1 : 4);
+    c.tiles = (C + c.W - 1) / c.W;
+    c.chunks = (int)((T + STRETCHES * L - 1) / (STRETCHES * L));
+    return c;
 }
+int64_t slot_bytes(int64_t B, const Cut& c) { return c.chunks > 1 ? B * c.tiles * slots_of_row(c.chunks, c.W) * 8 : 0; }
 
-// The kernel's arguments for chunks of STRETCHES * L steps; the workspace is filled on the way.
-wnv_status prepare(const char* who, const wnv_recurrence_args* a, int L, RecArgs& k) {
+// The kernel's arguments; the workspace is filled on the way.
+wnv_status prepare(const char* who, const wnv_recurrence_args* a, const Cut& c, RecArgs& k) {
     k.B = a->B; k.C = a->C; k.T = (int)a->T;
-    k.tiles = (a->C + width_of(a->C) - 1) / width_of(a->C);
-    k.chunks = chunks_of(a->T, L);
+    k.tiles = c.tiles; k.chunks = c.chunks;
     k.zb = a->z_batch_stride; k.zt = a->T > 1 ? a->z_time_stride : 0; k.h0b = a->h0_batch_stride;
     k.z = a->z; k.h0 = a->h0; k.lengths = a->lengths; k.seg_start = a->seg_start;
     k.y = a->y; k.h_last = a->h_last; k.saved = (float*)a->saved; k.slots = (unsigned long long*)a->workspace;
     k.dy = a->dy; k.dyb = a->dy_batch_stride; k.dyt = a->T > 1 ? a->dy_time_stride : 0;
     k.dh_last = a->dh_last; k.dz = a->dz; k.dh0 = a->dh0;
-    const int64_t blocks = (int64_t)k.B * k.tiles * k.chunks, bytes = slot_bytes(a->B, a->T, a->C, L);
+    const int64_t blocks = (int64_t)k.B * k.tiles * k.chunks, bytes = slot_bytes(a->B, c);
     if (blocks >= (1 << 24)) return fail(WNV_ERR_UNSUPPORTED, "%s: B x T x C is too large", who);
     if (bytes) {
         if (!a->workspace) return fail(WNV_ERR_INVALID_ARG, "%s: workspace is NULL", who);
@@ -524,30 +542,34 @@ wnv_status prepare(const char* who, const wnv_recurrence_args* a, int L, RecArgs
     return WNV_OK;
 }
 
+template <typename E, int G, int V> void launch(bool back, const wnv_recurrence_args* a, const RecArgs& k) {
+    const dim3 grid((unsigned)((int64_t)k.B * k.tiles * k.chunks)), block(THREADS);
+    hipStream_t s = (hipStream_t)a->stream;
+    if (back) {
+        if (a->seg_start) hipLaunchKernelGGL((wnv_recurrence_bwd<E, G, V, true>), grid, block, 0, s, k);
+        else hipLaunchKernelGGL((wnv_recurrence_bwd<E, G, V, false>), grid, block, 0, s, k);
+    } else {
+        if (a->seg_start) hipLaunchKernelGGL((wnv_recurrence_fwd<E, G, V, true>), grid, block, 0, s, k);
+        else hipLaunchKernelGGL((wnv_recurrence_fwd<E, G, V, false>), grid, block, 0, s, k);
+    }
+}
+template <typename E> void launch(bool back, const wnv_recurrence_args* a, const RecArgs& k) {
+    if (a->gates == 3) a->C < 4 ? launch<E, 3, 1>(back, a, k) : launch<E, 3, 4>(back, a, k);
+    else a->C < 4 ? launch<E, 2, 1>(back, a, k) : launch<E, 2, 4>(back, a, k);
+}
+
 }  // namespace
 
 extern "C" int64_t wnv_recurrence_saved_bytes(int32_t B, int64_t T, int32_t C, int32_t gates, int32_t dtype) {
     if (check_shape("wnv_recurrence_saved_bytes", 0, B, T, C, gates, dtype) != WNV_OK) return -1;
-    const int W = width_of(C);
-    return (int64_t)B * ((C + W - 1) / W) * chunks_of(T, BWD_L) * W * 4;
+    const Cut c = cut_of(T, C);
+    return (int64_t)B * c.tiles * c.chunks * c.W * 4;
 }
 
 extern "C" int64_t wnv_recurrence_workspace_bytes(int32_t B, int64_t T, int32_t C, int32_t gates, int32_t dtype) {
     if (check_shape("wnv_recurrence_workspace_bytes", 0, B, T, C, gates, dtype) != WNV_OK) return -1;
-    return std::max(slot_bytes(B, T, C, FWD_L), slot_bytes(B, T, C, BWD_L));
+    return slot_bytes(B, cut_of(T, C));
 }
-
-#define WNV_LAUNCH_BY_SHAPE(kernel, a, k)                                                                                       \
-    do {                                                                                                                        \
-        const dim3 grid((unsigned)((int64_t)k.B * k.tiles * k.chunks));                                                         \
-        hipStream_t s = (hipStream_t)a->stream;                                                                                 \
-        WNV_BY_TYPE(a->dtype, {                                                                                                 \
-            if (a->gates == 3 && a->C >= 4) hipLaunchKernelGGL((kernel<E, 3, 4>), grid, dim3(THREADS), 0, s, k);                 \
-            else if (a->gates == 3) hipLaunchKernelGGL((kernel<E, 3, 1>), grid, dim3(THREADS), 0, s, k);                         \
-            else if (a->C >= 4) hipLaunchKernelGGL((kernel<E, 2, 4>), grid, dim3(THREADS), 0, s, k);                             \
-            else hipLaunchKernelGGL((kernel<E, 2, 1>), grid, dim3(THREADS), 0, s, k);                                            \
-        });                                                                                                                     \
-    } while (0)
 
 extern "C" wnv_status wnv_recurrence_forward(int32_t device, const wnv_recurrence_args* a) {
     if (!a || !a->z || !a->y || !a->h_last) return fail(WNV_ERR_INVALID_ARG, "wnv_recurrence_forward: NULL argument");
@@ -556,8 +578,9 @@ extern "C" wnv_status wnv_recurrence_forward(int32_t device, const wnv_recurrenc
     DeviceGuard guard(device);
     if (!guard.ok) return fail(WNV_ERR_HIP, "wnv_recurrence_forward: cannot select device %d", device);
     RecArgs k{};
-    if (wnv_status st = prepare("wnv_recurrence_forward", a, FWD_L, k)) return st;
-    WNV_LAUNCH_BY_SHAPE(wnv_recurrence_fwd, a, k);
+    const Cut c = cut_of(a->T, a->C);
+    if (wnv_status st = prepare("wnv_recurrence_forward", a, c, k)) return st;
+    WNV_BY_TYPE(a->dtype, launch<E>(false, a, k));
     return launched("wnv_recurrence_forward");
 }
 
@@ -568,8 +591,9 @@ extern "C" wnv_status wnv_recurrence_backward(int32_t device, const wnv_recurren
     DeviceGuard guard(device);
     if (!guard.ok) return fail(WNV_ERR_HIP, "wnv_recurrence_backward: cannot select device %d", device);
     RecArgs k{};
-    if (wnv_status st = prepare("wnv_recurrence_backward", a, BWD_L, k)) return st;
-    WNV_LAUNCH_BY_SHAPE(wnv_recurrence_bwd, a, k);
+    const Cut c = cut_of(a->T, a->C);
+    if (wnv_status st = prepare("wnv_recurrence_backward", a, c, k)) return st;
+    WNV_BY_TYPE(a->dtype, launch<E>(true, a, k));
     return launched("wnv_recurrence_backward");
 }
 
