@@ -1,10 +1,17 @@
 // wnv_q4.hip -- products of a few rows with weights of 4 bits: y = x W^T + bias, W[n, k] = scale[n, k/g] (code[n, k] - zero[n, k/g]),
 // and the step of the gated recurrence (wnv_recurrence.hip) straight behind the product with its gates.
 //
+// The matrix instruction does the dot products, with the weights as its rows and up to 16 rows of x as its columns, so that a code
+// costs a shift and an and-or per pair, and not an operation per code and row of x: a 16-bit float 16 + code is a mask and a constant
+// away from the code (bf16: 0x4180 | code << 3, f16: 0x4c00 | code << 6), exact, and a second instruction with -(16 + zero) in every
+// place takes the offset out again: the sum of x (code - zero) over a group, in float32, which the group's scale then joins to the
+// rest.  float32 x is cut into three bf16 parts that add up to it exactly; they share the weights.
+//
 // Weights are laid out once, in tiles of 16 rows x 128 inputs: lane l of a wave holds row l % 16 and, in word j of its 16 bytes, the
 // inputs 32 j + 8 (l / 16) ... + 7 of the tile -- what a 16 x 16 x 32 matrix instruction wants of a lane.  Inputs 2p and 2p + 1 of a
 // word sit at bits 4p and 16 + 4p.  The rows of each gate are padded to a multiple of 16, so that one tile of each gate holds the
-// same channels; scales and zero points are stored [tile][group][16 rows], the bias [tile][16 rows].
+// same channels.  Behind a tile's codes, in arrays of their own: its scales as [4 rows of a result lane][group], its zero points as
+// [row][group], its bias.
 #include <hip/hip_runtime.h>
 
 #include "wnv_hostutil.h"
@@ -14,17 +21,25 @@ namespace {
 
 struct Q4Dev {
     int cin, rows, gates, group;    // rows: of one gate
-    int tiles, kb, groups;          // tiles of one gate, 128-wide blocks and groups along the inputs (padded)
+    int tiles, kb;                  // tiles of one gate, 128-wide blocks along the inputs
+    int per_block;                  // groups in a block: 128 / group
     const uint4* codes;             // [gates * tiles][kb][64]
-    const wnv_bf16* scales;         // [gates * tiles][groups][16]
-    const uint8_t* zeros;           // [gates * tiles][groups][16]
+    const wnv_bf16* scales;         // [gates * tiles][kb][4][per_block][4]: row 4 a + b at [a][group][b]
+    const uint8_t* zeros;           // [gates * tiles][kb][16][per_block]
     const float* bias;              // [gates * tiles][16]
 };
+
+__device__ __forceinline__ long long scale_at(const Q4Dev& q, long long tile, int group, int row) {
+    return (((tile * q.kb + group / q.per_block) * 4 + row / 4) * q.per_block + group % q.per_block) * 4 + row % 4;
+}
+__device__ __forceinline__ long long zero_at(const Q4Dev& q, long long tile, int group, int row) {
+    return ((tile * q.kb + group / q.per_block) * 16 + row) * q.per_block + group % q.per_block;
+}
 
 __global__ void __launch_bounds__(256) wnv_q4_pack(const uint8_t* codes, const wnv_bf16* scales, const uint8_t* zeros, const float* bias,
                                                    Q4Dev q, int n_groups, uint32_t* pcodes, wnv_bf16* pscales, uint8_t* pzeros,
                                                    float* pbias, int* bad) {
-    const long long words = (long long)q.gates * q.tiles * q.kb * 256, gs = (long long)q.gates * q.tiles * q.groups * 16;
+    const long long words = (long long)q.gates * q.tiles * q.kb * 256, gs = (long long)q.gates * q.tiles * q.kb * q.per_block * 16;
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
     if (i < words) {
         const int j = i & 3, lane = (i >> 2) & 63;
@@ -46,7 +61,7 @@ __global__ void __launch_bounds__(256) wnv_q4_pack(const uint8_t* codes, const w
     if (i < gs) {
         const int r = i & 15;
         const long long tg = i >> 4;
-        const int g = tg % q.groups, tile = tg / q.groups, row = (tile % q.tiles) * 16 + r;
+        const int groups = q.kb * q.per_block, g = tg % groups, tile = tg / groups, row = (tile % q.tiles) * 16 + r;
         wnv_bf16 s = (wnv_bf16)0.f;
         uint8_t zp = 0;
         if (row < q.rows && g < n_groups) {
@@ -55,8 +70,8 @@ __global__ void __launch_bounds__(256) wnv_q4_pack(const uint8_t* codes, const w
             zp = zeros ? zeros[src] : 8;
             if (zp > 15) *bad = 1;
         }
-        pscales[i] = s;
-        pzeros[i] = zp;
+        pscales[scale_at(q, tile, g, r)] = s;
+        pzeros[zero_at(q, tile, g, r)] = zp;
     }
     if (i < (long long)q.gates * q.tiles * 16) {
         const int tile = i >> 4, row = (tile % q.tiles) * 16 + (int)(i & 15);
@@ -100,8 +115,8 @@ __global__ void __launch_bounds__(256) wnv_q4_unpack(Q4Dev q, float* w) {
     const long long tile = (n / q.rows) * q.tiles + row / 16;
     const int lane = ((k >> 3) & 3) * 16 + row % 16, j = (k >> 5) & 3, e = k & 7;
     const uint32_t word = ((const uint32_t*)(q.codes + (tile * q.kb + k / 128) * 64 + lane))[j];
-    const long long at = (tile * q.groups + k / q.group) * 16 + row % 16;
-    w[i] = (float)q.scales[at] * ((float)((word >> (4 * (e / 2) + 16 * (e & 1))) & 15) - (float)q.zeros[at]);
+    const float code = (float)((word >> (4 * (e / 2) + 16 * (e & 1))) & 15), zero = (float)q.zeros[zero_at(q, tile, k / q.group, row % 16)];
+    w[i] = (float)q.scales[scale_at(q, tile, k / q.group, row % 16)] * (code - zero);
 }
 
 struct Q4Call {
@@ -112,46 +127,171 @@ struct Q4Call {
     int B;
 };
 
-// One wave per tile of 16 channels and row of x, a lane per weight row and quarter of the inputs.
-template <typename E, int GATES, bool STEP>
-__global__ void __launch_bounds__(64) wnv_q4_rows(Q4Dev q, Q4Call a) {
-    const int lane = threadIdx.x, r = lane % 16, quarter = lane / 16, b = blockIdx.y;
-    const E* x = (const E*)a.x + b * a.xs;
-    float z[GATES];
-    for (int g = 0; g < GATES; ++g) {
-        const long long tile = STEP ? (long long)g * q.tiles + blockIdx.x : blockIdx.x;
-        float acc = 0.f;
-        for (int kb = 0; kb < q.kb; ++kb) {
-            const uint4 w = q.codes[(tile * q.kb + kb) * 64 + lane];
-            const uint32_t words[4] = {w.x, w.y, w.z, w.w};
-            for (int j = 0; j < 4; ++j) {
-                const int k0 = kb * 128 + j * 32 + quarter * 8;
-                const long long at = (tile * q.groups + k0 / q.group) * 16 + r;
-                const float zero = (float)q.zeros[at];
-                float sum = 0.f;
-                for (int e = 0; e < 8; ++e)
-                    if (k0 + e < q.cin)
-                        sum = fmaf(wnv_up(x[k0 + e]), (float)((words[j] >> (4 * (e / 2) + 16 * (e & 1))) & 15) - zero, sum);
-                acc = fmaf((float)q.scales[at], sum, acc);
-            }
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef u32x4 u32x4_any __attribute__((aligned(1)));
+
+// What the kernels need to know of x's type: the 16-bit float that its products run in, and how many parts of that make one x.
+template <typename E> struct Q4Type;
+template <> struct Q4Type<wnv_bf16> { static constexpr int PARTS = 1, AT = 3; static constexpr uint32_t ONE = 0x4180u; };
+template <> struct Q4Type<wnv_f16> { static constexpr int PARTS = 1, AT = 6; static constexpr uint32_t ONE = 0x4c00u; };
+template <> struct Q4Type<float> : Q4Type<wnv_bf16> { static constexpr int PARTS = 3; };
+
+template <typename E> __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+    if constexpr (__is_same(E, wnv_f16))
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// The 8 codes of a word as 16 + code, in the order of x's memory.
+template <typename E> __device__ __forceinline__ u32x4 codes_up(uint32_t w) {
+    constexpr int AT = Q4Type<E>::AT;
+    constexpr uint32_t MASK = 0x000f000fu << AT, ONE = Q4Type<E>::ONE * 0x10001u;
+    u32x4 r;
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+        const uint32_t s = 4 * p <= AT ? w << (AT - 4 * p) : w >> (4 * p - AT);
+        r[p] = (s & MASK) | ONE;
+    }
+    return r;
+}
+template <typename E> __device__ __forceinline__ u32x4 offset_of(uint32_t zero) {        // -(16 + zero), 8 times
+    const uint32_t h = (zero << Q4Type<E>::AT) | Q4Type<E>::ONE | 0x8000u, w = h | h << 16;
+    return u32x4{w, w, w, w};
+}
+
+// Inputs k0 ... k0 + 7 of a row, zeros behind its end; as they stand in memory, cut into parts at their use.
+template <typename E> struct Inputs { u32x4 w[sizeof(E) / 2]; };
+template <typename E> __device__ __forceinline__ Inputs<E> load_inputs(const E* row, int k0, int cin) {
+    Inputs<E> r{};
+    if (k0 + 8 <= cin) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(E) / 2; ++i) r.w[i] = *(const u32x4_any*)((const char*)(row + k0) + 16 * i);
+    } else {
+        E e[8] = {};
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (k0 + i < cin) e[i] = row[k0 + i];
+        __builtin_memcpy(&r, e, sizeof r);
+    }
+    return r;
+}
+template <typename E> __device__ __forceinline__ void parts_of(const Inputs<E>& x, u32x4 (&part)[Q4Type<E>::PARTS]) {
+    if constexpr (sizeof(E) == 2) {
+        part[0] = x.w[0];
+    } else {                            // the upper 8 bits of the 24, of what is left, and of what is left then: nothing remains
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            const uint32_t w0 = x.w[p / 2][p % 2 * 2], w1 = x.w[p / 2][p % 2 * 2 + 1];
+            const float r0 = __uint_as_float(w0) - __uint_as_float(w0 & 0xffff0000u), r1 = __uint_as_float(w1) - __uint_as_float(w1 & 0xffff0000u);
+            const uint32_t m0 = __float_as_uint(r0), m1 = __float_as_uint(r1);
+            const float s0 = r0 - __uint_as_float(m0 & 0xffff0000u), s1 = r1 - __uint_as_float(m1 & 0xffff0000u);
+            part[0][p] = __builtin_amdgcn_perm(w1, w0, 0x07060302u);
+            part[1][p] = __builtin_amdgcn_perm(m1, m0, 0x07060302u);
+            part[2][p] = __builtin_amdgcn_perm(__float_as_uint(s1), __float_as_uint(s0), 0x07060302u);
         }
-        acc += __shfl_xor(acc, 16);
-        acc += __shfl_xor(acc, 32);
-        z[g] = acc + q.bias[tile * 16 + r];
     }
-    if (quarter != 0) return;
-    if (!STEP) {
-        const int gate = blockIdx.x / q.tiles, row = (blockIdx.x % q.tiles) * 16 + r;
-        if (row < q.rows) ((E*)a.y)[((long long)b * q.gates + gate) * q.rows + row] = wnv_down<E>(z[0]);
-        return;
+}
+
+// What a wave reads of the weights for one block of 128 inputs.
+template <int GROUPS> struct Q4Block {
+    uint4 code;
+    uint2 scale[GROUPS];
+    uint32_t zero;
+};
+template <int GROUPS> __device__ __forceinline__ Q4Block<GROUPS> load_block(const Q4Dev& q, long long at, int lane) {
+    Q4Block<GROUPS> f;
+    f.code = q.codes[at * 64 + lane];
+    const uint2* s = (const uint2*)(q.scales + (at * 4 + lane / 16) * GROUPS * 4);
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) f.scale[g] = s[g];
+    const uint8_t* z = q.zeros + (at * 16 + lane % 16) * GROUPS;
+    f.zero = GROUPS == 4 ? *(const uint32_t*)z : GROUPS == 2 ? *(const uint16_t*)z : *z;
+    return f;
+}
+
+// One tile (GATES > 0: one of each gate, of the same 16 channels, and the sums go straight into the recurrence's step) x 16 MT rows
+// of x.  A wave takes a gate and shares out the blocks of 128 inputs with the `split` waves of the same gate; their sums are joined
+// in LDS in the waves' order: no atomics, and a row's result does not depend on the rows beside it (the split goes by the weights'
+// shape alone).  The weights of a wave's next block are asked for before this one's products; x, which every workgroup reads, comes
+// out of L2 at its use.
+template <typename E, int MT, int GROUPS, int GATES>
+__global__ void __launch_bounds__(1024) wnv_q4_rows(Q4Dev q, Q4Call a, int split) {
+    extern __shared__ f32x4 sums[];     // [wave][MT][64]
+    constexpr int PARTS = Q4Type<E>::PARTS, JG = 4 / GROUPS;
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, r = lane % 16, quarter = lane / 16, slice = wave % split;
+    const long long tile = blockIdx.x + (GATES ? wave / split * q.tiles : 0);
+    const int b0 = blockIdx.y * (16 * MT);
+
+    f32x4 acc[MT] = {};
+    Q4Block<GROUPS> f{};
+    if (slice < q.kb) f = load_block<GROUPS>(q, tile * q.kb + slice, lane);
+    for (int kb = slice; kb < q.kb; kb += split) {
+        Q4Block<GROUPS> next{};
+        if (kb + split < q.kb) next = load_block<GROUPS>(q, tile * q.kb + kb + split, lane);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            const int b = b0 + 16 * m + r;
+            const E* x = (const E*)a.x + (long long)min(b, a.B - 1) * a.xs;
+            Inputs<E> in[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) in[j] = b < a.B ? load_inputs<E>(x, kb * 128 + j * 32 + quarter * 8, q.cin) : Inputs<E>{};
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g) {
+                f32x4 sum = {};
+                const u32x4 o = offset_of<E>(f.zero >> (8 * g) & 255);
+#pragma unroll
+                for (int j = g * JG; j < (g + 1) * JG; ++j) {
+                    const u32x4 w = codes_up<E>(j == 0 ? f.code.x : j == 1 ? f.code.y : j == 2 ? f.code.z : f.code.w);
+                    u32x4 part[PARTS];
+                    parts_of<E>(in[j], part);
+#pragma unroll
+                    for (int i = 0; i < PARTS; ++i) {
+                        sum = mfma<E>(w, part[i], sum);
+                        sum = mfma<E>(o, part[i], sum);
+                    }
+                }
+                const uint2 s = f.scale[g];
+                const f32x4 scale{__uint_as_float(s.x << 16), __uint_as_float(s.x & 0xffff0000u), __uint_as_float(s.y << 16),
+                                  __uint_as_float(s.y & 0xffff0000u)};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[m][i] = fmaf(scale[i], sum[i], acc[m][i]);
+            }
+            if (MT > 1) __builtin_amdgcn_sched_barrier(0);      // the rows' loads one tile at a time: all at once do not fit the registers
+        }
+        f = next;
     }
-    const int row = blockIdx.x * 16 + r;
-    if (row >= q.rows) return;
-    float h = a.state[(long long)b * q.rows + row];
-    h = fmaf(wnv_gate(-z[0]), z[GATES > 1 ? 1 : 0] - h, h);
-    a.state[(long long)b * q.rows + row] = h;
-    if (GATES == 3) h *= wnv_gate(z[GATES > 2 ? 2 : 0]);
-    ((E*)a.y)[(long long)b * q.rows + row] = wnv_down<E>(h);
+#pragma unroll
+    for (int m = 0; m < MT; ++m) sums[(wave * MT + m) * 64 + lane] = acc[m];
+    __syncthreads();
+
+    // 16 neighbouring threads write 16 neighbouring outputs of a row; lane l of a result holds its column l % 16, rows 4 (l / 16) ...
+    const float* part = (const float*)sums;
+    for (int e = threadIdx.x; e < MT * 256; e += blockDim.x) {
+        const int n = e % 16, col = e / 16 % 16, m = e / 256, b = b0 + 16 * m + col;
+        const int gate = GATES ? 0 : blockIdx.x / q.tiles, channel = (blockIdx.x - gate * q.tiles) * 16 + n;
+        if (b >= a.B || channel >= q.rows) continue;
+        float z[GATES ? GATES : 1];
+#pragma unroll
+        for (int g = 0; g < (GATES ? GATES : 1); ++g) {
+            const int at = (m * 64 + n / 4 * 16 + col) * 4 + n % 4;
+            float sum = 0.f;
+            for (int w = 0; w < split; ++w) sum += part[at + (g * split + w) * (MT * 256)];
+            z[g] = sum + q.bias[(blockIdx.x + g * q.tiles) * 16 + n];
+        }
+        if (!GATES) {
+            ((E*)a.y)[((long long)b * q.gates + gate) * q.rows + channel] = wnv_down<E>(z[0]);
+        } else {
+            float h = a.state[(long long)b * q.rows + channel];
+            h = fmaf(wnv_gate(-z[0]), z[GATES > 1 ? 1 : 0] - h, h);
+            a.state[(long long)b * q.rows + channel] = h;
+            if (GATES == 3) h *= wnv_gate(z[GATES - 1]);
+            ((E*)a.y)[(long long)b * q.rows + channel] = wnv_down<E>(h);
+        }
+    }
 }
 
 #define WNV_BY_TYPE(dtype, ...)                                                       \
@@ -160,6 +300,26 @@ __global__ void __launch_bounds__(64) wnv_q4_rows(Q4Dev q, Q4Call a) {
         case WNV_BF16: { using E = wnv_bf16; __VA_ARGS__; break; }                    \
         default: { using E = wnv_f16; __VA_ARGS__; break; }                           \
     }
+
+template <typename E, int MT, int GATES> void launch(const Q4Dev& q, const Q4Call& a, int split, hipStream_t s) {
+    const dim3 grid(GATES ? q.tiles : q.gates * q.tiles, (a.B + 16 * MT - 1) / (16 * MT)), block(64 * split * (GATES ? GATES : 1));
+    const size_t lds = (size_t)block.x * MT * 16;
+    if (q.per_block == 1) hipLaunchKernelGGL((wnv_q4_rows<E, MT, 1, GATES>), grid, block, lds, s, q, a, split);
+    else if (q.per_block == 2) hipLaunchKernelGGL((wnv_q4_rows<E, MT, 2, GATES>), grid, block, lds, s, q, a, split);
+    else hipLaunchKernelGGL((wnv_q4_rows<E, MT, 4, GATES>), grid, block, lds, s, q, a, split);
+}
+template <typename E, int GATES> void launch(const Q4Dev& q, const Q4Call& a, hipStream_t s) {
+    const int most = GATES == 0 ? 16 : GATES == 2 ? 8 : 4;      // a workgroup is 16 waves at most, 12 with three gates
+    const int split = std::min(most, q.kb);
+    if (a.B <= 16) launch<E, 1, GATES>(q, a, split, s);
+    else if (a.B <= 32) launch<E, 2, GATES>(q, a, split, s);
+    else launch<E, 4, GATES>(q, a, split, s);
+}
+template <typename E> void launch(const Q4Dev& q, const Q4Call& a, hipStream_t s) {
+    if (!a.state) launch<E, 0>(q, a, s);
+    else if (q.gates == 2) launch<E, 2>(q, a, s);
+    else launch<E, 3>(q, a, s);
+}
 
 struct Alloc {                      // a device buffer that goes with its scope
     void* p = nullptr;
@@ -194,7 +354,7 @@ extern "C" wnv_status wnv_q4_create(int32_t cin, int32_t cout, int32_t gates, in
     h->device = device;
     Q4Dev& q = h->q;
     q.cin = cin; q.rows = cout / gates; q.gates = gates; q.group = group;
-    q.tiles = (q.rows + 15) / 16; q.kb = (cin + 127) / 128; q.groups = q.kb * (128 / group);
+    q.tiles = (q.rows + 15) / 16; q.kb = (cin + 127) / 128; q.per_block = 128 / group;
     *out = h;
     return WNV_OK;
 }
@@ -202,7 +362,7 @@ extern "C" wnv_status wnv_q4_create(int32_t cin, int32_t cout, int32_t gates, in
 static wnv_status q4_pack(wnv_q4* h, const uint8_t* codes, const wnv_bf16* scales, const uint8_t* zeros, const float* bias, int* bad,
                           hipStream_t s) {
     Q4Dev& q = h->q;
-    const size_t tiles = (size_t)q.gates * q.tiles, words = tiles * q.kb * 256, gs = tiles * q.groups * 16;
+    const size_t tiles = (size_t)q.gates * q.tiles, words = tiles * q.kb * 256, gs = tiles * q.kb * q.per_block * 16;
     h->loaded = false;
     HIP_TRY(h->codes.ensure(words * 4));
     HIP_TRY(h->scales.ensure(gs * 2));
@@ -281,8 +441,7 @@ extern "C" wnv_status wnv_q4_step(wnv_q4_handle h, const void* x, int64_t x_row_
     DeviceGuard guard(h->device);
     if (!guard.ok) return fail(WNV_ERR_HIP, "wnv_q4_step: cannot select device %d", h->device);
     const Q4Call a{x, x_row_stride, y, nullptr, B};
-    const dim3 grid(h->q.gates * h->q.tiles, B);
-    WNV_BY_TYPE(dtype, hipLaunchKernelGGL((wnv_q4_rows<E, 1, false>), grid, dim3(64), 0, (hipStream_t)stream, h->q, a));
+    WNV_BY_TYPE(dtype, launch<E>(h->q, a, (hipStream_t)stream));
     HIP_TRY(hipGetLastError());
     return WNV_OK;
 }
@@ -295,12 +454,7 @@ extern "C" wnv_status wnv_q4_recurrence_step(wnv_q4_handle h, const void* x, int
     DeviceGuard guard(h->device);
     if (!guard.ok) return fail(WNV_ERR_HIP, "wnv_q4_recurrence_step: cannot select device %d", h->device);
     const Q4Call a{x, x_row_stride, y, state, B};
-    const dim3 grid(h->q.tiles, B);
-    if (h->q.gates == 3) {
-        WNV_BY_TYPE(dtype, hipLaunchKernelGGL((wnv_q4_rows<E, 3, true>), grid, dim3(64), 0, (hipStream_t)stream, h->q, a));
-    } else {
-        WNV_BY_TYPE(dtype, hipLaunchKernelGGL((wnv_q4_rows<E, 2, true>), grid, dim3(64), 0, (hipStream_t)stream, h->q, a));
-    }
+    WNV_BY_TYPE(dtype, launch<E>(h->q, a, (hipStream_t)stream));
     HIP_TRY(hipGetLastError());
     return WNV_OK;
 }
