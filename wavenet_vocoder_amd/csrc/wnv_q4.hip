@@ -163,20 +163,22 @@ template <typename E> __device__ __forceinline__ u32x4 offset_of(uint32_t zero) 
     return u32x4{w, w, w, w};
 }
 
-// Inputs k0 ... k0 + 7 of a row, zeros behind its end; as they stand in memory, cut into parts at their use.
+// Eight inputs as they stand in memory, and cut into parts.
 template <typename E> struct Inputs { u32x4 w[sizeof(E) / 2]; };
-template <typename E> __device__ __forceinline__ Inputs<E> load_inputs(const E* row, int k0, int cin) {
-    Inputs<E> r{};
-    if (k0 + 8 <= cin) {
+template <typename E> __device__ __forceinline__ Inputs<E> load_inputs(const E* p) {             // at any alignment
+    Inputs<E> r;
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(E) / 2; ++i) r.w[i] = *(const u32x4_any*)((const char*)(row + k0) + 16 * i);
-    } else {
-        E e[8] = {};
+    for (int i = 0; i < (int)sizeof(E) / 2; ++i) r.w[i] = *(const u32x4_any*)((const char*)p + 16 * i);
+    return r;
+}
+template <typename E> __device__ __forceinline__ Inputs<E> load_inputs(const E* p, int left) {   // zeros behind the row's end
+    if (left >= 8) return load_inputs(p);
+    E e[8] = {};
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (k0 + i < cin) e[i] = row[k0 + i];
-        __builtin_memcpy(&r, e, sizeof r);
-    }
+    for (int i = 0; i < 7; ++i)
+        if (i < left) e[i] = p[i];
+    Inputs<E> r;
+    __builtin_memcpy(&r, e, sizeof r);
     return r;
 }
 template <typename E> __device__ __forceinline__ void parts_of(const Inputs<E>& x, u32x4 (&part)[Q4Type<E>::PARTS]) {
@@ -213,83 +215,127 @@ template <int GROUPS> __device__ __forceinline__ Q4Block<GROUPS> load_block(cons
     return f;
 }
 
-// One tile (GATES > 0: one of each gate, of the same 16 channels, and the sums go straight into the recurrence's step) x 16 MT rows
-// of x.  A wave takes a gate and shares out the blocks of 128 inputs with the `split` waves of the same gate; their sums are joined
-// in LDS in the waves' order: no atomics, and a row's result does not depend on the rows beside it (the split goes by the weights'
-// shape alone).  The weights of a wave's next block are asked for before this one's products; x, which every workgroup reads, comes
-// out of L2 at its use.
-template <typename E, int MT, int GROUPS, int GATES>
-__global__ void __launch_bounds__(1024) wnv_q4_rows(Q4Dev q, Q4Call a, int split) {
-    extern __shared__ f32x4 sums[];     // [wave][MT][64]
-    constexpr int PARTS = Q4Type<E>::PARTS, JG = 4 / GROUPS;
+// NT tiles side by side (GATES > 0: one tile of each gate, of the same 16 channels, and the sums go straight into the recurrence's
+// step) x 16 rows of x.  A wave takes NT tiles (a gate's) and shares out the blocks of 128 inputs with the `split` waves of the same
+// tiles; their sums are joined in LDS in the waves' order: no atomics, and a row's result does not depend on the rows beside it (the
+// split goes by the weights' shape alone).
+// STAGED: the rows of x go through LDS behind the first weights' request, and the parts of float32 rows are columns of their own there
+// (up to 5 rows); else each wave takes its own of x from L2, and the parts follow each other into sums of their own.  Both add the
+// parts' sums in the same order at the end: which of the two runs does not show in the result.  The weights of a wave's next block are
+// asked for before this one's products where registers allow it (STAGED).
+template <typename E, int NT, int GROUPS, int GATES, bool STAGED>
+__global__ void __launch_bounds__(1024) wnv_q4_rows(Q4Dev q, Q4Call a, int split, int most) {
+    static_assert(!GATES || NT == 1, "a wave holds one gate");
+    extern __shared__ u32x4 shared[];   // STAGED: [part][row][16 kb + 1], 8 inputs each; then sums [wave][NT][SUMS][64]
+    constexpr int PARTS = Q4Type<E>::PARTS, SUMS = STAGED ? 1 : PARTS, JG = 4 / GROUPS;
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, r = lane % 16, quarter = lane / 16, slice = wave % split;
-    const long long tile = blockIdx.x + (GATES ? wave / split * q.tiles : 0);
-    const int b0 = blockIdx.y * (16 * MT);
+    const int all = q.gates * q.tiles, tile0 = blockIdx.x * NT + (GATES ? wave / split * q.tiles : 0), b0 = blockIdx.y * most;
+    const int rows = min(most, a.B - b0), pitch = 16 * q.kb + 1;          // a pitch of 16 bytes more spreads the rows over the banks
+    const E* x = (const E*)a.x + (long long)(b0 + min(r, rows - 1)) * a.xs;
 
-    f32x4 acc[MT] = {};
-    Q4Block<GROUPS> f{};
-    if (slice < q.kb) f = load_block<GROUPS>(q, tile * q.kb + slice, lane);
+    f32x4 acc[NT][SUMS] = {};
+    Q4Block<GROUPS> f[NT] = {};
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+        if (slice < q.kb) f[t] = load_block<GROUPS>(q, (long long)min(tile0 + t, all - 1) * q.kb + slice, lane);
+    if (STAGED) {
+        for (int i = threadIdx.x; i < rows * 16 * q.kb; i += blockDim.x) {
+            const int row = i / (16 * q.kb), k = i - row * (16 * q.kb);
+            u32x4 part[PARTS];
+            parts_of<E>(load_inputs<E>((const E*)a.x + (long long)(b0 + row) * a.xs + k * 8, q.cin - k * 8), part);
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p) shared[(p * rows + row) * pitch + k] = part[p];
+        }
+        __syncthreads();
+    }
     for (int kb = slice; kb < q.kb; kb += split) {
-        Q4Block<GROUPS> next{};
-        if (kb + split < q.kb) next = load_block<GROUPS>(q, tile * q.kb + kb + split, lane);
+        if (!STAGED && kb != slice) {
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            const int b = b0 + 16 * m + r;
-            const E* x = (const E*)a.x + (long long)min(b, a.B - 1) * a.xs;
-            Inputs<E> in[4];
+            for (int t = 0; t < NT; ++t) f[t] = load_block<GROUPS>(q, (long long)min(tile0 + t, all - 1) * q.kb + kb, lane);
+        }
+        Q4Block<GROUPS> next[NT] = {};
 #pragma unroll
-            for (int j = 0; j < 4; ++j) in[j] = b < a.B ? load_inputs<E>(x, kb * 128 + j * 32 + quarter * 8, q.cin) : Inputs<E>{};
+        for (int t = 0; t < NT; ++t)
+            if (STAGED && kb + split < q.kb) next[t] = load_block<GROUPS>(q, (long long)min(tile0 + t, all - 1) * q.kb + kb + split, lane);
+        Inputs<E> in[4] = {};
+        if (!STAGED) {
+            if ((kb + 1) * 128 <= q.cin) {
+                if (r < rows) {
 #pragma unroll
-            for (int g = 0; g < GROUPS; ++g) {
-                f32x4 sum = {};
-                const u32x4 o = offset_of<E>(f.zero >> (8 * g) & 255);
+                    for (int j = 0; j < 4; ++j) in[j] = load_inputs<E>(x + kb * 128 + j * 32 + quarter * 8);
+                }
+            } else if (r < rows) {
 #pragma unroll
-                for (int j = g * JG; j < (g + 1) * JG; ++j) {
-                    const u32x4 w = codes_up<E>(j == 0 ? f.code.x : j == 1 ? f.code.y : j == 2 ? f.code.z : f.code.w);
-                    u32x4 part[PARTS];
-                    parts_of<E>(in[j], part);
+                for (int j = 0; j < 4; ++j) in[j] = load_inputs<E>(x + kb * 128 + j * 32 + quarter * 8, q.cin - (kb * 128 + j * 32 + quarter * 8));
+            }
+        }
 #pragma unroll
-                    for (int i = 0; i < PARTS; ++i) {
-                        sum = mfma<E>(w, part[i], sum);
-                        sum = mfma<E>(o, part[i], sum);
+        for (int g = 0; g < GROUPS; ++g) {
+            f32x4 sum[NT][SUMS] = {};
+#pragma unroll
+            for (int j = g * JG; j < (g + 1) * JG; ++j) {
+                u32x4 part[SUMS] = {};
+                if constexpr (!STAGED) parts_of<E>(in[j], part);
+                else if (r < PARTS * rows) part[0] = shared[r * pitch + kb * 16 + j * 4 + quarter];
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const u32x4 w = codes_up<E>(j == 0 ? f[t].code.x : j == 1 ? f[t].code.y : j == 2 ? f[t].code.z : f[t].code.w);
+                    const u32x4 o = offset_of<E>(f[t].zero >> (8 * g) & 255);
+#pragma unroll
+                    for (int p = 0; p < SUMS; ++p) {
+                        sum[t][p] = mfma<E>(w, part[p], sum[t][p]);
+                        sum[t][p] = mfma<E>(o, part[p], sum[t][p]);
                     }
                 }
-                const uint2 s = f.scale[g];
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const uint2 s = f[t].scale[g];
                 const f32x4 scale{__uint_as_float(s.x << 16), __uint_as_float(s.x & 0xffff0000u), __uint_as_float(s.y << 16),
                                   __uint_as_float(s.y & 0xffff0000u)};
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[m][i] = fmaf(scale[i], sum[i], acc[m][i]);
-            }
-            if (MT > 1) __builtin_amdgcn_sched_barrier(0);      // the rows' loads one tile at a time: all at once do not fit the registers
-        }
-        f = next;
-    }
+                for (int p = 0; p < SUMS; ++p)
 #pragma unroll
-    for (int m = 0; m < MT; ++m) sums[(wave * MT + m) * 64 + lane] = acc[m];
+                    for (int i = 0; i < 4; ++i) acc[t][p][i] = fmaf(scale[i], sum[t][p][i], acc[t][p][i]);
+            }
+        }
+        if (STAGED) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t) f[t] = next[t];
+        }
+    }
+    f32x4* sums = (f32x4*)shared + (STAGED ? PARTS * rows * pitch : 0);
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int p = 0; p < SUMS; ++p) sums[((wave * NT + t) * SUMS + p) * 64 + lane] = acc[t][p];
     __syncthreads();
 
     // 16 neighbouring threads write 16 neighbouring outputs of a row; lane l of a result holds its column l % 16, rows 4 (l / 16) ...
     const float* part = (const float*)sums;
-    for (int e = threadIdx.x; e < MT * 256; e += blockDim.x) {
-        const int n = e % 16, col = e / 16 % 16, m = e / 256, b = b0 + 16 * m + col;
-        const int gate = GATES ? 0 : blockIdx.x / q.tiles, channel = (blockIdx.x - gate * q.tiles) * 16 + n;
-        if (b >= a.B || channel >= q.rows) continue;
+    for (int e = threadIdx.x; e < NT * 256; e += blockDim.x) {
+        const int n = e % 16, col = e / 16 % 16, row = b0 + col, t = e / 256, tile = blockIdx.x * NT + t, gate = GATES ? 0 : tile / q.tiles;
+        const int channel = (tile - gate * q.tiles) * 16 + n, at = (t * SUMS * 64 + n / 4 * 16 + col) * 4 + n % 4;
+        const int apart = STAGED ? rows * 4 : 256;      // from a part's sum to the next one's
+        if (col >= rows || tile >= all || channel >= q.rows) continue;
         float z[GATES ? GATES : 1];
 #pragma unroll
         for (int g = 0; g < (GATES ? GATES : 1); ++g) {
-            const int at = (m * 64 + n / 4 * 16 + col) * 4 + n % 4;
             float sum = 0.f;
-            for (int w = 0; w < split; ++w) sum += part[at + (g * split + w) * (MT * 256)];
-            z[g] = sum + q.bias[(blockIdx.x + g * q.tiles) * 16 + n];
+            for (int w = 0; w < split; ++w) {
+                const float* one = part + at + (g * split + w) * (NT * SUMS * 256);
+                sum += PARTS == 3 ? one[0] + one[apart] + one[2 * apart] : one[0];
+            }
+            z[g] = sum + q.bias[(tile + g * q.tiles) * 16 + n];
         }
         if (!GATES) {
-            ((E*)a.y)[((long long)b * q.gates + gate) * q.rows + channel] = wnv_down<E>(z[0]);
+            ((E*)a.y)[((long long)row * q.gates + gate) * q.rows + channel] = wnv_down<E>(z[0]);
         } else {
-            float h = a.state[(long long)b * q.rows + channel];
+            float h = a.state[(long long)row * q.rows + channel];
             h = fmaf(wnv_gate(-z[0]), z[GATES > 1 ? 1 : 0] - h, h);
-            a.state[(long long)b * q.rows + channel] = h;
+            a.state[(long long)row * q.rows + channel] = h;
             if (GATES == 3) h *= wnv_gate(z[GATES - 1]);
-            ((E*)a.y)[(long long)b * q.rows + channel] = wnv_down<E>(h);
+            ((E*)a.y)[(long long)row * q.rows + channel] = wnv_down<E>(h);
         }
     }
 }
@@ -301,19 +347,34 @@ __global__ void __launch_bounds__(1024) wnv_q4_rows(Q4Dev q, Q4Call a, int split
         default: { using E = wnv_f16; __VA_ARGS__; break; }                           \
     }
 
-template <typename E, int MT, int GATES> void launch(const Q4Dev& q, const Q4Call& a, int split, hipStream_t s) {
-    const dim3 grid(GATES ? q.tiles : q.gates * q.tiles, (a.B + 16 * MT - 1) / (16 * MT)), block(64 * split * (GATES ? GATES : 1));
-    const size_t lds = (size_t)block.x * MT * 16;
-    if (q.per_block == 1) hipLaunchKernelGGL((wnv_q4_rows<E, MT, 1, GATES>), grid, block, lds, s, q, a, split);
-    else if (q.per_block == 2) hipLaunchKernelGGL((wnv_q4_rows<E, MT, 2, GATES>), grid, block, lds, s, q, a, split);
-    else hipLaunchKernelGGL((wnv_q4_rows<E, MT, 4, GATES>), grid, block, lds, s, q, a, split);
+// Which form runs (us a launch in a graph, both sides measured):
+//  * x through LDS if its rows fit (two workgroups a CU then) and it pays: float32, whose three parts become columns of one product
+//    (1 x 8192 x 8192: 11.6, from L2 23.4; 8 x 512 x 3 512 with the step: 4.4 and 5.4) -- at most 5 rows a workgroup --, and 16-bit
+//    types if a wave has several blocks of inputs to wait for (1 x 8192 x 8192 bf16: 11.1 and 13.2; 8 x 1616 x 512, one block a wave:
+//    4.6 and 3.9).
+//  * else two tiles a wave, which halves what is read of x, as soon as single tiles would be more workgroups than CUs (bf16
+//    64 x 4096 x 4096: 15.5 and 19.6, 48 x 2048 x 2048: 5.3 and 6.6; with fewer, 16 x 2048 x 2048: 5.0 and 4.4).
+constexpr size_t STAGE_MOST = 64 << 10;
+constexpr int CUS = 256;
+
+template <typename E, int NT, int GATES, bool STAGED>
+void launch(const Q4Dev& q, const Q4Call& a, int split, int most, size_t staged, hipStream_t s) {
+    const dim3 grid(GATES ? q.tiles : (q.gates * q.tiles + NT - 1) / NT, (a.B + most - 1) / most), block(64 * split * (GATES ? GATES : 1));
+    const size_t lds = (size_t)block.x * NT * 16 * (STAGED ? 1 : Q4Type<E>::PARTS) + staged;
+    if (q.per_block == 1) hipLaunchKernelGGL((wnv_q4_rows<E, NT, 1, GATES, STAGED>), grid, block, lds, s, q, a, split, most);
+    else if (q.per_block == 2) hipLaunchKernelGGL((wnv_q4_rows<E, NT, 2, GATES, STAGED>), grid, block, lds, s, q, a, split, most);
+    else hipLaunchKernelGGL((wnv_q4_rows<E, NT, 4, GATES, STAGED>), grid, block, lds, s, q, a, split, most);
 }
 template <typename E, int GATES> void launch(const Q4Dev& q, const Q4Call& a, hipStream_t s) {
-    const int most = GATES == 0 ? 16 : GATES == 2 ? 8 : 4;      // a workgroup is 16 waves at most, 12 with three gates
-    const int split = std::min(most, q.kb);
-    if (a.B <= 16) launch<E, 1, GATES>(q, a, split, s);
-    else if (a.B <= 32) launch<E, 2, GATES>(q, a, split, s);
-    else launch<E, 4, GATES>(q, a, split, s);
+    constexpr int PARTS = Q4Type<E>::PARTS;
+    const int waves = GATES == 0 ? 16 : GATES == 2 ? 8 : 4;     // of one tile: a workgroup is 16 waves at most, 12 with three gates
+    const int split = std::min(waves, q.kb), most = 16 / PARTS;
+    const size_t staged = (size_t)PARTS * std::min(a.B, most) * (16 * q.kb + 1) * 16;
+    if (staged <= STAGE_MOST && (PARTS == 3 || (a.B <= 16 && q.kb > split))) return launch<E, 1, GATES, true>(q, a, split, most, staged, s);
+    if constexpr (!GATES) {
+        if ((int64_t)q.gates * q.tiles * ((a.B + 15) / 16) > CUS) return launch<E, 2, GATES, false>(q, a, split, 16, 0, s);
+    }
+    launch<E, 1, GATES, false>(q, a, split, 16, 0, s);
 }
 template <typename E> void launch(const Q4Dev& q, const Q4Call& a, hipStream_t s) {
     if (!a.state) launch<E, 0>(q, a, s);

@@ -477,17 +477,17 @@ class Q4Linear:
         return w
 
     def _x(self, x: torch.Tensor) -> int:
-        if not x.is_cuda:
-            require_gpu_tensor(x, "x")
-        if x.device != self.device:
-            raise ValueError(f"x lives on {x.device}, the weights on {self.device}")
-        if x.dim() != 2 or x.shape[1] != self.cin or x.shape[0] == 0:
-            raise ValueError(f"x is {tuple(x.shape)}, expected (B, {self.cin})")
-        if torch.is_grad_enabled() and x.requires_grad:
-            raise RuntimeError("4-bit products are not differentiable: use torch.no_grad()")
         code = self._DTYPES.get(x.dtype)
+        if x.get_device() != self.device.index:
+            require_gpu_tensor(x, "x")
+            raise ValueError(f"x lives on {x.device}, the weights on {self.device}")
+        shape = x.shape
+        if len(shape) != 2 or shape[1] != self.cin or shape[0] == 0:
+            raise ValueError(f"x is {tuple(shape)}, expected (B, {self.cin})")
         if code is None:
             raise TypeError(f"x is {x.dtype}: float32, bfloat16 and float16 are implemented")
+        if x.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("4-bit products are not differentiable: use torch.no_grad()")
         return code
 
     def step(self, x: torch.Tensor) -> torch.Tensor:
@@ -495,22 +495,26 @@ class Q4Linear:
         code = self._x(x)
         if x.stride(1) != 1:
             x = x.contiguous()
-        y = torch.empty(x.shape[0], self.cout, device=x.device, dtype=x.dtype)
-        check(_lib.lib().wnv_q4_step(self._h, x.data_ptr(), x.stride(0), y.data_ptr(), x.shape[0], code,
+        B = x.shape[0]
+        y = torch.empty(B, self.cout, device=self.device, dtype=x.dtype)
+        check(_lib.lib().wnv_q4_step(self._h, x.data_ptr(), x.stride(0), y.data_ptr(), B, code,
                                      torch._C._cuda_getCurrentRawStream(self.device.index)))
         return y
 
     def recurrence_step(self, x: torch.Tensor, state: torch.Tensor) -> torch.Tensor:
         """x (B, cin), ``state`` (B, channels) float32 contiguous, updated in place -> y (B, channels) of x's type."""
         code = self._x(x)
-        if tuple(state.shape) != (x.shape[0], self.channels):
-            raise ValueError(f"state is {tuple(state.shape)}, expected {(x.shape[0], self.channels)}")
-        if state.dtype != torch.float32 or state.device != x.device or not state.is_contiguous():
+        B = x.shape[0]
+        if state.shape != (B, self.channels):
+            raise ValueError(f"state is {tuple(state.shape)}, expected {(B, self.channels)}")
+        if state.dtype != torch.float32 or state.get_device() != self.device.index or not state.is_contiguous():
             raise ValueError("state is updated in place: it has to be float32, contiguous and on x's device")
+        if state.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("4-bit products are not differentiable: use torch.no_grad()")
         if x.stride(1) != 1:
             x = x.contiguous()
-        y = torch.empty(x.shape[0], self.channels, device=x.device, dtype=x.dtype)
-        check(_lib.lib().wnv_q4_recurrence_step(self._h, x.data_ptr(), x.stride(0), state.data_ptr(), y.data_ptr(), x.shape[0], code,
+        y = torch.empty(B, self.channels, device=self.device, dtype=x.dtype)
+        check(_lib.lib().wnv_q4_recurrence_step(self._h, x.data_ptr(), x.stride(0), state.data_ptr(), y.data_ptr(), B, code,
                                                 torch._C._cuda_getCurrentRawStream(self.device.index)))
         return y
 

@@ -10,6 +10,7 @@ include/wnv.h); there is no CPU path.
 from __future__ import annotations
 
 import ctypes as C
+from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
@@ -32,33 +33,25 @@ def _dtype(z: torch.Tensor) -> int:
     return code
 
 
-def _channels(z: torch.Tensor, gates: int) -> int:
-    if z.shape[-1] == 0 or z.shape[-1] % gates:
-        raise ValueError(f"z has {z.shape[-1]} channels, which are not {gates} gates of the same size")
-    return z.shape[-1] // gates
-
-
 def _state(h: torch.Tensor, name: str, B: int, n: int, z: torch.Tensor) -> torch.Tensor:
-    if tuple(h.shape) != (B, n):
+    if h.shape != (B, n):
         raise ValueError(f"{name} is {tuple(h.shape)}, expected {(B, n)}")
     if h.dtype != torch.float32:
         raise TypeError(f"{name} is {h.dtype}: the state is float32")
-    if h.device != z.device:
+    if h.get_device() != z.get_device():
         raise ValueError(f"{name} lives on {h.device}, z on {z.device}")
     return h
 
 
-def _map(m: Optional[torch.Tensor], name: str, shape: Tuple[int, ...], z: torch.Tensor) -> Optional[torch.Tensor]:
-    if m is None:
-        return None
-    if tuple(m.shape) != shape:
+def _map(m: torch.Tensor, name: str, shape: Tuple[int, ...], z: torch.Tensor) -> torch.Tensor:
+    if m.shape != shape:
         raise ValueError(f"{name} is {tuple(m.shape)}, expected {shape}")
-    if m.dtype not in (torch.int32, torch.int64):
-        raise TypeError(f"{name} is {m.dtype}: int32 or int64")
-    if m.device != z.device:
+    if m.get_device() != z.get_device():
         raise ValueError(f"{name} lives on {m.device}, z on {z.device}")
     if m.dtype == torch.int64:
         m = m.clamp(-1, 2 ** 31 - 1).to(torch.int32)
+    elif m.dtype != torch.int32:
+        raise TypeError(f"{name} is {m.dtype}: int32 or int64")
     return m.contiguous()
 
 
@@ -67,32 +60,57 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if (t.stride(-1) == 1 or t.shape[-1] == 1) and (t.dim() < 3 or t.stride(1) < 1 << 22) else t.contiguous()
 
 
-def _call(fn, z, gates, h0, lengths, seg_start, *, y=None, h_last=None, saved=None, dy=None, dh_last=None, dz=None, dh0=None):
-    B, T, n = z.shape[0], z.shape[1], z.shape[2] // gates
-    code = _DTYPES[z.dtype]
-    dev = z.device.index
-    ws = None
-    nbytes = _lib.lib().wnv_recurrence_workspace_bytes(B, T, n, gates, code)
-    if nbytes > 0:          # of the stream that runs the call: torch's allocator hands it out again behind the call's own work only
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=z.device)
-    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    a = RecurrenceArgs(B, n, T, gates, code, z.data_ptr(), z.stride(0), z.stride(1), ptr(h0), 0 if h0 is None else h0.stride(0),
-                       ptr(lengths), ptr(seg_start), ptr(y), ptr(h_last), ptr(saved), ptr(ws), ptr(dy),
-                       0 if dy is None else dy.stride(0), 0 if dy is None else dy.stride(1), ptr(dh_last), ptr(dz), ptr(dh0),
+@lru_cache(maxsize=256)
+def _sizes(B: int, T: int, n: int, gates: int, code: int) -> Tuple[int, int]:
+    """Bytes of (saved, workspace), which go by the shape alone."""
+    lib = _lib.lib()
+    return (lib.wnv_recurrence_saved_bytes(B, T, n, gates, code), lib.wnv_recurrence_workspace_bytes(B, T, n, gates, code))
+
+
+def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
+def _call(fn, z, B, T, n, gates, code, ws_bytes, h0, lengths, seg_start, y, h_last, saved, dy, dh_last, dz, dh0):
+    # the workspace is of the stream that runs the call: torch's allocator hands it out again behind the call's own work only
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=z.device) if ws_bytes else None
+    dev = z.get_device()
+    zb, zt, _ = z.stride()
+    db, dt, _ = (0, 0, 0) if dy is None else dy.stride()
+    a = RecurrenceArgs(B, n, T, gates, code, z.data_ptr(), zb, zt, _ptr(h0), 0 if h0 is None else h0.stride(0), _ptr(lengths),
+                       _ptr(seg_start), _ptr(y), _ptr(h_last), _ptr(saved), _ptr(ws), _ptr(dy), db, dt, _ptr(dh_last), _ptr(dz), _ptr(dh0),
                        _raw_stream(dev))
     check(fn(dev, C.byref(a)))
 
 
 def _forward(z, h0, gates, lengths, seg_start, keep: bool):
-    B, T, n = z.shape[0], z.shape[1], z.shape[2] // gates
-    y = torch.empty(B, T, n, dtype=z.dtype, device=z.device)
-    h_last = torch.empty(B, n, dtype=torch.float32, device=z.device)
-    saved = None
-    if keep:
-        nbytes = _lib.lib().wnv_recurrence_saved_bytes(B, T, n, gates, _DTYPES[z.dtype])
-        saved = torch.empty(nbytes, dtype=torch.uint8, device=z.device)
-    _call(_lib.lib().wnv_recurrence_forward, z, gates, h0, lengths, seg_start, y=y, h_last=h_last, saved=saved)
+    B, T, n = z.shape
+    n //= gates
+    code, dev = _DTYPES[z.dtype], z.device
+    saved_bytes, ws_bytes = _sizes(B, T, n, gates, code)
+    y = torch.empty(B, T, n, dtype=z.dtype, device=dev)
+    h_last = torch.empty(B, n, dtype=torch.float32, device=dev)
+    saved = torch.empty(saved_bytes, dtype=torch.uint8, device=dev) if keep else None
+    _call(_lib.lib().wnv_recurrence_forward, z, B, T, n, gates, code, ws_bytes, h0, lengths, seg_start, y, h_last, saved, None, None, None,
+          None)
     return y, h_last, saved
+
+
+def _backward(ctx, dy, dh_last):
+    z, saved, h0, lengths, seg_start = ctx.saved_tensors
+    gates = ctx.gates
+    B, T, n = z.shape
+    n //= gates
+    code, dev = _DTYPES[z.dtype], z.device
+    needs_z, needs_h0 = ctx.needs_input_grad[:2]
+    dz = torch.empty(B, T, gates * n, dtype=z.dtype, device=dev)
+    dh0 = torch.empty(B, n, dtype=torch.float32, device=dev) if needs_h0 else None
+    _call(_lib.lib().wnv_recurrence_backward, z, B, T, n, gates, code, _sizes(B, T, n, gates, code)[1], h0, lengths, seg_start, None, None,
+          saved, None if dy is None else _rows(dy), None if dh_last is None else dh_last.contiguous(), dz, dh0)
+    return (dz if needs_z else None), dh0, None, None, None
+
+
+_backward_once = once_differentiable(_backward)
 
 
 class _GatedRecurrence(torch.autograd.Function):
@@ -100,21 +118,13 @@ class _GatedRecurrence(torch.autograd.Function):
     def forward(ctx, z, h0, gates, lengths, seg_start):
         ctx.set_materialize_grads(False)
         y, h_last, saved = _forward(z, h0, gates, lengths, seg_start, True)
-        ctx.gates, ctx.optional = gates, (h0 is not None, lengths is not None, seg_start is not None)
-        ctx.save_for_backward(z, saved, *(t for t in (h0, lengths, seg_start) if t is not None))
+        ctx.gates = gates
+        ctx.save_for_backward(z, saved, h0, lengths, seg_start)
         return y, h_last
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, dh_last):
-        z, saved, *rest = ctx.saved_tensors
-        h0, lengths, seg_start = ((rest.pop(0) if there else None) for there in ctx.optional)
-        dz = torch.empty(z.shape, dtype=z.dtype, device=z.device)
-        dh0 = torch.empty(h0.shape, dtype=torch.float32, device=z.device) if h0 is not None and ctx.needs_input_grad[1] else None
-        dy = None if dy is None else _rows(dy)
-        dh_last = None if dh_last is None else dh_last.contiguous()
-        _call(_lib.lib().wnv_recurrence_backward, z, ctx.gates, h0, lengths, seg_start, saved=saved, dy=dy, dh_last=dh_last, dz=dz, dh0=dh0)
-        return (dz if ctx.needs_input_grad[0] else None), dh0, None, None, None
+        return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, dy, dh_last)
 
 
 def gated_recurrence(z: torch.Tensor, h0: Optional[torch.Tensor] = None, *, output_gate: bool = True,
@@ -128,19 +138,21 @@ def gated_recurrence(z: torch.Tensor, h0: Optional[torch.Tensor] = None, *, outp
     entry is an utterance begun before this call, which goes on from ``h0``.  Differentiable (once) in z and h0.  Runs on the current
     stream of z's device and is capturable; the same call gives the same bits."""
     require_gpu_tensor(z, "z")
+    _dtype(z)
     if z.dim() != 3:
         raise ValueError(f"z is {tuple(z.shape)}, expected (B, T, channels)")
-    _dtype(z)
     gates = 3 if output_gate else 2
-    B, T = z.shape[0], z.shape[1]
-    n = _channels(z, gates)
-    if B == 0 or T == 0:
-        raise ValueError(f"z is {tuple(z.shape)}: an empty batch or sequence")
+    B, T, n = z.shape
+    if B == 0 or T == 0 or n == 0 or n % gates:
+        raise ValueError(f"z is {tuple(z.shape)}, expected (B, T, {gates} gates of the same size), none of them empty")
+    n //= gates
+    z = _rows(z)
     if h0 is not None:
         h0 = _rows(_state(h0, "h0", B, n, z))
-    lengths = _map(lengths, "lengths", (B,), z)
-    seg_start = _map(seg_start, "seg_start", (B, T), z)
-    z = _rows(z)
+    if lengths is not None:
+        lengths = _map(lengths, "lengths", (B,), z)
+    if seg_start is not None:
+        seg_start = _map(seg_start, "seg_start", (B, T), z)
     if torch.is_grad_enabled() and (z.requires_grad or (h0 is not None and h0.requires_grad)):
         return _GatedRecurrence.apply(z, h0, gates, lengths, seg_start)
     y, h_last, _ = _forward(z, h0, gates, lengths, seg_start, False)
@@ -151,20 +163,21 @@ def gated_recurrence_step(z: torch.Tensor, state: torch.Tensor, *, output_gate: 
     """One step: z (B, 3 C) (``output_gate=False``: (B, 2 C)), ``state`` (B, C) float32 contiguous, updated in place -> y (B, C) of z's
     type.  Not differentiable: the training form is ``gated_recurrence``."""
     require_gpu_tensor(z, "z")
+    code = _dtype(z)
     if z.dim() != 2:
         raise ValueError(f"z is {tuple(z.shape)}, expected (B, channels)")
-    code = _dtype(z)
     gates = 3 if output_gate else 2
-    B, n = z.shape[0], _channels(z, gates)
-    if B == 0:
-        raise ValueError("z is an empty batch")
+    B, n = z.shape
+    if B == 0 or n == 0 or n % gates:
+        raise ValueError(f"z is {tuple(z.shape)}, expected (B, {gates} gates of the same size), neither of them empty")
+    n //= gates
     if not _state(state, "state", B, n, z).is_contiguous():
         raise ValueError("state is updated in place: it has to be contiguous")
-    if torch.is_grad_enabled() and (z.requires_grad or state.requires_grad):
+    if (z.requires_grad or state.requires_grad) and torch.is_grad_enabled():
         raise RuntimeError("gated_recurrence_step is not differentiable: use gated_recurrence, or torch.no_grad()")
     z = _rows(z)
     y = torch.empty(B, n, dtype=z.dtype, device=z.device)
-    dev = z.device.index
+    dev = z.get_device()
     check(_lib.lib().wnv_recurrence_step(dev, z.data_ptr(), z.stride(0), state.data_ptr(), y.data_ptr(), B, n, gates, code,
                                          _raw_stream(dev)))
     return y
