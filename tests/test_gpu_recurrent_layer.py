@@ -1,0 +1,175 @@
+"""ResidualRecurrentGLU: the recurrence, its gradients, its step and the 4-bit products together, as a layer uses them."""
+import copy
+import math
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+from tests._ops import oracle_scan
+from wavenet_vocoder_amd.modules import ResidualConv1dGLU, ResidualRecurrentGLU
+
+pytestmark = pytest.mark.gpu
+
+GEOM = dict(residual_channels=48, gate_channels=64, skip_out_channels=40, cin_channels=20, gin_channels=8)
+
+
+def layer(seed=0, **kw):
+    torch.manual_seed(seed)
+    m = ResidualRecurrentGLU(**{**GEOM, **kw})
+    with torch.no_grad():
+        for p in m.parameters():
+            p.copy_(torch.randn_like(p) * 0.2)
+    return m
+
+
+def data(B, T, seed=1):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(B, 48, T, generator=g), torch.randn(B, 20, T, generator=g), torch.randn(B, 8, 1, generator=g).expand(B, 8, T).contiguous())
+
+
+def exact(m, x, c, g, seg_start=None, lengths=None):
+    """The layer in 64 bits, its projections through torch's float64 and the recurrence step by step."""
+    def proj(conv, t):
+        return F.conv1d(t, conv.weight.detach().double().cpu(), None if conv.bias is None else conv.bias.detach().double().cpu())
+    z = (proj(m.conv1x1_in, x.double()) + proj(m.conv1x1c, c.double()) + proj(m.conv1x1g, g.double())).transpose(1, 2)
+    y = oracle_scan(z, seg_start=seg_start, lengths=lengths)["y"].transpose(1, 2)
+    return (proj(m.conv1x1_out, y) + x.double()) * math.sqrt(0.5), proj(m.conv1x1_skip, y)
+
+
+# Random roundings: z sums 76 products to about 15 in magnitude, sqrt(76) EPS 15 = 8e-6; the state sums over 150 steps, sqrt(150) EPS 8 =
+# 6e-6; the projections behind it weigh 32 such errors with 0.2, times 1.2: 2e-5 in all.  The tolerance leaves a factor of 100 for
+# their largest among thousands; a wrong gate, step or row is off by tenths.
+TOL = 2e-3
+
+
+def test_forward_is_its_formula_and_the_steps_are_the_forward():
+    B, T = 3, 150
+    m = layer()
+    x, c, g = data(B, T)
+    want = exact(m, x, c, g)
+    m = m.cuda().eval()
+    with torch.no_grad():
+        out = m(x.cuda(), c.cuda(), g.cuda())
+    for a, b in zip(out, want):
+        assert float((a.double().cpu() - b).abs().max()) < TOL
+    for again in range(2):              # clear_buffer starts over
+        m.clear_buffer()
+        steps = [m.incremental_forward(x[:, :, t].cuda()[:, None], c[:, :, t].cuda()[:, None], g[:, :, t].cuda()[:, None]) for t in range(T)]
+        for k in range(2):
+            got = torch.cat([s[k] for s in steps], 1).transpose(1, 2)
+            assert float((got.double().cpu() - want[k]).abs().max()) < TOL
+    with pytest.raises(ValueError, match="without clear_buffer"):
+        m.incremental_forward(x[:1, :, 0].cuda()[:, None])
+
+
+def test_packed_slots_and_padded_batches_are_the_utterances_alone():
+    m = layer(3).cuda().eval()
+    x, c, g = (t.cuda() for t in data(1, 200))
+    start = torch.zeros(1, 200, dtype=torch.int32, device="cuda")
+    start[:, 70:] = 70
+    with torch.no_grad():
+        packed = m(x, c, g, seg_start=start)
+        alone = [m(x[..., a:b], c[..., a:b], g[..., a:b]) for a, b in ((0, 70), (70, 200))]
+        padded = m(x.expand(2, -1, -1), c.expand(2, -1, -1), g.expand(2, -1, -1), lengths=torch.tensor([70, 200], device="cuda"))
+        whole = m(x, c, g)
+    for k in range(2):
+        assert float((packed[k][..., :70] - alone[0][k]).abs().max()) < TOL and float((packed[k][..., 70:] - alone[1][k]).abs().max()) < TOL
+        assert float((padded[k][:1, :, :70] - alone[0][k]).abs().max()) < TOL and float((padded[k][1:] - whole[k]).abs().max()) < TOL
+
+
+def test_gradients_of_the_layer():
+    """Against torch's own, through the formula in 64 bits."""
+    B, T = 2, 90
+    m = layer(5, dropout=0.0)
+    x, c, g = data(B, T, 7)
+    ref = copy.deepcopy(m).double()
+    xr = x.double().requires_grad_()
+    conv = lambda k, t: F.conv1d(t, k.weight, k.bias)  # noqa: E731
+    z = conv(ref.conv1x1_in, xr) + conv(ref.conv1x1c, c.double()) + conv(ref.conv1x1g, g.double())
+    f, v, o = z.split(32, 1)
+    h, ys = torch.zeros(B, 32).double(), []
+    for t in range(T):
+        h = torch.sigmoid(f[..., t]) * h + torch.sigmoid(-f[..., t]) * v[..., t]
+        ys.append(h * torch.sigmoid(o[..., t]))
+    y = torch.stack(ys, -1)
+    out = (conv(ref.conv1x1_out, y) + xr) * math.sqrt(0.5), conv(ref.conv1x1_skip, y)
+    gen = torch.Generator().manual_seed(9)
+    heads = [torch.randn(t.shape, generator=gen) for t in out]
+    names = [n for n, _ in ref.named_parameters()]
+    want = torch.autograd.grad(out, [xr, *ref.parameters()], [h.double() for h in heads])
+    m = m.cuda().train()
+    xc = x.cuda().requires_grad_()
+    got = torch.autograd.grad(m(xc, c.cuda(), g.cuda()), [xc, *m.parameters()], [h.cuda() for h in heads])
+    for n, a, b in zip(["x", *names], got, want):
+        assert a.shape == b.shape
+        assert float((a.double().cpu() - b).norm()) <= 1e-4 * float(b.norm()), n
+
+
+def test_a_step_of_training_in_bfloat16_runs():
+    m = layer(11).cuda().to(torch.bfloat16).train()
+    x, c, g = (t.cuda().to(torch.bfloat16) for t in data(2, 130))
+    opt = torch.optim.SGD(m.parameters(), lr=1e-3)
+    before = [p.detach().clone() for p in m.parameters()]
+    o, s = m(x, c, g)
+    (o.float().square().mean() + s.float().square().mean()).backward()
+    assert all(p.grad is not None and torch.isfinite(p.grad).all() for p in m.parameters())
+    opt.step()
+    assert any(not torch.equal(a, b) for a, b in zip(before, m.parameters()))
+
+
+@pytest.mark.parametrize("group", [32, 64])
+def test_four_bit_steps_are_the_rounded_layer(group):
+    """The steps of a quantized layer are the steps of the same layer with the weights that the rounding gives."""
+    B, T = 4, 60
+    m = layer(13).cuda().eval().quantize_(group)
+    x, c, g = data(B, T, 15)
+    steps = [m.incremental_forward(x[:, :, t].cuda()[:, None], c[:, :, t].cuda()[:, None], g[:, :, t].cuda()[:, None]) for t in range(T)]
+    gates, heads = m._engine()
+    ref = copy.deepcopy(m).cpu()
+    w, h = gates.weight().cpu(), heads.weight().cpu()
+    with torch.no_grad():
+        for conv, part in zip((ref.conv1x1_in, ref.conv1x1c, ref.conv1x1g), w.split((48, 20, 8), 1)):
+            conv.weight.copy_(part[..., None])
+        for conv, part in zip((ref.conv1x1_out, ref.conv1x1_skip), h.split((48, 40), 0)):
+            conv.weight.copy_(part[..., None])
+    want = exact(ref, x, c, g)
+    for k in range(2):
+        got = torch.cat([s[k] for s in steps], 1).transpose(1, 2)
+        assert float((got.double().cpu() - want[k]).abs().max()) < TOL
+    # the rounding itself: an eighth of the weights' spread at most, so near the layer but not it
+    full = exact(copy.deepcopy(m).cpu(), x, c, g)
+    assert 1e-3 < float((full[1] - want[1]).abs().max()) < float(full[1].abs().max())
+    with torch.no_grad():
+        m.conv1x1_skip.bias.add_(1.0)   # changed weights are rounded again
+    m.clear_buffer()
+    s2 = m.incremental_forward(x[:, :, 0].cuda()[:, None], c[:, :, 0].cuda()[:, None], g[:, :, 0].cuda()[:, None])[1]
+    assert float((s2 - steps[0][1] - 1.0).abs().max()) < 1e-5
+    m.quantize_(None)
+    m.clear_buffer()
+    dense = m.incremental_forward(x[:, :, 0].cuda()[:, None], c[:, :, 0].cuda()[:, None], g[:, :, 0].cuda()[:, None])[1]
+    assert float((dense[:, 0].double().cpu() - full[1][..., 0] - 1.0).abs().max()) < TOL
+
+
+def test_without_conditioning_and_next_to_the_convolution():
+    m = layer(17, cin_channels=-1, gin_channels=-1).cuda().eval()
+    n = ResidualConv1dGLU(48, 64, kernel_size=2, skip_out_channels=40, dilation=2).cuda().eval()
+    x = torch.randn(2, 48, 20, device="cuda")
+    with torch.no_grad():
+        a, s1 = m(x)
+        b, s2 = n(a)
+        full = s1 + s2
+    for q in (None, 32):
+        m.quantize_(q)
+        m.clear_buffer()
+        n.clear_buffer()
+        skips = []
+        for t in range(20):
+            a1, k1 = m.incremental_forward(x[:, :, t][:, None])
+            _, k2 = n.incremental_forward(a1)
+            skips.append(k1 + k2)
+        if q is None:
+            assert float((torch.cat(skips, 1).transpose(1, 2) - full).abs().max()) < TOL
+    m.train()
+    with pytest.raises(RuntimeError, match="eval mode"):
+        m.incremental_forward(x[:, :, 0][:, None])

@@ -11,6 +11,7 @@ import torch
 from tests._ops import oracle_scan, q4_weight, random_q4
 from wavenet_vocoder_amd import _lib
 from wavenet_vocoder_amd.engine import Q4Linear
+from wavenet_vocoder_amd.modules import ResidualRecurrentGLU
 from wavenet_vocoder_amd.recurrence import gated_recurrence, gated_recurrence_step
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -24,6 +25,15 @@ def test_no_cpu_path():
         gated_recurrence_step(torch.zeros(1, 6), torch.zeros(1, 2))
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         Q4Linear(64, 64, torch.device("cpu"))
+    m = ResidualRecurrentGLU(8, 12, skip_out_channels=4).eval()
+    with pytest.raises(RuntimeError, match="HIP device"):
+        m(torch.zeros(1, 8, 3))
+    with pytest.raises(RuntimeError, match="HIP device"):
+        m.incremental_forward(torch.zeros(1, 1, 8))
+    with pytest.raises(RuntimeError, match="HIP device"):
+        m.quantize_(32).incremental_forward(torch.zeros(1, 1, 8))
+    assert sorted(m.state_dict()) == ["conv1x1_in.bias", "conv1x1_in.weight", "conv1x1_out.bias", "conv1x1_out.weight", "conv1x1_skip.bias",
+                                      "conv1x1_skip.weight"]
 
 
 def status(fn, *args):
