@@ -381,3 +381,55 @@ def test_steps_far_apart():
     v = torch.empty(2 * far + 24, dtype=torch.bfloat16, device="cuda").as_strided((1, 3, 24), (3 * far, far, 1))
     v.copy_(z)
     assert torch.equal(gated_recurrence(v, h0.cuda())[0], gated_recurrence(z.cuda(), h0.cuda())[0])
+
+
+def test_refusals_on_the_device():
+    z = torch.zeros(2, 5, 12, device="cuda")
+    ok = torch.zeros(2, 4, device="cuda")
+    i32 = torch.int32
+    for bad, err in ((dict(z=z[0]), ValueError), (dict(z=z[..., :11]), ValueError), (dict(z=z[:0]), ValueError), (dict(z=z[:, :0]), ValueError),
+                     (dict(z=z[..., :0]), ValueError), (dict(z=z.double()), TypeError), (dict(h0=ok[:1]), ValueError),
+                     (dict(h0=ok.double()), TypeError), (dict(h0=ok.cpu()), ValueError), (dict(lengths=torch.zeros(3, dtype=i32, device="cuda")), ValueError),
+                     (dict(lengths=torch.zeros(2, device="cuda")), TypeError), (dict(lengths=torch.zeros(2, dtype=i32)), ValueError),
+                     (dict(seg_start=torch.zeros(2, 4, dtype=i32, device="cuda")), ValueError)):
+        a = dict(z=z)
+        a.update(bad)
+        with pytest.raises(err):
+            gated_recurrence(a.pop("z"), a.pop("h0", None), **a)
+    zs, st = torch.zeros(2, 12, device="cuda"), torch.zeros(2, 4, device="cuda")
+    for zz, ss, err in ((zs[:, :11], st, ValueError), (zs[0], st, ValueError), (zs[:0], st[:0], ValueError), (zs.double(), st, TypeError),
+                        (zs, st[:1], ValueError), (zs, st.double(), TypeError), (zs, st.cpu(), ValueError), (zs.cpu(), st, RuntimeError),
+                        (zs, torch.zeros(2, 8, device="cuda")[:, ::2], ValueError), (zs, torch.zeros(1, 4, device="cuda").expand(2, 4), ValueError),
+                        (zs.clone().requires_grad_(), st, RuntimeError), (zs, st.clone().requires_grad_(), RuntimeError)):
+        with pytest.raises(err):
+            gated_recurrence_step(zz, ss)
+    w = z.clone().requires_grad_()
+    y, _ = gated_recurrence(w)
+    g, = torch.autograd.grad(y.sum(), w, create_graph=True)     # asked for, though nothing goes through it
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), w)
+
+
+def test_lengths_outside_the_sequence_and_of_64_bits():
+    z, h0, dy, dh = inputs(4, 90, 12, 3, torch.float32, seed=71)
+    want = run(z, h0, dy, dh, 3, dict(lengths=torch.tensor([0, 90, 7, 90], dtype=torch.int32)))
+    got = run(z, h0, dy, dh, 3, dict(lengths=torch.tensor([-5, 2 ** 40, 7, 91])))
+    for k in want:
+        assert torch.equal(got[k], want[k]), k
+
+
+def test_work_under_way_on_another_stream():
+    """The call runs on the current stream and waits there for the inputs' producer."""
+    z, h0, _, _ = (t.cuda() for t in inputs(2, 2000, 64, 3, torch.float32, seed=73))
+    want = gated_recurrence(z, h0)
+    s = torch.cuda.Stream()
+    for _ in range(5):
+        late = torch.zeros_like(z)
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            for _ in range(20):
+                late.copy_(z * 0.5)
+            late.copy_(z)
+            y, h = gated_recurrence(late, h0)
+        torch.cuda.current_stream().wait_stream(s)
+        assert torch.equal(y, want[0]) and torch.equal(h, want[1])

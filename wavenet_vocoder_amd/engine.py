@@ -141,6 +141,9 @@ def _empty_pinned():
     return b
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream          # of a device by its index: the layer-level steps are a few microseconds long
+
+
 def _stream(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
@@ -442,6 +445,8 @@ class Q4Linear:
         self.cin, self.cout, self.group_size, self.gates = int(cin), int(cout), int(group_size), int(gates)
         check(_lib.lib().wnv_q4_create(self.cin, self.cout, self.gates, self.group_size, idx, C.byref(self._h)))
         self.channels = self.cout // self.gates
+        self._index = idx
+        self._step, self._recurrence_step = _lib.lib().wnv_q4_step, _lib.lib().wnv_q4_recurrence_step
 
     def _given(self, t: torch.Tensor, what: str, shape, dtype: torch.dtype) -> torch.Tensor:
         if tuple(t.shape) != tuple(shape):
@@ -476,46 +481,47 @@ class Q4Linear:
         check(_lib.lib().wnv_q4_dequantise(self._h, w.data_ptr(), _stream(self.device)))
         return w
 
-    def _x(self, x: torch.Tensor) -> int:
-        code = self._DTYPES.get(x.dtype)
-        if x.get_device() != self.device.index:
-            require_gpu_tensor(x, "x")
+    def _refuse(self, x: torch.Tensor) -> None:
+        require_gpu_tensor(x, "x")
+        if x.get_device() != self._index:
             raise ValueError(f"x lives on {x.device}, the weights on {self.device}")
-        shape = x.shape
-        if len(shape) != 2 or shape[1] != self.cin or shape[0] == 0:
-            raise ValueError(f"x is {tuple(shape)}, expected (B, {self.cin})")
-        if code is None:
+        if x.dim() != 2 or x.shape[1] != self.cin or x.shape[0] == 0:
+            raise ValueError(f"x is {tuple(x.shape)}, expected (B, {self.cin})")
+        if x.dtype not in self._DTYPES:
             raise TypeError(f"x is {x.dtype}: float32, bfloat16 and float16 are implemented")
-        if x.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError("4-bit products are not differentiable: use torch.no_grad()")
-        return code
+        raise RuntimeError("4-bit products are not differentiable: use torch.no_grad()")
+
+    def _rows(self, x: torch.Tensor):
+        """x as the kernels take it, its number of rows and its type."""
+        shape = x.shape
+        code = self._DTYPES.get(x.dtype)
+        if (code is None or x.get_device() != self._index or len(shape) != 2 or shape[1] != self.cin or shape[0] == 0
+                or (x.requires_grad and torch.is_grad_enabled())):
+            self._refuse(x)
+        return (x if x.stride(1) == 1 else x.contiguous()), shape[0], code
 
     def step(self, x: torch.Tensor) -> torch.Tensor:
         """x (B, cin) float32, bfloat16 or float16 -> (B, cout) of the same type."""
-        code = self._x(x)
-        if x.stride(1) != 1:
-            x = x.contiguous()
-        B = x.shape[0]
-        y = torch.empty(B, self.cout, device=self.device, dtype=x.dtype)
-        check(_lib.lib().wnv_q4_step(self._h, x.data_ptr(), x.stride(0), y.data_ptr(), B, code,
-                                     torch._C._cuda_getCurrentRawStream(self.device.index)))
+        x, B, code = self._rows(x)
+        y = x.new_empty((B, self.cout))
+        st = self._step(self._h, x.data_ptr(), x.stride(0), y.data_ptr(), B, code, _raw_stream(self._index))
+        if st:
+            check(st)
         return y
 
     def recurrence_step(self, x: torch.Tensor, state: torch.Tensor) -> torch.Tensor:
         """x (B, cin), ``state`` (B, channels) float32 contiguous, updated in place -> y (B, channels) of x's type."""
-        code = self._x(x)
-        B = x.shape[0]
+        x, B, code = self._rows(x)
         if state.shape != (B, self.channels):
             raise ValueError(f"state is {tuple(state.shape)}, expected {(B, self.channels)}")
-        if state.dtype != torch.float32 or state.get_device() != self.device.index or not state.is_contiguous():
+        if state.dtype != torch.float32 or state.get_device() != self._index or not state.is_contiguous():
             raise ValueError("state is updated in place: it has to be float32, contiguous and on x's device")
         if state.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("4-bit products are not differentiable: use torch.no_grad()")
-        if x.stride(1) != 1:
-            x = x.contiguous()
-        y = torch.empty(B, self.channels, device=self.device, dtype=x.dtype)
-        check(_lib.lib().wnv_q4_recurrence_step(self._h, x.data_ptr(), x.stride(0), state.data_ptr(), y.data_ptr(), B, code,
-                                                torch._C._cuda_getCurrentRawStream(self.device.index)))
+        y = x.new_empty((B, self.channels))
+        st = self._recurrence_step(self._h, x.data_ptr(), x.stride(0), state.data_ptr(), y.data_ptr(), B, code, _raw_stream(self._index))
+        if st:
+            check(st)
         return y
 
     def __del__(self):  # pragma: no cover

@@ -18,12 +18,11 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import DTYPE, RecurrenceArgs, check
-from .engine import require_gpu_tensor
+from .engine import _raw_stream, require_gpu_tensor
 
 __all__ = ["gated_recurrence", "gated_recurrence_step"]
 
 _DTYPES = {getattr(torch, name): code for name, code in DTYPE.items()}
-_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _dtype(z: torch.Tensor) -> int:
@@ -88,7 +87,7 @@ def _forward(z, h0, gates, lengths, seg_start, keep: bool):
     n //= gates
     code, dev = _DTYPES[z.dtype], z.device
     saved_bytes, ws_bytes = _sizes(B, T, n, gates, code)
-    y = torch.empty(B, T, n, dtype=z.dtype, device=dev)
+    y = z.new_empty((B, T, n))
     h_last = torch.empty(B, n, dtype=torch.float32, device=dev)
     saved = torch.empty(saved_bytes, dtype=torch.uint8, device=dev) if keep else None
     _call(_lib.lib().wnv_recurrence_forward, z, B, T, n, gates, code, ws_bytes, h0, lengths, seg_start, y, h_last, saved, None, None, None,
@@ -103,7 +102,7 @@ def _backward(ctx, dy, dh_last):
     n //= gates
     code, dev = _DTYPES[z.dtype], z.device
     needs_z, needs_h0 = ctx.needs_input_grad[:2]
-    dz = torch.empty(B, T, gates * n, dtype=z.dtype, device=dev)
+    dz = z.new_empty((B, T, gates * n))
     dh0 = torch.empty(B, n, dtype=torch.float32, device=dev) if needs_h0 else None
     _call(_lib.lib().wnv_recurrence_backward, z, B, T, n, gates, code, _sizes(B, T, n, gates, code)[1], h0, lengths, seg_start, None, None,
           saved, None if dy is None else _rows(dy), None if dh_last is None else dh_last.contiguous(), dz, dh0)
@@ -162,22 +161,26 @@ def gated_recurrence(z: torch.Tensor, h0: Optional[torch.Tensor] = None, *, outp
 def gated_recurrence_step(z: torch.Tensor, state: torch.Tensor, *, output_gate: bool = True) -> torch.Tensor:
     """One step: z (B, 3 C) (``output_gate=False``: (B, 2 C)), ``state`` (B, C) float32 contiguous, updated in place -> y (B, C) of z's
     type.  Not differentiable: the training form is ``gated_recurrence``."""
-    require_gpu_tensor(z, "z")
-    code = _dtype(z)
-    if z.dim() != 2:
-        raise ValueError(f"z is {tuple(z.shape)}, expected (B, channels)")
-    gates = 3 if output_gate else 2
-    B, n = z.shape
-    if B == 0 or n == 0 or n % gates:
-        raise ValueError(f"z is {tuple(z.shape)}, expected (B, {gates} gates of the same size), neither of them empty")
-    n //= gates
-    if not _state(state, "state", B, n, z).is_contiguous():
-        raise ValueError("state is updated in place: it has to be contiguous")
-    if (z.requires_grad or state.requires_grad) and torch.is_grad_enabled():
-        raise RuntimeError("gated_recurrence_step is not differentiable: use gated_recurrence, or torch.no_grad()")
+    shape, sshape, gates, dev = z.shape, state.shape, 3 if output_gate else 2, z.get_device()
+    code = _DTYPES.get(z.dtype)
+    if (code is None or dev < 0 or len(shape) != 2 or len(sshape) != 2 or sshape[0] != shape[0] or sshape[1] * gates != shape[1]
+            or not z.numel() or state.dtype != torch.float32 or state.get_device() != dev or not state.is_contiguous()
+            or ((z.requires_grad or state.requires_grad) and torch.is_grad_enabled())):
+        _refuse_step(z, state, gates)
+    B, n = sshape
     z = _rows(z)
-    y = torch.empty(B, n, dtype=z.dtype, device=z.device)
-    dev = z.get_device()
-    check(_lib.lib().wnv_recurrence_step(dev, z.data_ptr(), z.stride(0), state.data_ptr(), y.data_ptr(), B, n, gates, code,
-                                         _raw_stream(dev)))
+    y = z.new_empty(sshape)
+    st = _lib.lib().wnv_recurrence_step(dev, z.data_ptr(), z.stride(0), state.data_ptr(), y.data_ptr(), B, n, gates, code, _raw_stream(dev))
+    if st:
+        check(st)
     return y
+
+
+def _refuse_step(z, state, gates):
+    require_gpu_tensor(z, "z")
+    _dtype(z)
+    if z.dim() != 2 or not z.numel() or z.shape[1] % gates:
+        raise ValueError(f"z is {tuple(z.shape)}, expected (B, {gates} gates of the same size), neither of them empty")
+    if not _state(state, "state", z.shape[0], z.shape[1] // gates, z).is_contiguous():
+        raise ValueError("state is updated in place: it has to be contiguous")
+    raise RuntimeError("gated_recurrence_step is not differentiable: use gated_recurrence, or torch.no_grad()")
