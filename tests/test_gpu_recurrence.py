@@ -51,7 +51,7 @@ def run(z, h0, dy, dh, gates, m, grads=True):
 
 
 SHAPES = [(1, 1, 1), (2, 2, 3), (3, 7, 20), (2, 127, 64), (2, 128, 65), (3, 129, 33), (1, 300, 128), (2, 513, 17), (4, 1000, 72),
-          (1, 2500, 8), (2, 1025, 201), (1, 4097, 40)]
+          (1, 2500, 8), (2, 1025, 201), (1, 4097, 40), (2, 511, 2), (1, 513, 3), (3, 1500, 4), (2, 9000, 16), (1, 2100, 17)]
 
 
 @pytest.mark.parametrize("dtype", sorted(DTYPES))
@@ -375,7 +375,7 @@ def test_offsets_of_the_step_over_32_bits():
 
 
 def test_steps_far_apart():
-    """Time strides of 2^22 elements and more are copied once."""
+    """Time strides of 2^20 elements and more are copied once."""
     z, h0, dy, dh = inputs(1, 3, 8, 3, torch.bfloat16, seed=61)
     far = (1 << 22) + 16
     v = torch.empty(2 * far + 24, dtype=torch.bfloat16, device="cuda").as_strided((1, 3, 24), (3 * far, far, 1))

@@ -137,8 +137,10 @@ __device__ __forceinline__ bool ends_section(int k, int chunks) { return (k + 1)
 // Registers decide how many workgroups share a CU: 3 forward and 2 backward, each with 32 steps x channels a thread.  Half the steps
 // and 3 workgroups backward took 356 us for 316.  The last lane of a tile that ends in no multiple of V
 // starts earlier and shares channels with its neighbour (both compute and write the same); V = 1 is for rows narrower than 4.
-constexpr int WAVES = 4, THREADS = 64 * WAVES, LANES = 16, STRETCHES = THREADS / LANES;
-constexpr int L = 8;
+constexpr int WAVES = 4, THREADS = 64 * WAVES, L = 8;
+template <int LANES> struct Shape {
+    static constexpr int ROWS = 64 / LANES, STRETCHES = WAVES * ROWS, WAVE_STEPS = ROWS * L, STEPS = STRETCHES * L;
+};
 
 // V elements as they stand in memory, packed in as few registers; addresses are a uniform base and 32 bits of a lane's own.
 template <typename E, int V> struct Vec {
@@ -171,19 +173,32 @@ template <typename E, int V> __device__ __forceinline__ void store(E* base, uint
     __builtin_nontemporal_store(r, (R*)((char*)base + bytes));
 }
 
-// The maps of a wave's four rows joined in time (BACK: the last row first): of all four, and of those before the own row.
-template <bool BACK, bool SEG> __device__ __forceinline__ void join_rows(Map x, Map& all, Map& before) {
-    const auto u = __builtin_amdgcn_permlane16_swap(__float_as_uint(x.u), __float_as_uint(x.u), false, false);     // rows 0 0 2 2 | 1 1 3 3
-    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x.b), __float_as_uint(x.b), false, false);
-    const Map even{__uint_as_float(u[0]), __uint_as_float(b[0])}, odd{__uint_as_float(u[1]), __uint_as_float(b[1])};
-    const Map pair = BACK ? join<SEG>(odd, even) : join<SEG>(even, odd);
-    const auto pu = __builtin_amdgcn_permlane32_swap(__float_as_uint(pair.u), __float_as_uint(pair.u), false, false);  // rows 0 1 0 1 | 2 3 2 3
-    const auto pb = __builtin_amdgcn_permlane32_swap(__float_as_uint(pair.b), __float_as_uint(pair.b), false, false);
-    const Map low{__uint_as_float(pu[0]), __uint_as_float(pb[0])}, high{__uint_as_float(pu[1]), __uint_as_float(pb[1])};
-    const int row = (threadIdx.x / LANES) & 3;
-    all = BACK ? join<SEG>(high, low) : join<SEG>(low, high);
-    before = (row & 1) != BACK ? (BACK ? odd : even) : Map{0.f, 0.f};
-    if ((row >> 1) != BACK) before = join<SEG>(BACK ? high : low, before);
+// The maps of a wave's rows joined in time (BACK: the last row first): of all of them, and of those before the own row.
+template <int LANES, bool BACK, bool SEG> __device__ __forceinline__ void join_rows(Map x, Map& all, Map& before) {
+    if constexpr (LANES == 16) {        // four rows: two exchanges of registers, no LDS
+        const auto u = __builtin_amdgcn_permlane16_swap(__float_as_uint(x.u), __float_as_uint(x.u), false, false);     // rows 0 0 2 2 | 1 1 3 3
+        const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x.b), __float_as_uint(x.b), false, false);
+        const Map even{__uint_as_float(u[0]), __uint_as_float(b[0])}, odd{__uint_as_float(u[1]), __uint_as_float(b[1])};
+        const Map pair = BACK ? join<SEG>(odd, even) : join<SEG>(even, odd);
+        const auto pu = __builtin_amdgcn_permlane32_swap(__float_as_uint(pair.u), __float_as_uint(pair.u), false, false);  // rows 0 1 0 1 | 2 3 2 3
+        const auto pb = __builtin_amdgcn_permlane32_swap(__float_as_uint(pair.b), __float_as_uint(pair.b), false, false);
+        const Map low{__uint_as_float(pu[0]), __uint_as_float(pb[0])}, high{__uint_as_float(pu[1]), __uint_as_float(pb[1])};
+        const int row = (threadIdx.x / LANES) & 3;
+        all = BACK ? join<SEG>(high, low) : join<SEG>(low, high);
+        before = (row & 1) != BACK ? (BACK ? odd : even) : Map{0.f, 0.f};
+        if ((row >> 1) != BACK) before = join<SEG>(BACK ? high : low, before);
+    } else {                            // each row joined to the one 1, 2, 4, ... rows before it
+        const int row = BACK ? 63 / LANES - threadIdx.x % 64 / LANES : threadIdx.x % 64 / LANES;
+#pragma unroll
+        for (int d = LANES; d < 64; d *= 2) {
+            const Map other{BACK ? __shfl_down(x.u, d) : __shfl_up(x.u, d), BACK ? __shfl_down(x.b, d) : __shfl_up(x.b, d)};
+            if (row >= d / LANES) x = join<SEG>(other, x);
+        }
+        const int last = (BACK ? 0 : 64 - LANES) + threadIdx.x % LANES;
+        all = {__shfl(x.u, last), __shfl(x.b, last)};
+        before = {BACK ? __shfl_down(x.u, LANES) : __shfl_up(x.u, LANES), BACK ? __shfl_down(x.b, LANES) : __shfl_up(x.b, LANES)};
+        if (row == 0) before = {0.f, 0.f};
+    }
 }
 
 struct Place { int b, tile, chunk, row; };
@@ -213,31 +228,47 @@ template <bool BACK> __device__ __forceinline__ Place draw_place(const RecArgs& 
 __device__ __forceinline__ int live_steps(const RecArgs& a, int b, int t0) {
     return max(0, min(L, (a.lengths ? min(a.lengths[b], a.T) : a.T) - t0));
 }
-// The wave's 32 entries of the map in one load (asked for ahead of the data), a lane each; a stretch takes its 8 bits of the ballot.
-template <bool SEG> __device__ __forceinline__ int map_entry(const RecArgs& a, int b, int chunk) {
-    const int t = chunk * (STRETCHES * L) + threadIdx.x / 64 * (4 * L) + threadIdx.x % 64;
-    return SEG && threadIdx.x % 64 < 4 * L && t < a.T ? a.seg_start[(long long)b * a.T + t] - t : 1;
+// The wave's entries of the map in one or two loads (asked for ahead of the data), a lane each; a stretch takes its 8 bits of a ballot.
+template <int LANES> struct Entries { int e[(Shape<LANES>::WAVE_STEPS + 63) / 64]; };
+template <int LANES, bool SEG> __device__ __forceinline__ Entries<LANES> map_entries(const RecArgs& a, int b, int chunk) {
+    constexpr int N = Shape<LANES>::WAVE_STEPS;
+    Entries<LANES> r{};
+    if (SEG) {
+#pragma unroll
+        for (int i = 0; i < (N + 63) / 64; ++i) {
+            const int at = 64 * i + threadIdx.x % 64, t = chunk * Shape<LANES>::STEPS + threadIdx.x / 64 * N + at;
+            r.e[i] = at < N && t < a.T ? a.seg_start[(long long)b * a.T + t] - t : 1;
+        }
+    }
+    return r;
 }
-template <bool SEG> __device__ __forceinline__ int begins_in(int entry, int live) {
-    static_assert(L == 8, "a stretch is a byte of the ballot");
-    return SEG ? (int)(__ballot(entry == 0) >> (threadIdx.x / LANES % 4 * L)) & ((1 << live) - 1) : 0;
+template <int LANES, bool SEG> __device__ __forceinline__ int begins_in(const Entries<LANES>& entries, int live) {
+    static_assert(L == 8, "a stretch is a byte of a ballot");
+    if (!SEG) return 0;
+    const int row = threadIdx.x % 64 / LANES;
+    unsigned long long bits = __ballot(entries.e[0] == 0);
+    if constexpr (Shape<LANES>::WAVE_STEPS > 64) {
+        const unsigned long long more = __ballot(entries.e[1] == 0);
+        if (row >= 8) bits = more;
+    }
+    return (int)(bits >> (row % 8 * L)) & ((1 << live) - 1);
 }
 
 // One chunk of one tile.  Each thread reduces its stretch to a map, the wave joins its four, wave 0 the chunk's and its group's while
 // waves 1 and 2 find the state before the group; then each thread knows the state before its stretch and runs over it again, out of its
 // registers.  z is read once.
-template <typename E, int G, int V, bool SEG>
+template <typename E, int G, int V, int LANES, bool SEG>
 __global__ void __launch_bounds__(THREADS, SEG && sizeof(E) == 2 ? 4 : 3) wnv_recurrence_fwd(RecArgs a) {
-    constexpr int W = LANES * V;
+    constexpr int W = LANES * V, STEPS = Shape<LANES>::STEPS;
     __shared__ Map totals[WAVES][W], prev[W], groups[W];
     __shared__ float base[W];
     const int tid = threadIdx.x, lane = tid % LANES, wave = tid / 64, at = lane * V;
     const Place p = draw_place<false>(a, W);
     const bool on = p.tile * W + at < a.C;
     const int c = min(p.tile * W + at, a.C - V);
-    const int t0 = p.chunk * (STRETCHES * L) + tid / LANES * L, steps = live_steps(a, p.b, t0), live = on ? steps : 0;
-    const int entry = map_entry<SEG>(a, p.b, p.chunk);
-    const E* z = (const E*)a.z + (long long)p.b * a.zb + (long long)p.chunk * (STRETCHES * L) * a.zt;
+    const int t0 = p.chunk * STEPS + tid / LANES * L, steps = live_steps(a, p.b, t0), live = on ? steps : 0;
+    const Entries<LANES> entries = map_entries<LANES, SEG>(a, p.b, p.chunk);
+    const E* z = (const E*)a.z + (long long)p.b * a.zb + (long long)p.chunk * STEPS * a.zt;
     const uint32_t from = (uint32_t)(tid / LANES * L * a.zt + c) * (uint32_t)sizeof(E);
 
     Vec<E, V> f[L], v[L], o[L];
@@ -248,7 +279,7 @@ __global__ void __launch_bounds__(THREADS, SEG && sizeof(E) == 2 ? 4 : 3) wnv_re
             v[l] = load<E, V>(z + l * a.zt + a.C, from);
             if (G == 3) o[l] = load<E, V>(z + l * a.zt + 2 * a.C, from);
         }
-    const int begins = begins_in<SEG>(entry, steps);
+    const int begins = begins_in<LANES, SEG>(entries, steps);
     float u[L][V];
     Map m[V], before[V];
 #pragma unroll
@@ -268,7 +299,7 @@ __global__ void __launch_bounds__(THREADS, SEG && sizeof(E) == 2 ? 4 : 3) wnv_re
     for (int i = 0; i < V; ++i) {
         if (SEG && begins) m[i].u = -1.f;
         Map all;
-        join_rows<false, SEG>(m[i], all, before[i]);
+        join_rows<LANES, false, SEG>(m[i], all, before[i]);
         if (tid % 64 < LANES) totals[wave][at + i] = all;
     }
     __syncthreads();
@@ -303,7 +334,7 @@ __global__ void __launch_bounds__(THREADS, SEG && sizeof(E) == 2 ? 4 : 3) wnv_re
             if (p.chunk + 1 == a.chunks && on) a.h_last[(long long)p.b * a.C + c + i] = last;
         }
     }
-    E* y = (E*)a.y + ((long long)p.b * a.T + (long long)p.chunk * (STRETCHES * L)) * a.C;
+    E* y = (E*)a.y + ((long long)p.b * a.T + (long long)p.chunk * STEPS) * a.C;
     const uint32_t to = (uint32_t)(tid / LANES * L * a.C + c) * (uint32_t)sizeof(E);
 #pragma unroll
     for (int l = 0; l < L; ++l)
@@ -328,9 +359,9 @@ __global__ void __launch_bounds__(THREADS, SEG && sizeof(E) == 2 ? 4 : 3) wnv_re
 // df = dh (h_{t-1} - v) sigmoid(f) u;  dv = dh u;  do = dy h sigmoid(o) (1 - sigmoid(o))
 // The chunks run from the last to the first, r is found the way the forward pass finds h; h itself starts from the state that the
 // forward pass saved before each chunk and is run through again.
-template <typename E, int G, int V, bool SEG>
+template <typename E, int G, int V, int LANES, bool SEG>
 __global__ void __launch_bounds__(THREADS, 2) wnv_recurrence_bwd(RecArgs a) {
-    constexpr int W = LANES * V;
+    constexpr int W = LANES * V, STEPS = Shape<LANES>::STEPS;
     __shared__ Map ahead[WAVES][W], back[WAVES][W], prev[W], groups[W];        // of h and of r
     __shared__ float base[W];
     const int tid = threadIdx.x, lane = tid % LANES, wave = tid / 64, at = lane * V;
@@ -338,10 +369,10 @@ __global__ void __launch_bounds__(THREADS, 2) wnv_recurrence_bwd(RecArgs a) {
     const int order = a.chunks - 1 - p.chunk;
     const bool on = p.tile * W + at < a.C;
     const int c = min(p.tile * W + at, a.C - V);
-    const int t0 = p.chunk * (STRETCHES * L) + tid / LANES * L, steps = live_steps(a, p.b, t0), live = on ? steps : 0;
-    const int entry = map_entry<SEG>(a, p.b, p.chunk);
-    const E* z = (const E*)a.z + (long long)p.b * a.zb + (long long)p.chunk * (STRETCHES * L) * a.zt;
-    const E* dy = (const E*)a.dy + (long long)p.b * a.dyb + (long long)p.chunk * (STRETCHES * L) * a.dyt;
+    const int t0 = p.chunk * STEPS + tid / LANES * L, steps = live_steps(a, p.b, t0), live = on ? steps : 0;
+    const Entries<LANES> entries = map_entries<LANES, SEG>(a, p.b, p.chunk);
+    const E* z = (const E*)a.z + (long long)p.b * a.zb + (long long)p.chunk * STEPS * a.zt;
+    const E* dy = (const E*)a.dy + (long long)p.b * a.dyb + (long long)p.chunk * STEPS * a.dyt;
     const uint32_t from = (uint32_t)(tid / LANES * L * a.zt + c) * (uint32_t)sizeof(E);
     const uint32_t dfrom = (uint32_t)(tid / LANES * L * a.dyt + c) * (uint32_t)sizeof(E);
 
@@ -355,7 +386,7 @@ __global__ void __launch_bounds__(THREADS, 2) wnv_recurrence_bwd(RecArgs a) {
             if (a.dy) d[l] = load<E, V>(dy + l * a.dyt, dfrom);
         }
     const Vec<float, V> saved = load<float, V>(a.saved + ((long long)p.row * a.chunks + p.chunk) * W, at * 4);
-    const int begins = begins_in<SEG>(entry, steps);
+    const int begins = begins_in<LANES, SEG>(entries, steps);
     float u[L][V], uk[L][V], g[L][V], q[L][V];          // u sigmoid(f); dy sigmoid(o); dy sigmoid(o) (1 - sigmoid(o))
     Map m[V], r[V];
 #pragma unroll
@@ -392,8 +423,8 @@ __global__ void __launch_bounds__(THREADS, 2) wnv_recurrence_bwd(RecArgs a) {
         if (SEG && begins) m[i].u = -1.f;
         r[i].u = m[i].u;
         Map all, all_back;
-        join_rows<false, SEG>(m[i], all, h_before[i]);
-        join_rows<true, SEG>(r[i], all_back, r_before[i]);
+        join_rows<LANES, false, SEG>(m[i], all, h_before[i]);
+        join_rows<LANES, true, SEG>(r[i], all_back, r_before[i]);
         if (tid % 64 < LANES) ahead[wave][at + i] = all, back[wave][at + i] = all_back;
     }
     __syncthreads();
@@ -436,7 +467,7 @@ __global__ void __launch_bounds__(THREADS, 2) wnv_recurrence_bwd(RecArgs a) {
                 h = fmaf(u[l][i], v[l].get(i) - before[l][i], before[l][i]);
             }
     }
-    E* dz = (E*)a.dz + ((long long)p.b * a.T + (long long)p.chunk * (STRETCHES * L)) * (G * (long long)a.C);
+    E* dz = (E*)a.dz + ((long long)p.b * a.T + (long long)p.chunk * STEPS) * (G * (long long)a.C);
     const uint32_t to = (uint32_t)(tid / LANES * L * G * a.C + c) * (uint32_t)sizeof(E);
 #pragma unroll
     for (int l = L - 1; l >= 0; --l)
@@ -504,21 +535,31 @@ wnv_status launched(const char* who) {
     return e == hipSuccess ? WNV_OK : fail(WNV_ERR_HIP, "%s: launch failed: %s", who, hipGetErrorString(e));
 }
 
+// Up to here a tile is 16 channels (4 with V = 1) and a chunk 512 steps, beyond 64 and 128: where rows are narrow, lanes along the
+// channels are idle, and with them go a quarter of the chunks to wait for (forward and backward of 16 x 24064 float32, us: C = 5 92 and
+// 133 with wide tiles, C = 16 89 and 147; C = 20 219 and 162, for two narrow tiles read a row twice).
+constexpr int NARROW = 16;
+
 wnv_status check_strides(const char* who, const wnv_recurrence_args* a) {
     if (a->z_batch_stride < 0 || a->z_time_stride < 0 || (a->h0 && a->h0_batch_stride < 0) ||
         (a->dy && (a->dy_batch_stride < 0 || a->dy_time_stride < 0)))
         return fail(WNV_ERR_INVALID_ARG, "%s: negative stride", who);
-    if (a->T > 1 && (a->z_time_stride >= (1 << 22) || (a->dy && a->dy_time_stride >= (1 << 22))))
-        return fail(WNV_ERR_UNSUPPORTED, "%s: time strides of 2^22 elements and more", who);
+    // a lane's offset within a chunk is 32 bits
+    const int64_t most = a->C <= NARROW ? 1 << 20 : 1 << 22;
+    if (a->T > 1 && (a->z_time_stride >= most || (a->dy && a->dy_time_stride >= most)))
+        return fail(WNV_ERR_UNSUPPORTED, "%s: time strides of %lld elements and more", who, (long long)most);
     return WNV_OK;
 }
 
-struct Cut { int W, tiles, chunks; };
+struct Cut { int V, lanes, W, tiles, chunks; };
 Cut cut_of(int64_t T, int C) {
     Cut c;
-    c.W = LANES * (C < 4 ? 1 : 4);
+    c.V = C < 4 ? 1 : 4;
+    c.lanes = C <= NARROW ? 4 : 16;
+    c.W = c.lanes * c.V;
     c.tiles = (C + c.W - 1) / c.W;
-    c.chunks = (int)((T + STRETCHES * L - 1) / (STRETCHES * L));
+    const int steps = THREADS / c.lanes * L;
+    c.chunks = (int)((T + steps - 1) / steps);
     return c;
 }
 int64_t slot_bytes(int64_t B, const Cut& c) { return c.chunks > 1 ? B * c.tiles * slots_of_row(c.chunks, c.W) * 8 : 0; }
@@ -542,20 +583,25 @@ wnv_status prepare(const char* who, const wnv_recurrence_args* a, const Cut& c, 
     return WNV_OK;
 }
 
-template <typename E, int G, int V> void launch(bool back, const wnv_recurrence_args* a, const RecArgs& k) {
+template <typename E, int G, int V, int LANES> void launch(bool back, const wnv_recurrence_args* a, const RecArgs& k) {
     const dim3 grid((unsigned)((int64_t)k.B * k.tiles * k.chunks)), block(THREADS);
     hipStream_t s = (hipStream_t)a->stream;
     if (back) {
-        if (a->seg_start) hipLaunchKernelGGL((wnv_recurrence_bwd<E, G, V, true>), grid, block, 0, s, k);
-        else hipLaunchKernelGGL((wnv_recurrence_bwd<E, G, V, false>), grid, block, 0, s, k);
+        if (a->seg_start) hipLaunchKernelGGL((wnv_recurrence_bwd<E, G, V, LANES, true>), grid, block, 0, s, k);
+        else hipLaunchKernelGGL((wnv_recurrence_bwd<E, G, V, LANES, false>), grid, block, 0, s, k);
     } else {
-        if (a->seg_start) hipLaunchKernelGGL((wnv_recurrence_fwd<E, G, V, true>), grid, block, 0, s, k);
-        else hipLaunchKernelGGL((wnv_recurrence_fwd<E, G, V, false>), grid, block, 0, s, k);
+        if (a->seg_start) hipLaunchKernelGGL((wnv_recurrence_fwd<E, G, V, LANES, true>), grid, block, 0, s, k);
+        else hipLaunchKernelGGL((wnv_recurrence_fwd<E, G, V, LANES, false>), grid, block, 0, s, k);
     }
 }
-template <typename E> void launch(bool back, const wnv_recurrence_args* a, const RecArgs& k) {
-    if (a->gates == 3) a->C < 4 ? launch<E, 3, 1>(back, a, k) : launch<E, 3, 4>(back, a, k);
-    else a->C < 4 ? launch<E, 2, 1>(back, a, k) : launch<E, 2, 4>(back, a, k);
+template <typename E, int G> void launch(bool back, const wnv_recurrence_args* a, const Cut& c, const RecArgs& k) {
+    if (c.lanes == 16) launch<E, G, 4, 16>(back, a, k);
+    else if (c.V == 4) launch<E, G, 4, 4>(back, a, k);
+    else launch<E, G, 1, 4>(back, a, k);
+}
+template <typename E> void launch(bool back, const wnv_recurrence_args* a, const Cut& c, const RecArgs& k) {
+    if (a->gates == 3) launch<E, 3>(back, a, c, k);
+    else launch<E, 2>(back, a, c, k);
 }
 
 }  // namespace
@@ -580,7 +626,7 @@ extern "C" wnv_status wnv_recurrence_forward(int32_t device, const wnv_recurrenc
     RecArgs k{};
     const Cut c = cut_of(a->T, a->C);
     if (wnv_status st = prepare("wnv_recurrence_forward", a, c, k)) return st;
-    WNV_BY_TYPE(a->dtype, launch<E>(false, a, k));
+    WNV_BY_TYPE(a->dtype, launch<E>(false, a, c, k));
     return launched("wnv_recurrence_forward");
 }
 
@@ -593,7 +639,7 @@ extern "C" wnv_status wnv_recurrence_backward(int32_t device, const wnv_recurren
     RecArgs k{};
     const Cut c = cut_of(a->T, a->C);
     if (wnv_status st = prepare("wnv_recurrence_backward", a, c, k)) return st;
-    WNV_BY_TYPE(a->dtype, launch<E>(true, a, k));
+    WNV_BY_TYPE(a->dtype, launch<E>(true, a, c, k));
     return launched("wnv_recurrence_backward");
 }
 

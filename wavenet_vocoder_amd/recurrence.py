@@ -55,8 +55,9 @@ def _map(m: torch.Tensor, name: str, shape: Tuple[int, ...], z: torch.Tensor) ->
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
-    """``t`` with its last dimension contiguous: a copy only where it is not, or where steps lie 2^22 elements and more apart."""
-    return t if (t.stride(-1) == 1 or t.shape[-1] == 1) and (t.dim() < 3 or t.stride(1) < 1 << 22) else t.contiguous()
+    """``t`` with its last dimension contiguous: a copy only where it is not, or where steps lie 2^20 elements and more apart."""
+    n = t.shape[-1]
+    return t if (t.stride(-1) == 1 or n == 1) and (t.dim() < 3 or t.stride(1) < max(n + 1, 1 << 20)) else t.contiguous()
 
 
 @lru_cache(maxsize=256)
