@@ -216,29 +216,27 @@ template <int GROUPS> __device__ __forceinline__ Q4Block<GROUPS> load_block(cons
 }
 
 // NT tiles side by side (GATES > 0: one tile of each gate, of the same 16 channels, and the sums go straight into the recurrence's
-// step) x 16 rows of x.  A wave takes NT tiles (a gate's) and shares out the blocks of 128 inputs with the `split` waves of the same
-// tiles; their sums are joined in LDS in the waves' order: no atomics, and a row's result does not depend on the rows beside it (the
-// split goes by the weights' shape alone).
+// step) x 16 rows of x.  The blocks of 128 inputs are dealt to `split` slices, the slices to the `waves` waves of the same tiles (a
+// gate's); the slices' sums are joined in LDS in their order: no atomics, and a row's result does not depend on the rows beside it
+// (the split goes by the weights' shape alone).
 // STAGED: the rows of x go through LDS behind the first weights' request, and the parts of float32 rows are columns of their own there
 // (up to 5 rows); else each wave takes its own of x from L2, and the parts follow each other into sums of their own.  Both add the
 // parts' sums in the same order at the end: which of the two runs does not show in the result.  The weights of a wave's next block are
 // asked for before this one's products where registers allow it (STAGED).
 template <typename E, int NT, int GROUPS, int GATES, bool STAGED>
-__global__ void __launch_bounds__(1024) wnv_q4_rows(Q4Dev q, Q4Call a, int split, int most) {
+__global__ void __launch_bounds__(NT == 1 ? 1024 : 512) wnv_q4_rows(Q4Dev q, Q4Call a, int split, int waves, int most) {
     static_assert(!GATES || NT == 1, "a wave holds one gate");
-    extern __shared__ u32x4 shared[];   // STAGED: [part][row][16 kb + 1], 8 inputs each; then sums [wave][NT][SUMS][64]
+    extern __shared__ u32x4 shared[];   // STAGED: [part][row][16 kb + 1], 8 inputs each; then sums [gate][slice][NT][SUMS][64]
     constexpr int PARTS = Q4Type<E>::PARTS, SUMS = STAGED ? 1 : PARTS, JG = 4 / GROUPS;
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, r = lane % 16, quarter = lane / 16, slice = wave % split;
-    const int all = q.gates * q.tiles, tile0 = blockIdx.x * NT + (GATES ? wave / split * q.tiles : 0), b0 = blockIdx.y * most;
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, r = lane % 16, quarter = lane / 16;
+    const int all = q.gates * q.tiles, tile0 = blockIdx.x * NT + (GATES ? wave / waves * q.tiles : 0), b0 = blockIdx.y * most;
     const int rows = min(most, a.B - b0), pitch = 16 * q.kb + 1;          // a pitch of 16 bytes more spreads the rows over the banks
     const E* x = (const E*)a.x + (long long)(b0 + min(r, rows - 1)) * a.xs;
 
-    f32x4 acc[NT][SUMS] = {};
     Q4Block<GROUPS> f[NT] = {};
+    if (STAGED) {                       // one slice a wave: its first weights are on their way while x is staged
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
-        if (slice < q.kb) f[t] = load_block<GROUPS>(q, (long long)min(tile0 + t, all - 1) * q.kb + slice, lane);
-    if (STAGED) {
+        for (int t = 0; t < NT; ++t) f[t] = load_block<GROUPS>(q, (long long)min(tile0 + t, all - 1) * q.kb + wave % waves, lane);
         for (int i = threadIdx.x; i < rows * 16 * q.kb; i += blockDim.x) {
             const int row = i / (16 * q.kb), k = i - row * (16 * q.kb);
             u32x4 part[PARTS];
@@ -248,67 +246,71 @@ __global__ void __launch_bounds__(1024) wnv_q4_rows(Q4Dev q, Q4Call a, int split
         }
         __syncthreads();
     }
-    for (int kb = slice; kb < q.kb; kb += split) {
-        if (!STAGED && kb != slice) {
+    f32x4* sums = (f32x4*)shared + (STAGED ? PARTS * rows * pitch : 0);
+    for (int slice = wave % waves; slice < split; slice += waves) {
+        f32x4 acc[NT][SUMS] = {};
+        for (int kb = slice; kb < q.kb; kb += split) {
+            if (!STAGED) {
 #pragma unroll
-            for (int t = 0; t < NT; ++t) f[t] = load_block<GROUPS>(q, (long long)min(tile0 + t, all - 1) * q.kb + kb, lane);
-        }
-        Q4Block<GROUPS> next[NT] = {};
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-            if (STAGED && kb + split < q.kb) next[t] = load_block<GROUPS>(q, (long long)min(tile0 + t, all - 1) * q.kb + kb + split, lane);
-        Inputs<E> in[4] = {};
-        if (!STAGED) {
-            if ((kb + 1) * 128 <= q.cin) {
-                if (r < rows) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) in[j] = load_inputs<E>(x + kb * 128 + j * 32 + quarter * 8);
-                }
-            } else if (r < rows) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) in[j] = load_inputs<E>(x + kb * 128 + j * 32 + quarter * 8, q.cin - (kb * 128 + j * 32 + quarter * 8));
+                for (int t = 0; t < NT; ++t) f[t] = load_block<GROUPS>(q, (long long)min(tile0 + t, all - 1) * q.kb + kb, lane);
             }
-        }
+            Q4Block<GROUPS> next[NT] = {};
 #pragma unroll
-        for (int g = 0; g < GROUPS; ++g) {
-            f32x4 sum[NT][SUMS] = {};
+            for (int t = 0; t < NT; ++t)
+                if (STAGED && kb + split < q.kb) next[t] = load_block<GROUPS>(q, (long long)min(tile0 + t, all - 1) * q.kb + kb + split, lane);
+            Inputs<E> in[4] = {};
+            if (!STAGED) {
+                if ((kb + 1) * 128 <= q.cin) {
+                    if (r < rows) {
 #pragma unroll
-            for (int j = g * JG; j < (g + 1) * JG; ++j) {
-                u32x4 part[SUMS] = {};
-                if constexpr (!STAGED) parts_of<E>(in[j], part);
-                else if (r < PARTS * rows) part[0] = shared[r * pitch + kb * 16 + j * 4 + quarter];
+                        for (int j = 0; j < 4; ++j) in[j] = load_inputs<E>(x + kb * 128 + j * 32 + quarter * 8);
+                    }
+                } else if (r < rows) {
 #pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    const u32x4 w = codes_up<E>(j == 0 ? f[t].code.x : j == 1 ? f[t].code.y : j == 2 ? f[t].code.z : f[t].code.w);
-                    const u32x4 o = offset_of<E>(f[t].zero >> (8 * g) & 255);
+                    for (int j = 0; j < 4; ++j) in[j] = load_inputs<E>(x + kb * 128 + j * 32 + quarter * 8, q.cin - (kb * 128 + j * 32 + quarter * 8));
+                }
+            }
 #pragma unroll
-                    for (int p = 0; p < SUMS; ++p) {
-                        sum[t][p] = mfma<E>(w, part[p], sum[t][p]);
-                        sum[t][p] = mfma<E>(o, part[p], sum[t][p]);
+            for (int g = 0; g < GROUPS; ++g) {
+                f32x4 sum[NT][SUMS] = {};
+#pragma unroll
+                for (int j = g * JG; j < (g + 1) * JG; ++j) {
+                    u32x4 part[SUMS] = {};
+                    if constexpr (!STAGED) parts_of<E>(in[j], part);
+                    else if (r < PARTS * rows) part[0] = shared[r * pitch + kb * 16 + j * 4 + quarter];
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) {
+                        const u32x4 w = codes_up<E>(j == 0 ? f[t].code.x : j == 1 ? f[t].code.y : j == 2 ? f[t].code.z : f[t].code.w);
+                        const u32x4 o = offset_of<E>(f[t].zero >> (8 * g) & 255);
+#pragma unroll
+                        for (int p = 0; p < SUMS; ++p) {
+                            sum[t][p] = mfma<E>(w, part[p], sum[t][p]);
+                            sum[t][p] = mfma<E>(o, part[p], sum[t][p]);
+                        }
                     }
                 }
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const uint2 s = f[t].scale[g];
+                    const f32x4 scale{__uint_as_float(s.x << 16), __uint_as_float(s.x & 0xffff0000u), __uint_as_float(s.y << 16),
+                                      __uint_as_float(s.y & 0xffff0000u)};
+#pragma unroll
+                    for (int p = 0; p < SUMS; ++p)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) acc[t][p][i] = fmaf(scale[i], sum[t][p][i], acc[t][p][i]);
+                }
             }
+            if (STAGED) {
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const uint2 s = f[t].scale[g];
-                const f32x4 scale{__uint_as_float(s.x << 16), __uint_as_float(s.x & 0xffff0000u), __uint_as_float(s.y << 16),
-                                  __uint_as_float(s.y & 0xffff0000u)};
-#pragma unroll
-                for (int p = 0; p < SUMS; ++p)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[t][p][i] = fmaf(scale[i], sum[t][p][i], acc[t][p][i]);
+                for (int t = 0; t < NT; ++t) f[t] = next[t];
             }
         }
-        if (STAGED) {
+        f32x4* sum = sums + (long long)(wave / waves * split + slice) * (NT * SUMS * 64) + lane;
 #pragma unroll
-            for (int t = 0; t < NT; ++t) f[t] = next[t];
-        }
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int p = 0; p < SUMS; ++p) sum[(t * SUMS + p) * 64] = acc[t][p];
     }
-    f32x4* sums = (f32x4*)shared + (STAGED ? PARTS * rows * pitch : 0);
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int p = 0; p < SUMS; ++p) sums[((wave * NT + t) * SUMS + p) * 64 + lane] = acc[t][p];
     __syncthreads();
 
     // 16 neighbouring threads write 16 neighbouring outputs of a row; lane l of a result holds its column l % 16, rows 4 (l / 16) ...
@@ -353,28 +355,30 @@ __global__ void __launch_bounds__(1024) wnv_q4_rows(Q4Dev q, Q4Call a, int split
 //    types if a wave has several blocks of inputs to wait for (1 x 8192 x 8192 bf16: 11.1 and 13.2; 8 x 1616 x 512, one block a wave:
 //    4.6 and 3.9).
 //  * else two tiles a wave, which halves what is read of x, as soon as single tiles would be more workgroups than CUs (bf16
-//    64 x 4096 x 4096: 15.5 and 19.6, 48 x 2048 x 2048: 5.3 and 6.6; with fewer, 16 x 2048 x 2048: 5.0 and 4.4).
+//    64 x 4096 x 4096: 15.5 and 19.6, 48 x 2048 x 2048: 5.3 and 6.6; with fewer, 16 x 2048 x 2048: 5.0 and 4.4), and 8 waves of
+//    two slices, whose registers have room for it (64 x 8192 x 8192: bf16 40 and 47 with 16 waves, float32 83 and 106).
 constexpr size_t STAGE_MOST = 64 << 10;
 constexpr int CUS = 256;
 
 template <typename E, int NT, int GATES, bool STAGED>
-void launch(const Q4Dev& q, const Q4Call& a, int split, int most, size_t staged, hipStream_t s) {
-    const dim3 grid(GATES ? q.tiles : (q.gates * q.tiles + NT - 1) / NT, (a.B + most - 1) / most), block(64 * split * (GATES ? GATES : 1));
-    const size_t lds = (size_t)block.x * NT * 16 * (STAGED ? 1 : Q4Type<E>::PARTS) + staged;
-    if (q.per_block == 1) hipLaunchKernelGGL((wnv_q4_rows<E, NT, 1, GATES, STAGED>), grid, block, lds, s, q, a, split, most);
-    else if (q.per_block == 2) hipLaunchKernelGGL((wnv_q4_rows<E, NT, 2, GATES, STAGED>), grid, block, lds, s, q, a, split, most);
-    else hipLaunchKernelGGL((wnv_q4_rows<E, NT, 4, GATES, STAGED>), grid, block, lds, s, q, a, split, most);
+void launch(const Q4Dev& q, const Q4Call& a, int split, int waves, int most, size_t staged, hipStream_t s) {
+    constexpr int gates = GATES ? GATES : 1;
+    const dim3 grid(GATES ? q.tiles : (q.gates * q.tiles + NT - 1) / NT, (a.B + most - 1) / most), block(64 * waves * gates);
+    const size_t lds = (size_t)split * gates * NT * 1024 * (STAGED ? 1 : Q4Type<E>::PARTS) + staged;
+    if (q.per_block == 1) hipLaunchKernelGGL((wnv_q4_rows<E, NT, 1, GATES, STAGED>), grid, block, lds, s, q, a, split, waves, most);
+    else if (q.per_block == 2) hipLaunchKernelGGL((wnv_q4_rows<E, NT, 2, GATES, STAGED>), grid, block, lds, s, q, a, split, waves, most);
+    else hipLaunchKernelGGL((wnv_q4_rows<E, NT, 4, GATES, STAGED>), grid, block, lds, s, q, a, split, waves, most);
 }
 template <typename E, int GATES> void launch(const Q4Dev& q, const Q4Call& a, hipStream_t s) {
     constexpr int PARTS = Q4Type<E>::PARTS;
-    const int waves = GATES == 0 ? 16 : GATES == 2 ? 8 : 4;     // of one tile: a workgroup is 16 waves at most, 12 with three gates
-    const int split = std::min(waves, q.kb), most = 16 / PARTS;
+    const int slices = GATES == 0 ? 16 : GATES == 2 ? 8 : 4;    // a workgroup is 16 waves at most, 12 with three gates
+    const int split = std::min(slices, q.kb), most = 16 / PARTS;
     const size_t staged = (size_t)PARTS * std::min(a.B, most) * (16 * q.kb + 1) * 16;
-    if (staged <= STAGE_MOST && (PARTS == 3 || (a.B <= 16 && q.kb > split))) return launch<E, 1, GATES, true>(q, a, split, most, staged, s);
+    if (staged <= STAGE_MOST && (PARTS == 3 || (a.B <= 16 && q.kb > split))) return launch<E, 1, GATES, true>(q, a, split, split, most, staged, s);
     if constexpr (!GATES) {
-        if ((int64_t)q.gates * q.tiles * ((a.B + 15) / 16) > CUS) return launch<E, 2, GATES, false>(q, a, split, 16, 0, s);
+        if ((int64_t)q.gates * q.tiles * ((a.B + 15) / 16) > CUS) return launch<E, 2, GATES, false>(q, a, split, std::min(split, 8), 16, 0, s);
     }
-    launch<E, 1, GATES, false>(q, a, split, 16, 0, s);
+    launch<E, 1, GATES, false>(q, a, split, split, 16, 0, s);
 }
 template <typename E> void launch(const Q4Dev& q, const Q4Call& a, hipStream_t s) {
     if (!a.state) launch<E, 0>(q, a, s);
