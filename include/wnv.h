@@ -351,6 +351,7 @@ WNV_API wnv_status wnv_logmel(wnv_mel_handle h, const wnv_logmel_args* args);
  * of a padded batch end at lengths[b]: behind it z is not looked at, y and the gradients are zero and the state is handed on, so
  * h_last is the state behind the last real step (h0 for an empty row).  lengths are taken as min(max(lengths[b], 0), T).
  * The maps live in device memory and are not range-checked further: any value of seg_start other than t just does not begin one.
+ * An infinite input makes the rest of its utterance NaN.
  * No atomics on data: the same call gives the same bits.  Everything a call needs beyond its arguments is in `workspace`, which the
  * call writes before it reads: calls that may run at the same time (other streams, graphs replayed side by side) each have their own. */
 typedef enum wnv_dtype { WNV_F32 = 0, WNV_BF16 = 1, WNV_F16 = 2 } wnv_dtype;

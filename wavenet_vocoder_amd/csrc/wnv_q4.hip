@@ -428,6 +428,7 @@ static wnv_status q4_pack(wnv_q4* h, const uint8_t* codes, const wnv_bf16* scale
                           hipStream_t s) {
     Q4Dev& q = h->q;
     const size_t tiles = (size_t)q.gates * q.tiles, words = tiles * q.kb * 256, gs = tiles * q.kb * q.per_block * 16;
+    HIP_TRY(hipDeviceSynchronize());    // steps under way on other streams still read what is about to be written over
     h->loaded = false;
     HIP_TRY(h->codes.ensure(words * 4));
     HIP_TRY(h->scales.ensure(gs * 2));

@@ -4,7 +4,8 @@
 //   h_t = sigmoid(f_t) h_{t-1} + (1 - sigmoid(f_t)) v_t = h_{t-1} + u_t (v_t - h_{t-1})          y_t = h_t sigmoid(o_t)   (no o: y = h)
 //
 // The second form of h_t is what runs: a gate that remembers long has sigmoid(f) next to 1, where 32 bits leave it 6e-8 off, and a
-// state that sums over 1 / u steps then is 6e-8 / u off; u itself is held to its own precision.
+// state that sums over 1 / u steps then is 6e-8 / u off; u itself is held to its own precision.  (An infinite v leaves v - h without
+// a value a step later: the rest of its utterance is NaN.)
 // h_{t-1} reads as zero at a step that begins an utterance of a packed slot (seg_start[b][t] == t).  Behind lengths[b] the state is
 // handed on, y and the gradients are zero, and z is not looked at.
 #include <hip/hip_runtime.h>
@@ -87,8 +88,8 @@ template <int N, typename F> __device__ __forceinline__ void take_maps(const uns
 // How a chunk learns the state before it, without a chain through all chunks and in one order of arithmetic whatever the timing:
 // 16 chunks are a group, 16 groups a section.  Every chunk hands out its map; the last one of a group joins the 16 and hands out the
 // group's; the last one of a section hands out the state behind it.  A chunk takes the section's state, runs it through the maps
-// of the groups before its own and of the chunks before it in its group: two waits behind its own loads for 256 chunks (32768 steps
-// forward), and one more for each further section.
+// of the groups before its own and of the chunks before it in its group: two waits behind its own loads for 256 chunks (32768 steps),
+// and one more for each further section.
 constexpr int GROUP = 16, COUNTER = 16;      // a row's counter has 128 bytes of its own
 struct Slots {                      // of one row of tiles, one channel
     unsigned long long *chunk, *group, *section;
@@ -134,9 +135,10 @@ __device__ __forceinline__ bool ends_section(int k, int chunks) { return (k + 1)
 // 4 waves of 4 stretches of L steps; a stretch is 16 lanes, a row of the wave, along the channels.  A lane holds V = 4 channels, so
 // that a tile is 64 channels wide: 128 bytes of a 16-bit type, 256 of float32 (8 channels a lane and 4 steps, for rows of 256 bytes
 // of a 16-bit type too, took 213 us for 185 forward and 506 for 316 backward, bf16 8 x 24064 x 512: more maps to join per step).
-// Registers decide how many workgroups share a CU: 3 forward and 2 backward, each with 32 steps x channels a thread.  Half the steps
-// and 3 workgroups backward took 356 us for 316.  The last lane of a tile that ends in no multiple of V
-// starts earlier and shares channels with its neighbour (both compute and write the same); V = 1 is for rows narrower than 4.
+// Registers decide how many workgroups share a CU: 3 forward and 2 backward, each with 32 steps x channels a thread; half the steps
+// and 3 workgroups backward took 356 us for 316.  The last lane of a tile that ends in no multiple of V starts earlier and shares
+// channels with its neighbour (both compute and write the same); V = 1 is for rows narrower than 4.  Rows of up to 16 channels take
+// stretches of 4 lanes, 16 to a wave.
 constexpr int WAVES = 4, THREADS = 64 * WAVES, L = 8;
 template <int LANES> struct Shape {
     static constexpr int ROWS = 64 / LANES, STRETCHES = WAVES * ROWS, WAVE_STEPS = ROWS * L, STEPS = STRETCHES * L;
