@@ -156,25 +156,31 @@ template <typename E, int V> struct Vec {
         return (float)__builtin_bit_cast(wnv_f16, (uint16_t)(w[i / 2] >> (16 * (i & 1))));
     }
 };
-// Data goes past the caches: it is read and written once (bf16 8 x 24064 x 512 forward: 213 us without, 188 with the hint).
+// STREAM: past the caches, for data that no cache holds until its next use anyway (8 x 24064 x 512 forward: float32 271 us and 298
+// without, bf16 166 and 175).  What fits the last-level cache is better left to it (1 x 24064 x 128 float32: 15.7 with, 14.2 without),
+// and rows that are no multiple of 128 bytes have to be: their neighbours share a line, which the cache puts together (16 x 24064 x 100
+// float32 backward: 343 with, 250 without).
 template <int BYTES> struct Raw { typedef uint32_t T __attribute__((ext_vector_type(BYTES / 4), aligned(1))); };
 template <> struct Raw<2> { typedef uint16_t T __attribute__((aligned(1))); };
 template <> struct Raw<4> { typedef uint32_t T __attribute__((aligned(1))); };
-template <typename E, int V> __device__ __forceinline__ Vec<E, V> load(const E* base, uint32_t bytes) {        // at any alignment
+template <typename E, int V, bool STREAM> __device__ __forceinline__ Vec<E, V> load(const E* base, uint32_t bytes) {        // at any alignment
     typedef typename Raw<V * sizeof(E)>::T R;
-    const R r = __builtin_nontemporal_load((const R*)((const char*)base + bytes));
+    const R* p = (const R*)((const char*)base + bytes);
+    const R r = STREAM ? __builtin_nontemporal_load(p) : *p;
     Vec<E, V> v{};
     __builtin_memcpy(v.w, &r, sizeof r);
     return v;
 }
-template <typename E, int V> __device__ __forceinline__ void store(E* base, uint32_t bytes, const float (&x)[V]) {
+template <typename E, int V, bool STREAM> __device__ __forceinline__ void store(E* base, uint32_t bytes, const float (&x)[V]) {
     typedef typename Raw<V * sizeof(E)>::T R;
     E e[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) e[i] = wnv_down<E>(x[i]);
     R r;
     __builtin_memcpy(&r, e, sizeof r);
-    __builtin_nontemporal_store(r, (R*)((char*)base + bytes));
+    R* p = (R*)((char*)base + bytes);
+    if (STREAM) __builtin_nontemporal_store(r, p);
+    else *p = r;
 }
 
 // The maps of a wave's rows joined in time (BACK: the last row first): of all of them, and of those before the own row.
@@ -260,7 +266,7 @@ template <int LANES, bool SEG> __device__ __forceinline__ int begins_in(const En
 // waves 1 and 2 find the state before the group; then each thread knows the state before its stretch and runs over it again, out of
 // its registers.  z is read once.  Chunks that are live to their end (FULL) run without a test at every step: the steps' exponentials
 // and reciprocals then overlap (bf16 8 x 24064 x 512 forward: 185 us with the tests).
-template <typename E, int G, int V, int LANES, bool SEG>
+template <typename E, int G, int V, int LANES, bool SEG, bool STREAM>
 __global__ void __launch_bounds__(THREADS, SEG && sizeof(E) == 2 ? 4 : 3) wnv_recurrence_fwd(RecArgs a) {
     constexpr int W = LANES * V, STEPS = Shape<LANES>::STEPS;
     __shared__ Map totals[WAVES][W], prev[W], groups[W];
@@ -283,9 +289,9 @@ __global__ void __launch_bounds__(THREADS, SEG && sizeof(E) == 2 ? 4 : 3) wnv_re
 #pragma unroll
         for (int l = 0; l < L; ++l)
             if (FULL || l < live) {
-                f[l] = load<E, V>(z + l * a.zt, from);
-                v[l] = load<E, V>(z + l * a.zt + a.C, from);
-                if (G == 3) o[l] = load<E, V>(z + l * a.zt + 2 * a.C, from);
+                f[l] = load<E, V, STREAM>(z + l * a.zt, from);
+                v[l] = load<E, V, STREAM>(z + l * a.zt + a.C, from);
+                if (G == 3) o[l] = load<E, V, STREAM>(z + l * a.zt + 2 * a.C, from);
             }
         begins = begins_in<LANES, SEG>(entries, live);
 #pragma unroll
@@ -361,7 +367,7 @@ __global__ void __launch_bounds__(THREADS, SEG && sizeof(E) == 2 ? 4 : 3) wnv_re
                     }
                     out[i] = q;
                 }
-                store<E, V>(y + (long long)l * a.C, to, out);
+                store<E, V, STREAM>(y + (long long)l * a.C, to, out);
             }
     };
     if (whole) run(std::true_type{});
@@ -372,7 +378,7 @@ __global__ void __launch_bounds__(THREADS, SEG && sizeof(E) == 2 ? 4 : 3) wnv_re
 // df = dh (h_{t-1} - v) sigmoid(f) u;  dv = dh u;  do = dy h sigmoid(o) (1 - sigmoid(o))
 // The chunks run from the last to the first, r is found the way the forward pass finds h; h itself starts from the state that the
 // forward pass saved before each chunk and is run through again.
-template <typename E, int G, int V, int LANES, bool SEG>
+template <typename E, int G, int V, int LANES, bool SEG, bool STREAM>
 __global__ void __launch_bounds__(THREADS, 2) wnv_recurrence_bwd(RecArgs a) {
     constexpr int W = LANES * V, STEPS = Shape<LANES>::STEPS;
     __shared__ Map ahead[WAVES][W], back[WAVES][W], prev[W], groups[W];         // of h and of r
@@ -398,12 +404,12 @@ __global__ void __launch_bounds__(THREADS, 2) wnv_recurrence_bwd(RecArgs a) {
 #pragma unroll
         for (int l = 0; l < L; ++l)
             if (FULL || l < live) {
-                f[l] = load<E, V>(z + l * a.zt, from);
-                v[l] = load<E, V>(z + l * a.zt + a.C, from);
-                if (G == 3) o[l] = load<E, V>(z + l * a.zt + 2 * a.C, from);
-                if (a.dy) d[l] = load<E, V>(dy + l * a.dyt, dfrom);
+                f[l] = load<E, V, STREAM>(z + l * a.zt, from);
+                v[l] = load<E, V, STREAM>(z + l * a.zt + a.C, from);
+                if (G == 3) o[l] = load<E, V, STREAM>(z + l * a.zt + 2 * a.C, from);
+                if (a.dy) d[l] = load<E, V, STREAM>(dy + l * a.dyt, dfrom);
             }
-        saved = load<float, V>(a.saved + ((long long)p.row * a.chunks + p.chunk) * W, at * 4);
+        saved = load<float, V, false>(a.saved + ((long long)p.row * a.chunks + p.chunk) * W, at * 4);
         begins = begins_in<LANES, SEG>(entries, live);
 #pragma unroll
         for (int i = 0; i < V; ++i) m[i] = r[i] = {0.f, 0.f};
@@ -512,9 +518,9 @@ __global__ void __launch_bounds__(THREADS, 2) wnv_recurrence_bwd(RecArgs a) {
                     dg[i] = xo;
                 }
                 E* row = dz + (long long)l * G * a.C;
-                store<E, V>(row, to, df);
-                store<E, V>(row + a.C, to, dv);
-                if (G == 3) store<E, V>(row + 2 * (long long)a.C, to, dg);
+                store<E, V, STREAM>(row, to, df);
+                store<E, V, STREAM>(row + a.C, to, dv);
+                if (G == 3) store<E, V, STREAM>(row + 2 * (long long)a.C, to, dg);
             }
     };
     if (whole) run(std::true_type{});
@@ -610,21 +616,29 @@ wnv_status prepare(const char* who, const wnv_recurrence_args* a, const Cut& c, 
     return WNV_OK;
 }
 
-template <typename E, int G, int V, int LANES> void launch(bool back, const wnv_recurrence_args* a, const RecArgs& k) {
+template <typename E, int G, int V, int LANES, bool STREAM> void launch(bool back, const wnv_recurrence_args* a, const RecArgs& k) {
     const dim3 grid((unsigned)((int64_t)k.B * k.tiles * k.chunks)), block(THREADS);
     hipStream_t s = (hipStream_t)a->stream;
     if (back) {
-        if (a->seg_start) hipLaunchKernelGGL((wnv_recurrence_bwd<E, G, V, LANES, true>), grid, block, 0, s, k);
-        else hipLaunchKernelGGL((wnv_recurrence_bwd<E, G, V, LANES, false>), grid, block, 0, s, k);
+        if (a->seg_start) hipLaunchKernelGGL((wnv_recurrence_bwd<E, G, V, LANES, true, STREAM>), grid, block, 0, s, k);
+        else hipLaunchKernelGGL((wnv_recurrence_bwd<E, G, V, LANES, false, STREAM>), grid, block, 0, s, k);
     } else {
-        if (a->seg_start) hipLaunchKernelGGL((wnv_recurrence_fwd<E, G, V, LANES, true>), grid, block, 0, s, k);
-        else hipLaunchKernelGGL((wnv_recurrence_fwd<E, G, V, LANES, false>), grid, block, 0, s, k);
+        if (a->seg_start) hipLaunchKernelGGL((wnv_recurrence_fwd<E, G, V, LANES, true, STREAM>), grid, block, 0, s, k);
+        else hipLaunchKernelGGL((wnv_recurrence_fwd<E, G, V, LANES, false, STREAM>), grid, block, 0, s, k);
     }
 }
+// Whether data goes past the caches: more than the 256 MB of the last level, in whole lines.
+bool streams(bool back, const wnv_recurrence_args* a) {
+    const int64_t e = wnv_dtype_size(a->dtype), bytes = a->B * a->T * a->C * e * (back ? 2 * a->gates + 1 : a->gates + 1);
+    uint64_t odd = (uint64_t)a->z | (uint64_t)(a->C * e) | (uint64_t)(a->z_time_stride * e) | (uint64_t)(a->z_batch_stride * e);
+    if (back) odd |= (uint64_t)a->dz | (uint64_t)a->dy | (uint64_t)(a->dy_time_stride * e) | (uint64_t)(a->dy_batch_stride * e);
+    else odd |= (uint64_t)a->y;
+    return bytes > (256 << 20) && odd % 128 == 0;
+}
 template <typename E, int G> void launch(bool back, const wnv_recurrence_args* a, const Cut& c, const RecArgs& k) {
-    if (c.lanes == 16) launch<E, G, 4, 16>(back, a, k);
-    else if (c.V == 4) launch<E, G, 4, 4>(back, a, k);
-    else launch<E, G, 1, 4>(back, a, k);
+    if (c.lanes == 16) streams(back, a) ? launch<E, G, 4, 16, true>(back, a, k) : launch<E, G, 4, 16, false>(back, a, k);
+    else if (c.V == 4) launch<E, G, 4, 4, false>(back, a, k);      // rows of less than a line
+    else launch<E, G, 1, 4, false>(back, a, k);
 }
 template <typename E> void launch(bool back, const wnv_recurrence_args* a, const Cut& c, const RecArgs& k) {
     if (a->gates == 3) launch<E, 3>(back, a, c, k);
