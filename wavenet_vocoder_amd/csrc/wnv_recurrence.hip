@@ -139,7 +139,7 @@ __device__ __forceinline__ bool ends_section(int k, int chunks) { return (k + 1)
 // of a 16-bit type too, took 213 us for 185 forward and 506 for 316 backward, bf16 8 x 24064 x 512: more maps to join per step).
 // Registers decide how many workgroups share a CU: 3 forward and 2 backward, each with 32 steps x channels a thread; half the steps
 // and 3 workgroups backward took 356 us for 316.  The last lane of a tile that ends in no multiple of V starts earlier and shares
-// channels with its neighbour (both compute and write the same); V = 1 is for rows narrower than 4.  Rows of up to 16 channels take
+// channels with its neighbour (both compute and write the same); V = 1 is for rows narrower than 4.  Rows of up to NARROW channels take
 // stretches of 4 lanes, 16 to a wave.
 constexpr int WAVES = 4, THREADS = 64 * WAVES, L = 8;
 template <int LANES> struct Shape {
@@ -265,7 +265,7 @@ template <int LANES, bool SEG> __device__ __forceinline__ int begins_in(const En
 // One chunk of one tile.  Each thread reduces its stretch to a map, the wave joins its rows', wave 0 the chunk's and its group's while
 // waves 1 and 2 find the state before the group; then each thread knows the state before its stretch and runs over it again, out of
 // its registers.  z is read once.  Chunks that are live to their end (FULL) run without a test at every step: the steps' exponentials
-// and reciprocals then overlap (bf16 8 x 24064 x 512 forward: 185 us with the tests).
+// and reciprocals then overlap (bf16 8 x 24064 x 512 forward: 164 us, with the tests 185).
 template <typename E, int G, int V, int LANES, bool SEG, bool STREAM>
 __global__ void __launch_bounds__(THREADS, SEG && sizeof(E) == 2 ? 4 : 3) wnv_recurrence_fwd(RecArgs a) {
     constexpr int W = LANES * V, STEPS = Shape<LANES>::STEPS;
@@ -569,9 +569,9 @@ wnv_status launched(const char* who) {
 }
 
 // Up to here a tile is 16 channels (4 with V = 1) and a chunk 512 steps, beyond 64 and 128: where rows are narrow, lanes along the
-// channels are idle, and with them go a quarter of the chunks to wait for (forward and backward of 16 x 24064 float32, us: C = 5 92 and
-// 133 with wide tiles, C = 16 89 and 147; C = 20 219 and 162, for two narrow tiles read a row twice).
-constexpr int NARROW = 16;
+// channels are idle, and with them go a quarter of the chunks to wait for (forward and backward of 16 x 24064, us, narrow tiles and
+// wide ones: float32 C = 20 97 and 121, C = 40 198 and 170; bf16 C = 32 85 and 112, C = 48 134 and 133).
+constexpr int NARROW = 32;
 
 wnv_status check_strides(const char* who, const wnv_recurrence_args* a) {
     if (a->z_batch_stride < 0 || a->z_time_stride < 0 || (a->h0 && a->h0_batch_stride < 0) ||
