@@ -433,3 +433,33 @@ def test_work_under_way_on_another_stream():
             y, h = gated_recurrence(late, h0)
         torch.cuda.current_stream().wait_stream(s)
         assert torch.equal(y, want[0]) and torch.equal(h, want[1])
+
+
+@pytest.mark.parametrize("kind", ["full", "both"])
+@pytest.mark.parametrize("gates,dtype", [(2, "f32"), (3, "bf16")])
+def test_data_larger_than_the_caches(gates, dtype, kind):
+    """Rows of whole lines, more than the last-level cache holds, take another path to memory than the same values an element off:
+    the same bits."""
+    B, T, C, dt = 8, 12100, 512, DTYPES[dtype]
+    g = torch.Generator(device="cuda").manual_seed(79)
+    n = B * T * gates * C
+    z = torch.randn(n + 1, generator=g, device="cuda").to(dt)
+    off = z[1:].view(B, T, gates * C)
+    on = off.clone()
+    dy = torch.randn(B, T, C, generator=g, device="cuda").to(dt)
+    dh = torch.randn(B, C, generator=g, device="cuda")
+    h0 = torch.randn(B, C, generator=g, device="cuda")
+    m = {k: v.cuda() for k, v in maps(kind, B, T, seed=3).items()}
+    outs = []
+    for a in (on, off):
+        a = a.detach().requires_grad_()
+        y, h = gated_recurrence(a, h0, output_gate=gates == 3, **m)
+        outs.append((y, h, *torch.autograd.grad((y, h), a, (dy, dh))))
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+    row = B - 1                         # and one row against the definition
+    k = {n: v[row:row + 1].cpu() for n, v in m.items()}
+    zr, hr = on[row:row + 1].cpu(), h0[row:row + 1].cpu()
+    want = oracle_scan(zr, hr, gates == 3, dy=dy[row:row + 1].cpu(), dh_last=dh[row:row + 1].cpu(), **k)
+    got = dict(y=outs[0][0][row:row + 1], h_last=outs[0][1][row:row + 1], dz=outs[0][2][row:row + 1])
+    check_scan(got, want, zr, hr, gates == 3, k.get("lengths"), dy[row:row + 1], dh[row:row + 1])
