@@ -51,7 +51,8 @@ def run(z, h0, dy, dh, gates, m, grads=True):
 
 
 SHAPES = [(1, 1, 1), (2, 2, 3), (3, 7, 20), (2, 127, 64), (2, 128, 65), (3, 129, 33), (1, 300, 128), (2, 513, 17), (4, 1000, 72),
-          (1, 2500, 8), (2, 1025, 201), (1, 4097, 40), (2, 511, 2), (1, 513, 3), (3, 1500, 4), (2, 9000, 16), (1, 2100, 17)]
+          (1, 2500, 8), (2, 1025, 201), (1, 4097, 40), (2, 511, 2), (1, 513, 3), (3, 1500, 4), (2, 9000, 16), (1, 2100, 17),
+          (2, 300, 130), (1, 512, 67), (12, 400, 700)]
 
 
 @pytest.mark.parametrize("dtype", sorted(DTYPES))
@@ -66,7 +67,7 @@ def test_scan_and_gradients(shape, gates, dtype):
 
 @pytest.mark.parametrize("kind", ["lengths", "packed", "both"])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
-@pytest.mark.parametrize("shape", [(5, 1, 8), (4, 130, 24), (3, 700, 129), (5, 2049, 16)], ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("shape", [(5, 1, 8), (4, 130, 24), (3, 700, 129), (5, 2049, 16), (4, 400, 70)], ids=lambda s: "x".join(map(str, s)))
 def test_padded_batches_and_packed_slots(shape, dtype, kind):
     B, T, C = shape
     z, h0, dy, dh = inputs(B, T, C, 3, DTYPES[dtype], seed=T + 1)
@@ -79,6 +80,17 @@ def test_padded_batches_and_packed_slots(shape, dtype, kind):
         assert not got["y"].cpu()[behind].any() and not got["dz"].cpu()[behind].any()
         empty = m["lengths"] == 0
         assert torch.equal(got["h_last"].cpu()[empty], h0[empty]) and torch.equal(got["dh0"].cpu()[empty], dh[empty])
+
+
+@pytest.mark.parametrize("shape", [(9, 100, 70), (9, 300, 100), (9, 300, 300), (9, 1500, 70), (9, 3000, 20)], ids=lambda s: "x".join(map(str, s)))
+def test_a_rows_bits_do_not_depend_on_its_batch(shape):
+    B, T, C = shape
+    z, h0, dy, dh = inputs(B, T, C, 3, torch.bfloat16, seed=3)
+    all_ = run(z, h0, dy, dh, 3, {})
+    for b in (0, 4, B - 1):
+        one = run(z[b:b + 1], h0[b:b + 1], dy[b:b + 1], dh[b:b + 1], 3, {})
+        for k in all_:
+            assert torch.equal(one[k][0], all_[k][b]), k
 
 
 @pytest.mark.parametrize("T", [40, 1500])

@@ -139,8 +139,8 @@ __device__ __forceinline__ bool ends_section(int k, int chunks) { return (k + 1)
 // of a 16-bit type too, took 213 us for 185 forward and 506 for 316 backward, bf16 8 x 24064 x 512: more maps to join per step).
 // Registers decide how many workgroups share a CU: 3 forward and 2 backward, each with 32 steps x channels a thread; half the steps
 // and 3 workgroups backward took 356 us for 316.  The last lane of a tile that ends in no multiple of V starts earlier and shares
-// channels with its neighbour (both compute and write the same); V = 1 is for rows narrower than 4.  Rows of up to NARROW channels take
-// stretches of 4 lanes, 16 to a wave.
+// channels with its neighbour (both compute and write the same); V = 1 is for rows narrower than 4.  Narrow tiles take stretches of 4
+// lanes, 16 to a wave.
 constexpr int WAVES = 4, THREADS = 64 * WAVES, L = 8;
 template <int LANES> struct Shape {
     static constexpr int ROWS = 64 / LANES, STRETCHES = WAVES * ROWS, WAVE_STEPS = ROWS * L, STEPS = STRETCHES * L;
@@ -568,33 +568,39 @@ wnv_status launched(const char* who) {
     return e == hipSuccess ? WNV_OK : fail(WNV_ERR_HIP, "%s: launch failed: %s", who, hipGetErrorString(e));
 }
 
-// Up to here a tile is 16 channels (4 with V = 1) and a chunk 512 steps, beyond 64 and 128: where rows are narrow, lanes along the
-// channels are idle, and with them go a quarter of the chunks to wait for (forward and backward of 16 x 24064, us, narrow tiles and
-// wide ones: float32 C = 20 97 and 121, C = 40 198 and 170; bf16 C = 32 85 and 112, C = 48 134 and 133).
-constexpr int NARROW = 32;
+// How T x C is cut; B is no part of it, so that the bits of a row do not depend on the batch it runs in.  Tiles are 64 channels and
+// chunks 128 steps, or narrow ones of 16 channels (4 with V = 1) and 512 steps:
+//  * where rows are narrow, lanes along the channels are idle, and with them go a quarter of the chunks to wait for (forward and
+//    backward of 16 x 24064, us, narrow tiles and wide ones: float32 C = 20 97 and 121, C = 40 198 and 170; bf16 C = 32 85 and 112,
+//    C = 48 134 and 133);
+//  * where that makes one chunk of several, which needs neither a filled workspace nor a wait (forward, float32: 2 x 300 x 128 9.3
+//    and 13.7 us a call, 64 x 512 x 256 24.1 and 25.9).  Wider rows are read faster in whole lines (32 x 256 x 1000 float32 forward
+//    35 and 27, forward and backward of 64 x 512 x 512 179 and 134).
+constexpr int WIDE_STEPS = THREADS / 16 * L, NARROW_STEPS = THREADS / 4 * L, NARROW_CHANNELS = 32, NARROW_CHANNELS_ALONE = 256;
+struct Cut { int V, lanes, W, tiles, chunks; };
+Cut cut_of(int64_t T, int C) {
+    Cut c;
+    const bool narrow = C <= NARROW_CHANNELS || (C <= NARROW_CHANNELS_ALONE && T > WIDE_STEPS && T <= NARROW_STEPS);
+    c.V = C < 4 ? 1 : 4;
+    c.lanes = narrow ? 4 : 16;
+    c.W = c.lanes * c.V;
+    c.tiles = (C + c.W - 1) / c.W;
+    const int steps = narrow ? NARROW_STEPS : WIDE_STEPS;
+    c.chunks = (int)((T + steps - 1) / steps);
+    return c;
+}
 
-wnv_status check_strides(const char* who, const wnv_recurrence_args* a) {
+wnv_status check_strides(const char* who, const wnv_recurrence_args* a, const Cut& c) {
     if (a->z_batch_stride < 0 || a->z_time_stride < 0 || (a->h0 && a->h0_batch_stride < 0) ||
         (a->dy && (a->dy_batch_stride < 0 || a->dy_time_stride < 0)))
         return fail(WNV_ERR_INVALID_ARG, "%s: negative stride", who);
     // a lane's offset within a chunk is 32 bits
-    const int64_t most = a->C <= NARROW ? 1 << 20 : 1 << 22;
+    const int64_t most = c.lanes == 4 ? 1 << 20 : 1 << 22;
     if (a->T > 1 && (a->z_time_stride >= most || (a->dy && a->dy_time_stride >= most)))
         return fail(WNV_ERR_UNSUPPORTED, "%s: time strides of %lld elements and more", who, (long long)most);
     return WNV_OK;
 }
 
-struct Cut { int V, lanes, W, tiles, chunks; };
-Cut cut_of(int64_t T, int C) {
-    Cut c;
-    c.V = C < 4 ? 1 : 4;
-    c.lanes = C <= NARROW ? 4 : 16;
-    c.W = c.lanes * c.V;
-    c.tiles = (C + c.W - 1) / c.W;
-    const int steps = THREADS / c.lanes * L;
-    c.chunks = (int)((T + steps - 1) / steps);
-    return c;
-}
 int64_t slot_bytes(int64_t B, const Cut& c) { return c.chunks > 1 ? B * c.tiles * slots_of_row(c.chunks, c.W) * 8 : 0; }
 
 // The kernel's arguments; the workspace is filled on the way.
@@ -661,11 +667,11 @@ extern "C" int64_t wnv_recurrence_workspace_bytes(int32_t B, int64_t T, int32_t 
 extern "C" wnv_status wnv_recurrence_forward(int32_t device, const wnv_recurrence_args* a) {
     if (!a || !a->z || !a->y || !a->h_last) return fail(WNV_ERR_INVALID_ARG, "wnv_recurrence_forward: NULL argument");
     if (wnv_status st = check_shape("wnv_recurrence_forward", device, a->B, a->T, a->C, a->gates, a->dtype)) return st;
-    if (wnv_status st = check_strides("wnv_recurrence_forward", a)) return st;
+    const Cut c = cut_of(a->T, a->C);
+    if (wnv_status st = check_strides("wnv_recurrence_forward", a, c)) return st;
     DeviceGuard guard(device);
     if (!guard.ok) return fail(WNV_ERR_HIP, "wnv_recurrence_forward: cannot select device %d", device);
     RecArgs k{};
-    const Cut c = cut_of(a->T, a->C);
     if (wnv_status st = prepare("wnv_recurrence_forward", a, c, k)) return st;
     WNV_BY_TYPE(a->dtype, launch<E>(false, a, c, k));
     return launched("wnv_recurrence_forward");
@@ -674,11 +680,11 @@ extern "C" wnv_status wnv_recurrence_forward(int32_t device, const wnv_recurrenc
 extern "C" wnv_status wnv_recurrence_backward(int32_t device, const wnv_recurrence_args* a) {
     if (!a || !a->z || !a->saved || !a->dz) return fail(WNV_ERR_INVALID_ARG, "wnv_recurrence_backward: NULL argument");
     if (wnv_status st = check_shape("wnv_recurrence_backward", device, a->B, a->T, a->C, a->gates, a->dtype)) return st;
-    if (wnv_status st = check_strides("wnv_recurrence_backward", a)) return st;
+    const Cut c = cut_of(a->T, a->C);
+    if (wnv_status st = check_strides("wnv_recurrence_backward", a, c)) return st;
     DeviceGuard guard(device);
     if (!guard.ok) return fail(WNV_ERR_HIP, "wnv_recurrence_backward: cannot select device %d", device);
     RecArgs k{};
-    const Cut c = cut_of(a->T, a->C);
     if (wnv_status st = prepare("wnv_recurrence_backward", a, c, k)) return st;
     WNV_BY_TYPE(a->dtype, launch<E>(true, a, c, k));
     return launched("wnv_recurrence_backward");
