@@ -1,6 +1,7 @@
 """ResidualRecurrentGLU: the recurrence, its gradients, its step and the 4-bit products together, as a layer uses them."""
 import copy
 import math
+import pickle
 
 import pytest
 import torch
@@ -149,6 +150,19 @@ def test_four_bit_steps_are_the_rounded_layer(group):
     m.clear_buffer()
     dense = m.incremental_forward(x[:, :, 0].cuda()[:, None], c[:, :, 0].cuda()[:, None], g[:, :, 0].cuda()[:, None])[1]
     assert float((dense[:, 0].double().cpu() - full[1][..., 0] - 1.0).abs().max()) < TOL
+
+
+@pytest.mark.parametrize("how", [copy.deepcopy, lambda m: pickle.loads(pickle.dumps(m))], ids=["deepcopy", "pickle"])
+def test_a_copy_of_a_four_bit_layer_goes_on_by_itself(how):
+    m = layer(13).cuda().eval().quantize_(32)
+    x, c, g = (t.cuda() for t in data(2, 2, 15))
+    at = lambda t: (x[:, :, t][:, None], c[:, :, t][:, None], g[:, :, t][:, None])  # noqa: E731
+    m.incremental_forward(*at(0))
+    n = how(m)
+    n._q4_key = tuple((p.device, p.data_ptr(), p._version) for p in n.parameters())     # as if the copy lay where the original was
+    want = m.incremental_forward(*at(1))
+    got = n.incremental_forward(*at(1))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
 def test_without_conditioning_and_next_to_the_convolution():

@@ -148,7 +148,7 @@ class ResidualRecurrentGLU(nn.Module):
         self.conv1x1_skip = Conv1d1x1(half, skip_out_channels, bias=bias)
         self._state = None
         self._q4_group = None
-        self._q4 = None
+        self._q4_gates = self._q4_heads = None      # apart: in a copy of the module each is None
         self._q4_key = None
 
     # -- batch path: training and scoring ----------------------------------------------------------
@@ -186,7 +186,7 @@ class ResidualRecurrentGLU(nn.Module):
         params = list(self.parameters())
         require_gpu_tensor(params[0], "ResidualRecurrentGLU parameters")
         key = tuple((p.device, p.data_ptr(), p._version) for p in params)
-        if self._q4 is None or self._q4_key != key:
+        if self._q4_gates is None or self._q4_key != key:
             def layer(convs, dim, **kw):
                 w = torch.cat([m.weight.detach().squeeze(-1).float() for m in convs if m is not None], dim)
                 biases = [m.bias.detach().float() for m in convs if m is not None and m.bias is not None]
@@ -194,10 +194,10 @@ class ResidualRecurrentGLU(nn.Module):
                 q.set_weights(w, torch.cat(biases) if biases else None)
                 return q
             # what adds up shares its inputs side by side, what shares an input its outputs
-            self._q4 = (layer((self.conv1x1_in, self.conv1x1c, self.conv1x1g), 1, gates=3),
-                        layer((self.conv1x1_out, self.conv1x1_skip), 0))
+            self._q4_gates = layer((self.conv1x1_in, self.conv1x1c, self.conv1x1g), 1, gates=3)
+            self._q4_heads = layer((self.conv1x1_out, self.conv1x1_skip), 0)
             self._q4_key = key
-        return self._q4
+        return self._q4_gates, self._q4_heads
 
     def incremental_forward(self, x, c=None, g=None):
         """x (B,1,R), c (B,1,cin), g (B,1,gin) -> (x' (B,1,R), s (B,1,K))."""
@@ -234,7 +234,7 @@ class ResidualRecurrentGLU(nn.Module):
 
     def invalidate_engine(self):
         """Drop the packed weights (see WaveNet.invalidate_engine)."""
-        self._q4, self._q4_key = None, None
+        self._q4_gates = self._q4_heads = self._q4_key = None
         for m in (self.conv1x1_in, self.conv1x1_out, self.conv1x1_skip, self.conv1x1c, self.conv1x1g):
             if m is not None:
                 m.invalidate_engine()
