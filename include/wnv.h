@@ -351,7 +351,8 @@ WNV_API wnv_status wnv_logmel(wnv_mel_handle h, const wnv_logmel_args* args);
  * of a padded batch end at lengths[b]: behind it z is not looked at, y and the gradients are zero and the state is handed on, so
  * h_last is the state behind the last real step (h0 for an empty row).  lengths are taken as min(max(lengths[b], 0), T).
  * The maps live in device memory and are not range-checked further: any value of seg_start other than t just does not begin one.
- * An infinite input makes the rest of its utterance NaN.
+ * Infinite gates are their limits (f = inf keeps the state, f = -inf replaces it, o = -inf gives 0); an infinite v makes the rest of
+ * its utterance NaN.
  * No atomics on data: the same call gives the same bits.  Everything a call needs beyond its arguments is in `workspace`, which the
  * call writes before it reads: calls that may run at the same time (other streams, graphs replayed side by side) each have their own. */
 typedef enum wnv_dtype { WNV_F32 = 0, WNV_BF16 = 1, WNV_F16 = 2 } wnv_dtype;
@@ -382,7 +383,7 @@ typedef struct wnv_recurrence_args wnv_recurrence_args;
 WNV_API int64_t wnv_recurrence_saved_bytes(int32_t B, int64_t T, int32_t C, int32_t gates, int32_t dtype);
 WNV_API int64_t wnv_recurrence_workspace_bytes(int32_t B, int64_t T, int32_t C, int32_t gates, int32_t dtype);
 WNV_API wnv_status wnv_recurrence_forward(int32_t device, const wnv_recurrence_args* args);
-/* The same z, h0, lengths and seg_start as the forward call that filled `saved`. */
+/* The same z, lengths and seg_start as the forward call that filled `saved`; h0 is not looked at. */
 WNV_API wnv_status wnv_recurrence_backward(int32_t device, const wnv_recurrence_args* args);
 /* One step: z device (B, gates C) with a row stride, state device (B, C) float32 updated in place, y device (B, C). */
 WNV_API wnv_status wnv_recurrence_step(int32_t device, const void* z, int64_t z_batch_stride, float* state, void* y, int32_t B, int32_t C,

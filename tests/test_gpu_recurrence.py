@@ -143,6 +143,32 @@ def test_gates_at_their_ends(f, T):
     check_scan(run(z, h0, dy, dh, 3, {}), want, z, h0, True, None, dy, dh)
 
 
+@pytest.mark.parametrize("T", [5, 900])
+@pytest.mark.parametrize("gate", ["f", "o"])
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+@pytest.mark.parametrize("sign", [-1.0, 1.0])
+def test_infinite_gates_are_their_limits(sign, dtype, gate, T):
+    """Infinities and the type's ends give the bits of 300, whose sigmoid is 0 or 1 in 32 bits."""
+    z, h0, dy, dh = inputs(2, T, 12, 3, DTYPES[dtype], seed=10)
+    at, c = (slice(0, 12) if gate == "f" else slice(24, 36)), slice(1, T, 2)
+    outs = []
+    for x in (300.0, float("inf"), torch.finfo(DTYPES[dtype]).max):
+        z[:, c, at] = sign * x
+        outs.append(run(z, h0, dy, dh, 3, {}))
+    for k in outs[0]:
+        assert torch.isfinite(outs[0][k]).all() and torch.equal(outs[0][k], outs[1][k]) and torch.equal(outs[0][k], outs[2][k]), k
+
+
+def test_the_state_before_may_be_written_to_before_the_backward_pass():
+    z, h0, dy, dh = inputs(2, 300, 20, 3, torch.float32, seed=12)
+    want = run(z, h0, dy, dh, 3, {})
+    zc, state = z.cuda().requires_grad_(), h0.cuda()
+    y, h = gated_recurrence(zc, state)
+    state.copy_(h.detach())
+    dz, = torch.autograd.grad((y, h), zc, (dy.cuda(), dh.cuda()))
+    assert torch.equal(dz, want["dz"])
+
+
 def test_long_memory_keeps_its_precision():
     """f = 9 remembers 8000 steps: a gate held only as sigmoid(f) in float32 would be 2e-4 off here."""
     T, C = 12000, 8
@@ -403,7 +429,8 @@ def test_refusals_on_the_device():
                      (dict(z=z[..., :0]), ValueError), (dict(z=z.double()), TypeError), (dict(h0=ok[:1]), ValueError),
                      (dict(h0=ok.double()), TypeError), (dict(h0=ok.cpu()), ValueError), (dict(lengths=torch.zeros(3, dtype=i32, device="cuda")), ValueError),
                      (dict(lengths=torch.zeros(2, device="cuda")), TypeError), (dict(lengths=torch.zeros(2, dtype=i32)), ValueError),
-                     (dict(seg_start=torch.zeros(2, 4, dtype=i32, device="cuda")), ValueError)):
+                     (dict(seg_start=torch.zeros(2, 4, dtype=i32, device="cuda")), ValueError),
+                     (dict(z=z[:1].expand(65536, 5, 12)), ValueError), (dict(z=z[:1, :1].expand(1, (1 << 30) + 1, 12)), ValueError)):
         a = dict(z=z)
         a.update(bad)
         with pytest.raises(err):

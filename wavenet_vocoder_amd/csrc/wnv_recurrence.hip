@@ -618,6 +618,7 @@ wnv_status prepare(const char* who, const wnv_recurrence_args* a, const Cut& c, 
         if (!a->workspace) return fail(WNV_ERR_INVALID_ARG, "%s: workspace is NULL", who);
         hipLaunchKernelGGL(wnv_recurrence_fill, dim3((unsigned)((bytes / 16 + 255) / 256)), dim3(256), 0, (hipStream_t)a->stream,
                            (uint4*)a->workspace, (long long)(bytes / 16));
+        return launched(who);       // the chunks draw from what it writes: nothing runs without it
     }
     return WNV_OK;
 }

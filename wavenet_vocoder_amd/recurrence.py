@@ -64,7 +64,10 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 def _sizes(B: int, T: int, n: int, gates: int, code: int) -> Tuple[int, int]:
     """Bytes of (saved, workspace), which go by the shape alone."""
     lib = _lib.lib()
-    return (lib.wnv_recurrence_saved_bytes(B, T, n, gates, code), lib.wnv_recurrence_workspace_bytes(B, T, n, gates, code))
+    saved = lib.wnv_recurrence_saved_bytes(B, T, n, gates, code)
+    if saved < 0:
+        raise ValueError(lib.wnv_last_error().decode())
+    return saved, lib.wnv_recurrence_workspace_bytes(B, T, n, gates, code)
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -97,7 +100,7 @@ def _forward(z, h0, gates, lengths, seg_start, keep: bool):
 
 
 def _backward(ctx, dy, dh_last):
-    z, saved, h0, lengths, seg_start = ctx.saved_tensors
+    z, saved, lengths, seg_start = ctx.saved_tensors
     gates = ctx.gates
     B, T, n = z.shape
     n //= gates
@@ -105,7 +108,7 @@ def _backward(ctx, dy, dh_last):
     needs_z, needs_h0 = ctx.needs_input_grad[:2]
     dz = z.new_empty((B, T, gates * n))
     dh0 = torch.empty(B, n, dtype=torch.float32, device=dev) if needs_h0 else None
-    _call(_lib.lib().wnv_recurrence_backward, z, B, T, n, gates, code, _sizes(B, T, n, gates, code)[1], h0, lengths, seg_start, None, None,
+    _call(_lib.lib().wnv_recurrence_backward, z, B, T, n, gates, code, _sizes(B, T, n, gates, code)[1], None, lengths, seg_start, None, None,
           saved, None if dy is None else _rows(dy), None if dh_last is None else dh_last.contiguous(), dz, dh0)
     return (dz if needs_z else None), dh0, None, None, None
 
@@ -119,7 +122,7 @@ class _GatedRecurrence(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         y, h_last, saved = _forward(z, h0, gates, lengths, seg_start, True)
         ctx.gates = gates
-        ctx.save_for_backward(z, saved, h0, lengths, seg_start)
+        ctx.save_for_backward(z, saved, lengths, seg_start)       # what h0 did is in `saved`: its owner may go on with it
         return y, h_last
 
     @staticmethod
