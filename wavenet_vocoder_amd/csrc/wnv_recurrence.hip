@@ -134,16 +134,16 @@ template <int W, bool SEG> __device__ __forceinline__ Map map_of_groups(const Sl
 __device__ __forceinline__ bool ends_section(int k, int chunks) { return (k + 1) % (GROUP * GROUP) == 0 && k + 1 < chunks; }
 
 // ---- the shape of a workgroup -------------------------------------------------------------------------------------------------
-// 4 waves of 4 stretches of L steps; a stretch is 16 lanes, a row of the wave, along the channels.  A lane holds V = 4 channels, so
+// 4 (or 8) waves of 4 stretches of L steps; a stretch is 16 lanes, a row of the wave, along the channels.  A lane holds V = 4 channels, so
 // that a tile is 64 channels wide: 128 bytes of a 16-bit type, 256 of float32 (8 channels a lane and 4 steps, for rows of 256 bytes
 // of a 16-bit type too, took 213 us for 185 forward and 506 for 316 backward, bf16 8 x 24064 x 512: more maps to join per step).
 // Registers decide how many workgroups share a CU: 3 forward and 2 backward, each with 32 steps x channels a thread; half the steps
 // and 3 workgroups backward took 356 us for 316.  The last lane of a tile that ends in no multiple of V starts earlier and shares
 // channels with its neighbour (both compute and write the same); V = 1 is for rows narrower than 4.  Narrow tiles take stretches of 4
 // lanes, 16 to a wave.
-constexpr int WAVES = 4, THREADS = 64 * WAVES, L = 8;
-template <int LANES> struct Shape {
-    static constexpr int ROWS = 64 / LANES, STRETCHES = WAVES * ROWS, WAVE_STEPS = ROWS * L, STEPS = STRETCHES * L;
+constexpr int L = 8;
+template <int LANES, int WAVES> struct Shape {
+    static constexpr int ROWS = 64 / LANES, WAVE_STEPS = ROWS * L, STEPS = WAVES * WAVE_STEPS;
 };
 
 // V elements as they stand in memory, packed in as few registers; addresses are a uniform base and 32 bits of a lane's own.
@@ -237,14 +237,14 @@ template <bool BACK> __device__ __forceinline__ Place draw_place(const RecArgs& 
 // The number of a row's live steps.
 __device__ __forceinline__ int live_to(const RecArgs& a, int b) { return a.lengths ? max(0, min(a.lengths[b], a.T)) : a.T; }
 // The wave's entries of the map in one or two loads (asked for ahead of the data), a lane each; a stretch takes its 8 bits of a ballot.
-template <int LANES> struct Entries { int e[(Shape<LANES>::WAVE_STEPS + 63) / 64]; };
-template <int LANES, bool SEG> __device__ __forceinline__ Entries<LANES> map_entries(const RecArgs& a, int b, int chunk) {
-    constexpr int N = Shape<LANES>::WAVE_STEPS;
+template <int LANES> struct Entries { int e[(64 / LANES * L + 63) / 64]; };
+template <int LANES, bool SEG> __device__ __forceinline__ Entries<LANES> map_entries(const RecArgs& a, int b, int from) {
+    constexpr int N = 64 / LANES * L;
     Entries<LANES> r{};
     if (SEG) {
 #pragma unroll
         for (int i = 0; i < (N + 63) / 64; ++i) {
-            const int at = 64 * i + threadIdx.x % 64, t = chunk * Shape<LANES>::STEPS + threadIdx.x / 64 * N + at;
+            const int at = 64 * i + threadIdx.x % 64, t = from + threadIdx.x / 64 * N + at;
             r.e[i] = at < N && t < a.T ? a.seg_start[(long long)b * a.T + t] - t : 1;
         }
     }
@@ -255,7 +255,7 @@ template <int LANES, bool SEG> __device__ __forceinline__ int begins_in(const En
     if (!SEG) return 0;
     const int row = threadIdx.x % 64 / LANES;
     unsigned long long bits = __ballot(entries.e[0] == 0);
-    if constexpr (Shape<LANES>::WAVE_STEPS > 64) {
+    if constexpr (64 / LANES * L > 64) {
         const unsigned long long more = __ballot(entries.e[1] == 0);
         if (row >= 8) bits = more;
     }
@@ -266,9 +266,9 @@ template <int LANES, bool SEG> __device__ __forceinline__ int begins_in(const En
 // waves 1 and 2 find the state before the group; then each thread knows the state before its stretch and runs over it again, out of
 // its registers.  z is read once.  Chunks that are live to their end (FULL) run without a test at every step: the steps' exponentials
 // and reciprocals then overlap (bf16 8 x 24064 x 512 forward: 164 us, with the tests 185).
-template <typename E, int G, int V, int LANES, bool SEG, bool STREAM>
-__global__ void __launch_bounds__(THREADS, SEG && sizeof(E) == 2 ? 4 : 3) wnv_recurrence_fwd(RecArgs a) {
-    constexpr int W = LANES * V, STEPS = Shape<LANES>::STEPS;
+template <typename E, int G, int V, int LANES, int WAVES, bool SEG, bool STREAM>
+__global__ void __launch_bounds__(64 * WAVES, WAVES > 4 ? 2 : SEG && sizeof(E) == 2 ? 4 : 3) wnv_recurrence_fwd(RecArgs a) {
+    constexpr int W = LANES * V, STEPS = Shape<LANES, WAVES>::STEPS;
     __shared__ Map totals[WAVES][W], prev[W], groups[W];
     __shared__ float base[W];
     const int tid = threadIdx.x, lane = tid % LANES, wave = tid / 64, at = lane * V;
@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(THREADS, SEG && sizeof(E) == 2 ? 4 : 3) wnv_re
     const int c = min(p.tile * W + at, a.C - V), n = live_to(a, p.b);
     const int t0 = p.chunk * STEPS + tid / LANES * L, live = max(0, min(L, n - t0));
     const bool whole = p.chunk * STEPS + STEPS <= n;
-    const Entries<LANES> entries = map_entries<LANES, SEG>(a, p.b, p.chunk);
+    const Entries<LANES> entries = map_entries<LANES, SEG>(a, p.b, p.chunk * STEPS);
     const E* z = (const E*)a.z + (long long)p.b * a.zb + (long long)p.chunk * STEPS * a.zt;
     const uint32_t from = (uint32_t)(tid / LANES * L * a.zt + c) * (uint32_t)sizeof(E);
 
@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(THREADS, SEG && sizeof(E) == 2 ? 4 : 3) wnv_re
         if (a.saved && tid < LANES) a.saved[((long long)p.row * a.chunks + p.chunk) * W + at + i] = h[i];
         for (int w = 0; w < wave; ++w) h[i] = apply<SEG>(totals[w][at + i], h[i]);
         h[i] = apply<SEG>(before[i], h[i]);
-        if (tid >= THREADS - LANES) {                   // the chunk's last stretch: the state behind it
+        if (tid >= 64 * WAVES - LANES) {                   // the chunk's last stretch: the state behind it
             const float last = apply<SEG>(m[i], h[i]);
             if (ends_section(p.chunk, a.chunks))
                 publish(slots_at(a.slots, p.row, a.chunks, W, at + i).section + (long long)(p.chunk / (GROUP * GROUP)) * W, {-1.f, last});
@@ -378,9 +378,9 @@ __global__ void __launch_bounds__(THREADS, SEG && sizeof(E) == 2 ? 4 : 3) wnv_re
 // df = dh (h_{t-1} - v) sigmoid(f) u;  dv = dh u;  do = dy h sigmoid(o) (1 - sigmoid(o))
 // The chunks run from the last to the first, r is found the way the forward pass finds h; h itself starts from the state that the
 // forward pass saved before each chunk and is run through again.
-template <typename E, int G, int V, int LANES, bool SEG, bool STREAM>
-__global__ void __launch_bounds__(THREADS, 2) wnv_recurrence_bwd(RecArgs a) {
-    constexpr int W = LANES * V, STEPS = Shape<LANES>::STEPS;
+template <typename E, int G, int V, int LANES, int WAVES, bool SEG, bool STREAM>
+__global__ void __launch_bounds__(64 * WAVES, 2) wnv_recurrence_bwd(RecArgs a) {
+    constexpr int W = LANES * V, STEPS = Shape<LANES, WAVES>::STEPS;
     __shared__ Map ahead[WAVES][W], back[WAVES][W], prev[W], groups[W];         // of h and of r
     __shared__ float base[W];
     const int tid = threadIdx.x, lane = tid % LANES, wave = tid / 64, at = lane * V;
@@ -388,7 +388,7 @@ __global__ void __launch_bounds__(THREADS, 2) wnv_recurrence_bwd(RecArgs a) {
     const int order = a.chunks - 1 - p.chunk, c = min(p.tile * W + at, a.C - V), n = live_to(a, p.b);
     const int t0 = p.chunk * STEPS + tid / LANES * L, live = max(0, min(L, n - t0));
     const bool whole = p.chunk * STEPS + STEPS <= n;
-    const Entries<LANES> entries = map_entries<LANES, SEG>(a, p.b, p.chunk);
+    const Entries<LANES> entries = map_entries<LANES, SEG>(a, p.b, p.chunk * STEPS);
     const E* z = (const E*)a.z + (long long)p.b * a.zb + (long long)p.chunk * STEPS * a.zt;
     const E* dy = (const E*)a.dy + (long long)p.b * a.dyb + (long long)p.chunk * STEPS * a.dyt;
     const uint32_t from = (uint32_t)(tid / LANES * L * a.zt + c) * (uint32_t)sizeof(E);
@@ -576,16 +576,25 @@ wnv_status launched(const char* who) {
 //  * where that makes one chunk of several, which needs neither a filled workspace nor a wait (forward, float32: 2 x 300 x 128 9.3
 //    and 13.7 us a call, 64 x 512 x 256 24.1 and 25.9).  Wider rows are read faster in whole lines (32 x 256 x 1000 float32 forward
 //    35 and 27, forward and backward of 64 x 512 x 512 179 and 134).
-constexpr int WIDE_STEPS = THREADS / 16 * L, NARROW_STEPS = THREADS / 4 * L, NARROW_CHANNELS = 32, NARROW_CHANNELS_ALONE = 256;
-struct Cut { int V, lanes, W, tiles, chunks; };
+// And two chunks become one of 8 waves: the host's time falls by a launch and an allocation (float32, forward and both passes, a call:
+// 2 x 200 x 512 9.3 and 90 us, as two chunks 12.3 and 103; 2 x 700 x 128 9.6 and 91, 12.9 and 103), the GPU's rises where there is much
+// data (64 x 700 x 128 both passes 66, of chunks of 128 steps 58).
+constexpr int NARROW_CHANNELS = 32, NARROW_CHANNELS_ALONE = 256;
+struct Cut { int V, lanes, waves, W, tiles, chunks; };
 Cut cut_of(int64_t T, int C) {
+    constexpr int WIDE = Shape<16, 4>::STEPS, NARROW = Shape<4, 4>::STEPS;
     Cut c;
-    const bool narrow = C <= NARROW_CHANNELS || (C <= NARROW_CHANNELS_ALONE && T > WIDE_STEPS && T <= NARROW_STEPS);
+    const bool narrow = C <= NARROW_CHANNELS || (C <= NARROW_CHANNELS_ALONE && T > WIDE && T <= 2 * NARROW);
+    int steps = narrow ? NARROW : WIDE;
+    c.waves = 4;
+    if (T > steps && T <= 2 * steps) {
+        c.waves = 8;
+        steps *= 2;
+    }
     c.V = C < 4 ? 1 : 4;
     c.lanes = narrow ? 4 : 16;
     c.W = c.lanes * c.V;
     c.tiles = (C + c.W - 1) / c.W;
-    const int steps = narrow ? NARROW_STEPS : WIDE_STEPS;
     c.chunks = (int)((T + steps - 1) / steps);
     return c;
 }
@@ -594,7 +603,7 @@ wnv_status check_strides(const char* who, const wnv_recurrence_args* a, const Cu
     if (a->z_batch_stride < 0 || a->z_time_stride < 0 || (a->h0 && a->h0_batch_stride < 0) ||
         (a->dy && (a->dy_batch_stride < 0 || a->dy_time_stride < 0)))
         return fail(WNV_ERR_INVALID_ARG, "%s: negative stride", who);
-    // a lane's offset within a chunk is 32 bits
+    // a lane's offset within a chunk is 32 bits: of 1016 steps at most in narrow tiles, 248 in others, of 4 bytes an element
     const int64_t most = c.lanes == 4 ? 1 << 20 : 1 << 22;
     if (a->T > 1 && (a->z_time_stride >= most || (a->dy && a->dy_time_stride >= most)))
         return fail(WNV_ERR_UNSUPPORTED, "%s: time strides of %lld elements and more", who, (long long)most);
@@ -623,15 +632,15 @@ wnv_status prepare(const char* who, const wnv_recurrence_args* a, const Cut& c, 
     return WNV_OK;
 }
 
-template <typename E, int G, int V, int LANES, bool STREAM> void launch(bool back, const wnv_recurrence_args* a, const RecArgs& k) {
-    const dim3 grid((unsigned)((int64_t)k.B * k.tiles * k.chunks)), block(THREADS);
+template <typename E, int G, int V, int LANES, int WAVES, bool STREAM> void launch(bool back, const wnv_recurrence_args* a, const RecArgs& k) {
+    const dim3 grid((unsigned)((int64_t)k.B * k.tiles * k.chunks)), block(64 * WAVES);
     hipStream_t s = (hipStream_t)a->stream;
     if (back) {
-        if (a->seg_start) hipLaunchKernelGGL((wnv_recurrence_bwd<E, G, V, LANES, true, STREAM>), grid, block, 0, s, k);
-        else hipLaunchKernelGGL((wnv_recurrence_bwd<E, G, V, LANES, false, STREAM>), grid, block, 0, s, k);
+        if (a->seg_start) hipLaunchKernelGGL((wnv_recurrence_bwd<E, G, V, LANES, WAVES, true, STREAM>), grid, block, 0, s, k);
+        else hipLaunchKernelGGL((wnv_recurrence_bwd<E, G, V, LANES, WAVES, false, STREAM>), grid, block, 0, s, k);
     } else {
-        if (a->seg_start) hipLaunchKernelGGL((wnv_recurrence_fwd<E, G, V, LANES, true, STREAM>), grid, block, 0, s, k);
-        else hipLaunchKernelGGL((wnv_recurrence_fwd<E, G, V, LANES, false, STREAM>), grid, block, 0, s, k);
+        if (a->seg_start) hipLaunchKernelGGL((wnv_recurrence_fwd<E, G, V, LANES, WAVES, true, STREAM>), grid, block, 0, s, k);
+        else hipLaunchKernelGGL((wnv_recurrence_fwd<E, G, V, LANES, WAVES, false, STREAM>), grid, block, 0, s, k);
     }
 }
 // Whether data goes past the caches: more than the 256 MB of the last level, in whole lines.
@@ -643,9 +652,15 @@ bool streams(bool back, const wnv_recurrence_args* a) {
     return bytes > (256 << 20) && odd % 128 == 0;
 }
 template <typename E, int G> void launch(bool back, const wnv_recurrence_args* a, const Cut& c, const RecArgs& k) {
-    if (c.lanes == 16) streams(back, a) ? launch<E, G, 4, 16, true>(back, a, k) : launch<E, G, 4, 16, false>(back, a, k);
-    else if (c.V == 4) launch<E, G, 4, 4, false>(back, a, k);      // rows of less than a line
-    else launch<E, G, 1, 4, false>(back, a, k);
+    if (c.lanes == 16) {
+        if (c.waves == 8) launch<E, G, 4, 16, 8, false>(back, a, k);
+        else if (streams(back, a)) launch<E, G, 4, 16, 4, true>(back, a, k);
+        else launch<E, G, 4, 16, 4, false>(back, a, k);
+    } else if (c.V == 4) {              // rows of less than a line
+        c.waves == 8 ? launch<E, G, 4, 4, 8, false>(back, a, k) : launch<E, G, 4, 4, 4, false>(back, a, k);
+    } else {
+        c.waves == 8 ? launch<E, G, 1, 4, 8, false>(back, a, k) : launch<E, G, 1, 4, 4, false>(back, a, k);
+    }
 }
 template <typename E> void launch(bool back, const wnv_recurrence_args* a, const Cut& c, const RecArgs& k) {
     if (a->gates == 3) launch<E, 3>(back, a, c, k);
