@@ -27,7 +27,7 @@ struct RecArgs {
     void* y;
     float* h_last;
     float* saved;                   // [row][chunk][tile width]: the state before the chunk's first step
-    unsigned long long* slots;      // workspace: of each row a counter, then its maps
+    unsigned long long* slots;      // workspace: of each row of tiles a counter, then its maps
     const void* dy;
     long long dyb, dyt;
     const float* dh_last;
@@ -213,25 +213,27 @@ template <int LANES, bool BACK, bool SEG> __device__ __forceinline__ void join_r
 
 struct Place { int b, tile, chunk, row; };
 
-// Chunks are drawn from a counter, one for all tiles of a batch row, all tiles' first chunks first: the order that the waits rely on.
-// Workgroup i runs on XCD i % 8, so that for a batch of 8 a row's maps stay within one L2, which also reads whole rows of z: a
-// counter for each tile instead keeps an XCD to one column of tiles and to few of its L2's channels (float32 8 x 24064 x 512
-// backward: 562 us against 491), and one for all workgroups is drawn from by 700 at once (bf16 8 x 7680 x 128 forward: 28 against 18).
-template <bool BACK> __device__ __forceinline__ Place draw_place(const RecArgs& a, int W) {
+// Each row's tile has a counter from which its chunks are drawn, the order that the waits rely on.  (One for all tiles of a batch row is
+// drawn from by too many at once: forward of 1 x 24064 x 512 bf16 42 us for 31, 1 x 24064 x 128 float32 19.5 for 17.9.)
+// Workgroup i runs on XCD i % 8.  Units of one chunk in all tiles are dealt to the XCDs, so that the tiles' shares of a line meet in one
+// L2 (tiles dealt by themselves: 5 x 3001 x 201 float32 forward 20.1 us for 18, 3 x 16749 x 113 bf16 25 for 22.5); within an XCD the
+// tiles take turns, or each would stay on the same CUs and memory channels (float32 8 x 24064 x 512 both passes: 772 us for 758).
+// False for the workgroups that fill up the last units.
+template <bool BACK> __device__ __forceinline__ bool draw_place(const RecArgs& a, int W, Place& p) {
     __shared__ int drawn;
-    Place p;
-    p.b = blockIdx.x % a.B;
-    int i = blockIdx.x / a.B;
-    if (a.chunks > 1) {
-        if (threadIdx.x == 0) drawn = atomicAdd((int*)(a.slots + (long long)p.b * a.tiles * slots_of_row(a.chunks, W)), 1) + 1;     // it starts at -1
-        __syncthreads();
-        i = __builtin_amdgcn_readfirstlane(drawn);
-    }
-    p.tile = i % a.tiles;
-    p.chunk = i / a.tiles;
-    if (BACK) p.chunk = a.chunks - 1 - p.chunk;
+    const int i = blockIdx.x / 8, round = i / a.tiles, unit = round * 8 + blockIdx.x % 8;
+    if (unit >= a.B * a.chunks) return false;
+    p.b = unit % a.B;
+    p.tile = (i + round) % a.tiles;
     p.row = p.b * a.tiles + p.tile;
-    return p;
+    p.chunk = 0;
+    if (a.chunks > 1) {
+        if (threadIdx.x == 0) drawn = atomicAdd((int*)(a.slots + p.row * slots_of_row(a.chunks, W)), 1) + 1;     // it starts at -1
+        __syncthreads();
+        p.chunk = __builtin_amdgcn_readfirstlane(drawn);
+    }
+    if (BACK) p.chunk = a.chunks - 1 - p.chunk;
+    return true;
 }
 
 // The number of a row's live steps.
@@ -272,7 +274,8 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES > 4 ? 2 : SEG && sizeof(E) =
     __shared__ Map totals[WAVES][W], prev[W], groups[W];
     __shared__ float base[W];
     const int tid = threadIdx.x, lane = tid % LANES, wave = tid / 64, at = lane * V;
-    const Place p = draw_place<false>(a, W);
+    Place p;
+    if (!draw_place<false>(a, W, p)) return;
     const int c = min(p.tile * W + at, a.C - V), n = live_to(a, p.b);
     const int t0 = p.chunk * STEPS + tid / LANES * L, live = max(0, min(L, n - t0));
     const bool whole = p.chunk * STEPS + STEPS <= n;
@@ -384,7 +387,8 @@ __global__ void __launch_bounds__(64 * WAVES, 2) wnv_recurrence_bwd(RecArgs a) {
     __shared__ Map ahead[WAVES][W], back[WAVES][W], prev[W], groups[W];         // of h and of r
     __shared__ float base[W];
     const int tid = threadIdx.x, lane = tid % LANES, wave = tid / 64, at = lane * V;
-    const Place p = draw_place<true>(a, W);
+    Place p;
+    if (!draw_place<true>(a, W, p)) return;
     const int order = a.chunks - 1 - p.chunk, c = min(p.tile * W + at, a.C - V), n = live_to(a, p.b);
     const int t0 = p.chunk * STEPS + tid / LANES * L, live = max(0, min(L, n - t0));
     const bool whole = p.chunk * STEPS + STEPS <= n;
@@ -621,8 +625,8 @@ wnv_status prepare(const char* who, const wnv_recurrence_args* a, const Cut& c, 
     k.y = a->y; k.h_last = a->h_last; k.saved = (float*)a->saved; k.slots = (unsigned long long*)a->workspace;
     k.dy = a->dy; k.dyb = a->dy_batch_stride; k.dyt = a->T > 1 ? a->dy_time_stride : 0;
     k.dh_last = a->dh_last; k.dz = a->dz; k.dh0 = a->dh0;
-    const int64_t blocks = (int64_t)k.B * k.tiles * k.chunks, bytes = slot_bytes(a->B, c);
-    if (blocks >= (1 << 24)) return fail(WNV_ERR_UNSUPPORTED, "%s: B x T x C is too large", who);
+    const int64_t threads = ((int64_t)k.B * k.chunks + 7) * k.tiles * c.waves * 64, bytes = slot_bytes(a->B, c);
+    if (threads > UINT32_MAX) return fail(WNV_ERR_UNSUPPORTED, "%s: B x T x C is too large", who);
     if (bytes) {
         if (!a->workspace) return fail(WNV_ERR_INVALID_ARG, "%s: workspace is NULL", who);
         hipLaunchKernelGGL(wnv_recurrence_fill, dim3((unsigned)((bytes / 16 + 255) / 256)), dim3(256), 0, (hipStream_t)a->stream,
@@ -633,7 +637,7 @@ wnv_status prepare(const char* who, const wnv_recurrence_args* a, const Cut& c, 
 }
 
 template <typename E, int G, int V, int LANES, int WAVES, bool STREAM> void launch(bool back, const wnv_recurrence_args* a, const RecArgs& k) {
-    const dim3 grid((unsigned)((int64_t)k.B * k.tiles * k.chunks)), block(64 * WAVES);
+    const dim3 grid((unsigned)(((int64_t)k.B * k.chunks + 7) / 8 * 8 * k.tiles)), block(64 * WAVES);
     hipStream_t s = (hipStream_t)a->stream;
     if (back) {
         if (a->seg_start) hipLaunchKernelGGL((wnv_recurrence_bwd<E, G, V, LANES, WAVES, true, STREAM>), grid, block, 0, s, k);
