@@ -53,7 +53,7 @@ def run(z, h0, dy, dh, gates, m, grads=True):
 SHAPES = [(1, 1, 1), (2, 2, 3), (3, 7, 20), (2, 127, 64), (2, 128, 65), (3, 129, 33), (1, 300, 128), (2, 513, 17), (4, 1000, 72),
           (1, 2500, 8), (2, 1025, 201), (1, 4097, 40), (2, 511, 2), (1, 513, 3), (3, 1500, 4), (2, 9000, 16), (1, 2100, 17),
           (2, 300, 130), (1, 512, 67), (12, 400, 700), (2, 200, 300), (1, 256, 500), (2, 257, 300), (3, 1024, 33), (2, 1024, 2), (2, 1025, 256),
-          (12, 1000, 130)]
+          (12, 1000, 130), (40, 1000, 70), (3, 500, 1300), (80, 1000, 30), (2, 513, 600)]
 
 
 @pytest.mark.parametrize("dtype", sorted(DTYPES))
@@ -83,8 +83,9 @@ def test_padded_batches_and_packed_slots(shape, dtype, kind):
         assert torch.equal(got["h_last"].cpu()[empty], h0[empty]) and torch.equal(got["dh0"].cpu()[empty], dh[empty])
 
 
-@pytest.mark.parametrize("shape", [(9, 100, 70), (9, 200, 300), (9, 300, 100), (9, 300, 300), (9, 800, 100), (9, 1500, 70), (9, 3000, 20)], ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("shape", [(9, 100, 70), (9, 1500, 70), (9, 3000, 20), (90, 1025, 80)], ids=lambda s: "x".join(map(str, s)))
 def test_a_rows_bits_do_not_depend_on_its_batch(shape):
+    """Neither within short sequences (128 steps) nor within long ones (more than 1024); between them the cut goes by the amount of data."""
     B, T, C = shape
     z, h0, dy, dh = inputs(B, T, C, 3, torch.bfloat16, seed=3)
     all_ = run(z, h0, dy, dh, 3, {})

@@ -572,31 +572,29 @@ wnv_status launched(const char* who) {
     return e == hipSuccess ? WNV_OK : fail(WNV_ERR_HIP, "%s: launch failed: %s", who, hipGetErrorString(e));
 }
 
-// How T x C is cut; B is no part of it, so that the bits of a row do not depend on the batch it runs in.  Tiles are 64 channels and
-// chunks 128 steps, or narrow ones of 16 channels (4 with V = 1) and 512 steps:
+// How B x T x C is cut.  Tiles are 64 channels and chunks 128 steps, or narrow ones of 16 channels (4 with V = 1) and 512 steps:
 //  * where rows are narrow, lanes along the channels are idle, and with them go a quarter of the chunks to wait for (forward and
 //    backward of 16 x 24064, us, narrow tiles and wide ones: float32 C = 20 97 and 121, C = 40 198 and 170; bf16 C = 32 85 and 112,
 //    C = 48 134 and 133);
-//  * where that makes one chunk of several, which needs neither a filled workspace nor a wait (forward, float32: 2 x 300 x 128 9.3
-//    and 13.7 us a call, 64 x 512 x 256 24.1 and 25.9).  Wider rows are read faster in whole lines (32 x 256 x 1000 float32 forward
-//    35 and 27, forward and backward of 64 x 512 x 512 179 and 134).
-// And two chunks become one of 8 waves: the host's time falls by a launch and an allocation (float32, forward and both passes, a call:
-// 2 x 200 x 512 9.3 and 90 us, as two chunks 12.3 and 103; 2 x 700 x 128 9.6 and 91, 12.9 and 103), the GPU's rises where there is much
-// data (64 x 700 x 128 both passes 66, of chunks of 128 steps 58).
-constexpr int NARROW_CHANNELS = 32, NARROW_CHANNELS_ALONE = 256;
+//  * where there is little data and that makes one chunk of several, which needs neither a filled workspace nor a wait: the host's
+//    time falls by a launch and an allocation (2 x 300 x 128 float32 forward 9.3 us a call and 13.7, 2 x 400 x 512 9.4 and 12.7).
+// Of narrow tiles two chunks become one of 8 waves, for the same reason (2 x 700 x 128 float32 forward 9.6 us a call and 12.9, both
+// passes 91 and 103).
+// More data is the GPU's time, and is read faster in whole lines by more workgroups (64 x 700 x 128 float32 forward 26 us in narrow
+// tiles of 8 waves and 21 in wide ones, both passes 66 and 58; 64 x 512 x 512 both passes 179 and 134).
+constexpr int NARROW_CHANNELS = 32, LITTLE_CHANNELS = 256;
+constexpr int64_t LITTLE = 2 << 20;
 struct Cut { int V, lanes, waves, W, tiles, chunks; };
-Cut cut_of(int64_t T, int C) {
+Cut cut_of(int64_t B, int64_t T, int C) {
     constexpr int WIDE = Shape<16, 4>::STEPS, NARROW = Shape<4, 4>::STEPS;
     Cut c;
-    const bool narrow = C <= NARROW_CHANNELS || (C <= NARROW_CHANNELS_ALONE && T > WIDE && T <= 2 * NARROW);
-    int steps = narrow ? NARROW : WIDE;
-    c.waves = 4;
-    if (T > steps && T <= 2 * steps) {
-        c.waves = 8;
-        steps *= 2;
-    }
+    const bool little = B * T * C <= LITTLE;
+    const bool narrow = C <= NARROW_CHANNELS || (little && T > WIDE && T <= (C <= LITTLE_CHANNELS ? 2 * NARROW : NARROW));
+    const bool joined = narrow && little && T > NARROW && T <= 2 * NARROW;
+    const int steps = joined ? 2 * NARROW : narrow ? NARROW : WIDE;
     c.V = C < 4 ? 1 : 4;
     c.lanes = narrow ? 4 : 16;
+    c.waves = joined ? 8 : 4;
     c.W = c.lanes * c.V;
     c.tiles = (C + c.W - 1) / c.W;
     c.chunks = (int)((T + steps - 1) / steps);
@@ -607,7 +605,7 @@ wnv_status check_strides(const char* who, const wnv_recurrence_args* a, const Cu
     if (a->z_batch_stride < 0 || a->z_time_stride < 0 || (a->h0 && a->h0_batch_stride < 0) ||
         (a->dy && (a->dy_batch_stride < 0 || a->dy_time_stride < 0)))
         return fail(WNV_ERR_INVALID_ARG, "%s: negative stride", who);
-    // a lane's offset within a chunk is 32 bits: of 1016 steps at most in narrow tiles, 248 in others, of 4 bytes an element
+    // a lane's offset within a chunk is 32 bits: of 1016 steps at most in narrow tiles, 120 in others, of 4 bytes an element
     const int64_t most = c.lanes == 4 ? 1 << 20 : 1 << 22;
     if (a->T > 1 && (a->z_time_stride >= most || (a->dy && a->dy_time_stride >= most)))
         return fail(WNV_ERR_UNSUPPORTED, "%s: time strides of %lld elements and more", who, (long long)most);
@@ -657,9 +655,7 @@ bool streams(bool back, const wnv_recurrence_args* a) {
 }
 template <typename E, int G> void launch(bool back, const wnv_recurrence_args* a, const Cut& c, const RecArgs& k) {
     if (c.lanes == 16) {
-        if (c.waves == 8) launch<E, G, 4, 16, 8, false>(back, a, k);
-        else if (streams(back, a)) launch<E, G, 4, 16, 4, true>(back, a, k);
-        else launch<E, G, 4, 16, 4, false>(back, a, k);
+        streams(back, a) ? launch<E, G, 4, 16, 4, true>(back, a, k) : launch<E, G, 4, 16, 4, false>(back, a, k);
     } else if (c.V == 4) {              // rows of less than a line
         c.waves == 8 ? launch<E, G, 4, 4, 8, false>(back, a, k) : launch<E, G, 4, 4, 4, false>(back, a, k);
     } else {
@@ -675,19 +671,19 @@ template <typename E> void launch(bool back, const wnv_recurrence_args* a, const
 
 extern "C" int64_t wnv_recurrence_saved_bytes(int32_t B, int64_t T, int32_t C, int32_t gates, int32_t dtype) {
     if (check_shape("wnv_recurrence_saved_bytes", 0, B, T, C, gates, dtype) != WNV_OK) return -1;
-    const Cut c = cut_of(T, C);
+    const Cut c = cut_of(B, T, C);
     return (int64_t)B * c.tiles * c.chunks * c.W * 4;
 }
 
 extern "C" int64_t wnv_recurrence_workspace_bytes(int32_t B, int64_t T, int32_t C, int32_t gates, int32_t dtype) {
     if (check_shape("wnv_recurrence_workspace_bytes", 0, B, T, C, gates, dtype) != WNV_OK) return -1;
-    return slot_bytes(B, cut_of(T, C));
+    return slot_bytes(B, cut_of(B, T, C));
 }
 
 extern "C" wnv_status wnv_recurrence_forward(int32_t device, const wnv_recurrence_args* a) {
     if (!a || !a->z || !a->y || !a->h_last) return fail(WNV_ERR_INVALID_ARG, "wnv_recurrence_forward: NULL argument");
     if (wnv_status st = check_shape("wnv_recurrence_forward", device, a->B, a->T, a->C, a->gates, a->dtype)) return st;
-    const Cut c = cut_of(a->T, a->C);
+    const Cut c = cut_of(a->B, a->T, a->C);
     if (wnv_status st = check_strides("wnv_recurrence_forward", a, c)) return st;
     DeviceGuard guard(device);
     if (!guard.ok) return fail(WNV_ERR_HIP, "wnv_recurrence_forward: cannot select device %d", device);
@@ -700,7 +696,7 @@ extern "C" wnv_status wnv_recurrence_forward(int32_t device, const wnv_recurrenc
 extern "C" wnv_status wnv_recurrence_backward(int32_t device, const wnv_recurrence_args* a) {
     if (!a || !a->z || !a->saved || !a->dz) return fail(WNV_ERR_INVALID_ARG, "wnv_recurrence_backward: NULL argument");
     if (wnv_status st = check_shape("wnv_recurrence_backward", device, a->B, a->T, a->C, a->gates, a->dtype)) return st;
-    const Cut c = cut_of(a->T, a->C);
+    const Cut c = cut_of(a->B, a->T, a->C);
     if (wnv_status st = check_strides("wnv_recurrence_backward", a, c)) return st;
     DeviceGuard guard(device);
     if (!guard.ok) return fail(WNV_ERR_HIP, "wnv_recurrence_backward: cannot select device %d", device);
