@@ -4,6 +4,7 @@ import ctypes
 import os
 import shutil
 import subprocess
+import sys
 
 import pytest
 import torch
@@ -146,3 +147,13 @@ def test_the_oracle_is_its_definition():
     codes, scales, zp = random_q4(3, 70, 32, 1)
     w = q4_weight(codes, scales, zp, 32)
     assert float(w[2, 69]) == float(scales[2, 2]) * (int(codes[2, 69]) - int(zp[2, 2]))
+
+
+def test_the_package_imports_without_a_gpu_build_of_torch():
+    """A torch built for the CPU has none of torch._C's _cuda_* functions."""
+    code = ("import torch\n"
+            "for n in [n for n in dir(torch._C) if n.startswith('_cuda_getCurrentRawStream')]:\n"
+            "    delattr(torch._C, n)\n"
+            "import wavenet_vocoder_amd, wavenet_vocoder_amd.engine, wavenet_vocoder_amd.modules, wavenet_vocoder_amd.recurrence\n")
+    r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr

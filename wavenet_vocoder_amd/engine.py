@@ -141,7 +141,13 @@ def _empty_pinned():
     return b
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream          # of a device by its index: the layer-level steps are a few microseconds long
+def _current_stream(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+# The current stream of a device by its index.  The layer-level steps are a few microseconds long, so it is torch's own short way, which
+# a build of torch without a GPU does not have.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _current_stream)
 
 
 def _stream(device: torch.device) -> int:
