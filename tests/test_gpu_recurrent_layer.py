@@ -187,3 +187,25 @@ def test_without_conditioning_and_next_to_the_convolution():
     m.train()
     with pytest.raises(RuntimeError, match="eval mode"):
         m.incremental_forward(x[:, :, 0][:, None])
+
+
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("which", [0, 1])
+def test_forward_mode_derivatives_are_refused(which, grad):
+    """Dual tensors on the device, next to the same calls without tangents, which run inside a dual level too."""
+    from torch.autograd import forward_ad
+    from wavenet_vocoder_amd.engine import Q4Linear
+    from wavenet_vocoder_amd.recurrence import gated_recurrence, gated_recurrence_step
+    q = Q4Linear(6, 6, "cuda", group_size=32, gates=3)
+    q.set_weights(torch.ones(6, 6, device="cuda"))
+    calls = [(lambda z, h: gated_recurrence(z, h), (1, 3, 6), (1, 2)), (gated_recurrence_step, (1, 6), (1, 2)), (q.recurrence_step, (1, 6), (1, 2))]
+    if which == 0:
+        calls.append((lambda x: q.step(x), (1, 6)))
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        for f, *shapes in calls:
+            plain = [torch.zeros(s, device="cuda") for s in shapes]
+            f(*plain)
+            plain[which] = forward_ad.make_dual(plain[which], torch.ones_like(plain[which]))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                f(*plain)
+    torch.cuda.synchronize()

@@ -157,3 +157,19 @@ def test_the_package_imports_without_a_gpu_build_of_torch():
             "import wavenet_vocoder_amd, wavenet_vocoder_amd.engine, wavenet_vocoder_amd.modules, wavenet_vocoder_amd.recurrence\n")
     r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True)
     assert r.returncode == 0, r.stderr
+
+
+@pytest.mark.parametrize("which", [0, 1])
+def test_forward_mode_derivatives_are_refused(which):
+    """A dual tensor does not require grad; its tangent has to end in an error, not in an output without one."""
+    from torch.autograd import forward_ad
+
+    def duals(*shapes):
+        return [forward_ad.make_dual(torch.zeros(s), torch.ones(s)) if i == which else torch.zeros(s) for i, s in enumerate(shapes)]
+    layer = Q4Linear.__new__(Q4Linear)
+    layer._h, layer._index, layer.cin, layer.channels = ctypes.c_void_p(), -1, 6, 2      # as a handle on the CPU would be, had it one
+    with forward_ad.dual_level():
+        for call in (lambda: gated_recurrence(*duals((1, 3, 6), (1, 2))), lambda: gated_recurrence_step(*duals((1, 6), (1, 2))),
+                     lambda: layer.recurrence_step(*duals((1, 6), (1, 2)))) + (() if which else (lambda: layer.step(*duals((1, 6))),)):
+            with pytest.raises(RuntimeError, match="forward-mode"), torch.no_grad():
+                call()

@@ -18,7 +18,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import DTYPE, RecurrenceArgs, check
-from .engine import _raw_stream, require_gpu_tensor
+from .engine import _raw_stream, refuse_tangents, require_gpu_tensor
 
 __all__ = ["gated_recurrence", "gated_recurrence_step"]
 
@@ -147,8 +147,9 @@ def gated_recurrence(z: torch.Tensor, h0: Optional[torch.Tensor] = None, *, outp
     ``h0`` (B, C) float32: the state before the first step (zeros).  ``lengths`` (B,): rows of a padded batch end there -- behind it z
     is not looked at, y and the gradients are zero, and the state is handed on (an empty row's is ``h0``).  ``seg_start`` (B, T): the
     map of a packed slot (``wnv_generate_args``) -- the state reads as zero at each step t with ``seg_start[b, t] == t``; a negative
-    entry is an utterance begun before this call, which goes on from ``h0``.  Differentiable (once) in z and h0.  Runs on the current
-    stream of z's device and is capturable; the same call gives the same bits."""
+    entry is an utterance begun before this call, which goes on from ``h0``.  Differentiable (once, not in forward mode) in z and h0.
+    Runs on the current stream of z's device and is capturable; the same call gives the same bits."""
+    refuse_tangents("gated_recurrence", z, h0)
     require_gpu_tensor(z, "z")
     _dtype(z)
     if z.dim() != 3:
@@ -174,6 +175,7 @@ def gated_recurrence(z: torch.Tensor, h0: Optional[torch.Tensor] = None, *, outp
 def gated_recurrence_step(z: torch.Tensor, state: torch.Tensor, *, output_gate: bool = True) -> torch.Tensor:
     """One step: z (B, 3 C) (``output_gate=False``: (B, 2 C)), ``state`` (B, C) float32 contiguous, updated in place -> y (B, C) of z's
     type.  Not differentiable: the training form is ``gated_recurrence``."""
+    refuse_tangents("gated_recurrence_step", z, state)
     shape, sshape, gates, dev = z.shape, state.shape, 3 if output_gate else 2, z.get_device()
     code = _DTYPES.get(z.dtype)
     if (code is None or dev < 0 or len(shape) != 2 or len(sshape) != 2 or sshape[0] != shape[0] or sshape[1] * gates != shape[1]
