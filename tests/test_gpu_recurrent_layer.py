@@ -209,3 +209,39 @@ def test_forward_mode_derivatives_are_refused(which, grad):
             with pytest.raises(RuntimeError, match="forward-mode"):
                 f(*plain)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("step", ["recurrence", "product"])
+def test_a_step_tells_autograd_that_it_wrote_the_state(step):
+    """A graph that saved the state before the step refuses its backward pass, as it does after torch's own in-place operations."""
+    from wavenet_vocoder_amd.engine import Q4Linear
+    from wavenet_vocoder_amd.recurrence import gated_recurrence_step
+    if step == "recurrence":
+        f = gated_recurrence_step
+    else:
+        q = Q4Linear(6, 6, "cuda", group_size=32, gates=3)
+        q.set_weights(torch.ones(6, 6, device="cuda"))
+        f = q.recurrence_step
+    x, state = torch.ones(1, 6, device="cuda"), torch.ones(1, 2, device="cuda")
+    w = torch.ones(1, 2, device="cuda", requires_grad=True)
+    (w * state).sum().backward()        # nothing written in between: allowed
+    out, version = (w * state).sum(), state._version
+    f(x, state)
+    assert state._version == version + 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.backward()
+    with torch.inference_mode():        # such a state has no version, and needs none
+        mine = torch.ones(1, 2, device="cuda")
+        f(x, mine)
+        again = torch.ones(1, 2, device="cuda")
+    f(x, again)
+    assert torch.equal(mine, again)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        f(x, state)
+    state.fill_(1)
+    for _ in range(3):
+        want = state.clone()
+        f(x, want)
+        g.replay()
+        assert torch.equal(state, want)

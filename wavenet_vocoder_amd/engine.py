@@ -12,6 +12,7 @@ from typing import Dict, Optional, Sequence
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from ._lib import Config, GenerateArgs, GluConfig, Tensor, check
@@ -537,6 +538,7 @@ class Q4Linear:
         if state.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("4-bit products are not differentiable: use torch.no_grad()")
         y = x.new_empty((B, self.channels))
+        increment_version(state)
         st = self._recurrence_step(self._h, x.data_ptr(), x.stride(0), state.data_ptr(), y.data_ptr(), B, code, _raw_stream(self._index))
         if st:
             check(st)

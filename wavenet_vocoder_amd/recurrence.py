@@ -15,6 +15,7 @@ from typing import Optional, Tuple
 
 import torch
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from ._lib import DTYPE, RecurrenceArgs, check
@@ -185,6 +186,7 @@ def gated_recurrence_step(z: torch.Tensor, state: torch.Tensor, *, output_gate: 
     B, n = sshape
     z = _rows(z)
     y = z.new_empty(sshape)
+    increment_version(state)            # a graph that saved the state has to see that it changed
     st = _lib.lib().wnv_recurrence_step(dev, z.data_ptr(), z.stride(0), state.data_ptr(), y.data_ptr(), B, n, gates, code, _raw_stream(dev))
     if st:
         check(st)
