@@ -130,3 +130,32 @@ def random_q4(n, k, group, seed, zeros=True):
     scales = (torch.rand(n, groups, generator=g) * 0.1 + 0.01).to(torch.bfloat16)
     zp = torch.randint(0, 16, (n, groups), generator=g, dtype=torch.uint8) if zeros else None
     return codes, scales, zp
+
+
+# ---- bounds by what is left of each input ---------------------------------------------------------------------------------------
+# The bounds above go by the largest v, h0 and dh of the whole call.  These go by m_t = sigmoid(f) m_{t-1} + sigmoid(-f) |v|, m_{-1} = |h0|: what
+# the inputs still weigh at step t, so that a state that a gate forgot, or a spike long ago, does not excuse an error now.
+# One step: sigmoid(-|f|) is off by delta = (1.5 |f| + 8) eps of itself (as above), 1 - sigmoid(-|f|) by no more than that and a rounding, two sums
+# follow, and below 2^-126 a gate may read as 0: within (delta + 4 eps) m + 2^-126 (|h| + |v|).
+TINY = 2.0 ** -126
+
+
+def gate_ends(dtype):
+    """f, h, v: every combination of gates that remember, forget and do neither with states and inputs of all sizes."""
+    big = min(float(torch.finfo(dtype).max) * 0.9, 3e38)
+    f = torch.tensor([-float("inf"), -200.0, -88.0, -40.0, -20.0, -16.0, -12.0, -10.0, -3.0, 0.0, 3.0, 9.0, 20.0, 88.0, 200.0, float("inf")])
+    h = torch.tensor([0.0, 1e-3, -1.0, 1000.0, -1e6, 1e8, 3e38, -3e38])
+    v = torch.tensor([0.0, 1.2345, -1.0, 1e-3, 6e4, big, -big])
+    f, h, v = (t.reshape(-1) for t in torch.meshgrid(f, h, v, indexing="ij"))
+    return f.to(dtype), h, v.to(dtype)
+
+
+def check_blend(got, f, h, v):
+    """One step's state against sigmoid(f) h + sigmoid(-f) v in 64 bits; at the infinite gates exactly h and v."""
+    f, h, v, got = f.double(), h.double(), v.double(), got.double().cpu()
+    keep, new = torch.sigmoid(f), torch.sigmoid(-f)
+    want = torch.where(f == float("inf"), h, torch.where(f == -float("inf"), v, keep * h + new * v))
+    bound = ((1.5 * f.abs().clamp(max=200) + 8) + 4) * EPS * (keep * h.abs() + new * v.abs()) + TINY * (h.abs() + v.abs())
+    bound = torch.where(f.isinf(), 0.0, bound)
+    over = (got - want).abs() > bound
+    assert not (over | got.isnan()).any(), [(float(f[i]), float(h[i]), float(v[i]), float(got[i]), float(want[i])) for i in (over | got.isnan()).nonzero()[:5, 0]]

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from tests._ops import DTYPES, EPS, near, q4_bound, q4_weight, random_q4
+from tests._ops import DTYPES, EPS, check_blend, gate_ends, near, q4_bound, q4_weight, random_q4
 from wavenet_vocoder_amd.engine import Q4Linear
 
 pytestmark = pytest.mark.gpu
@@ -258,3 +258,20 @@ def test_weights_are_not_set_while_capturing():
     for _ in range(3):
         g.replay()
         assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("B", [1, 7, 20])
+@pytest.mark.parametrize("gates", [2, 3])
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+def test_recurrence_step_with_gates_at_both_ends(dtype, gates, B):
+    """All weights are zero, so that the bias alone is z, in float32 for every type of x."""
+    f, h, v = gate_ends(torch.float32)
+    C = f.numel()
+    q = Q4Linear(40, gates * C, "cuda", group_size=32, gates=gates)
+    q.set_codes(torch.full((gates * C, 40), 8, dtype=torch.uint8, device="cuda"), torch.ones(gates * C, 2, dtype=torch.bfloat16, device="cuda"), None,
+                torch.cat([f, v] + [torch.zeros(C)] * (gates - 2)).cuda())
+    state = h.expand(B, C).contiguous().cuda()
+    y = q.recurrence_step(torch.randn(B, 40, generator=torch.Generator().manual_seed(1)).to(DTYPES[dtype]).cuda(), state)
+    for row in state:
+        check_blend(row, f, h, v)
+    assert torch.equal(y, (state * (0.5 if gates == 3 else 1.0)).to(y.dtype))

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from tests._ops import DTYPES, check_scan, near, oracle_scan
+from tests._ops import DTYPES, check_blend, check_scan, gate_ends, near, oracle_scan
 from wavenet_vocoder_amd.recurrence import gated_recurrence, gated_recurrence_step
 
 pytestmark = pytest.mark.gpu
@@ -504,3 +504,15 @@ def test_data_larger_than_the_caches(gates, dtype, kind):
     want = oracle_scan(zr, hr, gates == 3, dy=dy[row:row + 1].cpu(), dh_last=dh[row:row + 1].cpu(), **k)
     got = dict(y=outs[0][0][row:row + 1], h_last=outs[0][1][row:row + 1], dz=outs[0][2][row:row + 1])
     check_scan(got, want, zr, hr, gates == 3, k.get("lengths"), dy[row:row + 1], dh[row:row + 1])
+
+
+@pytest.mark.parametrize("gates", [2, 3])
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+def test_step_with_gates_at_both_ends(dtype, gates):
+    """A gate that forgets leaves of the state what the formula leaves, not 2^-24 of what it was; one that replaces it gives v."""
+    f, h, v = gate_ends(DTYPES[dtype])
+    state = h[None].cuda()
+    z = torch.cat([f, v] + [torch.zeros_like(v)] * (gates - 2))[None].cuda()
+    y = gated_recurrence_step(z, state, output_gate=gates == 3)
+    check_blend(state[0], f, h, v)
+    assert torch.equal(y, (state * (0.5 if gates == 3 else 1.0)).to(y.dtype))

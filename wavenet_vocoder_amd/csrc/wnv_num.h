@@ -27,3 +27,14 @@ __device__ __forceinline__ float wnv_gate(float x, float& slope) {
     slope = er * r;
     return x >= 0.f ? r : er;
 }
+// sigmoid(f) h + (1 - sigmoid(f)) v.  Of the two weights the smaller, sigmoid(-|f|), is known to its own precision, and the other is 1 less
+// that: a state that a gate remembers for n steps is not off by n roundings of a weight next to 1, and one that it forgets leaves what
+// the formula leaves of it, not 2^-24 of what it was.  Nothing overflows that the result does not.  f = inf gives h, f = -inf gives v
+// (both finite); a weight below 2^-126 may read as 0.
+__device__ __forceinline__ float wnv_blend(float f, float h, float v) {
+    const float e = __builtin_amdgcn_exp2f(fabsf(f) * -1.44269504088896340736f);
+    const float less = e * __builtin_amdgcn_rcpf(1.0f + e);
+    const bool keeps = f > 0.f;
+    const float more = keeps ? h : v, rest = keeps ? v : h;
+    return fmaf(less, rest, fmaf(-less, more, more));
+}

@@ -334,7 +334,7 @@ __global__ void __launch_bounds__(NT == 1 ? 1024 : 512) wnv_q4_rows(Q4Dev q, Q4C
             ((E*)a.y)[((long long)row * q.gates + gate) * q.rows + channel] = wnv_down<E>(z[0]);
         } else {
             float h = a.state[(long long)row * q.rows + channel];
-            h = fmaf(wnv_gate(-z[0]), z[GATES > 1 ? 1 : 0] - h, h);
+            h = wnv_blend(z[0], h, z[GATES > 1 ? 1 : 0]);
             a.state[(long long)row * q.rows + channel] = h;
             if (GATES == 3) h *= wnv_gate(z[GATES - 1]);
             ((E*)a.y)[(long long)row * q.rows + channel] = wnv_down<E>(h);

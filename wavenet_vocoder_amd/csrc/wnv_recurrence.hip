@@ -544,7 +544,7 @@ __global__ void __launch_bounds__(RT) wnv_recurrence_one(const E* z, long long z
     if (c >= C) return;
     z += (long long)b * zb + c;
     float h = state[(long long)b * C + c];
-    h = fmaf(wnv_gate(-wnv_up(z[0])), wnv_up(z[C]) - h, h);
+    h = wnv_blend(wnv_up(z[0]), h, wnv_up(z[C]));
     state[(long long)b * C + c] = h;
     if (gates == 3) h *= wnv_gate(wnv_up(z[2 * C]));
     y[(long long)b * C + c] = wnv_down<E>(h);
