@@ -11,6 +11,7 @@ Bounds, M = max(|v|, |h0|), S = max|dh|, u = 1 - sigmoid(f), eps = 2^-24 (half a
   * df = dh (h_{t-1} - v) sigmoid(f) u: k S 2 M + S k M + S 2 M (2 delta + 4 eps), times sigmoid(f) u <= 1/4: within k S M;
     dv = dh u: (k + delta + eps) S <= 2 k S;  do = dy h sigmoid(o)(1 - sigmoid(o)): (k M + M (2 delta + 4 eps)) |dy| / 4 <= k M |dy|.
   * the result's own type rounds by finfo.eps / 2 of the value (half a step of the smallest number near zero)."""
+import numpy as np
 import torch
 
 EPS = 2.0 ** -24
@@ -159,3 +160,84 @@ def check_blend(got, f, h, v):
     bound = torch.where(f.isinf(), 0.0, bound)
     over = (got - want).abs() > bound
     assert not (over | got.isnan()).any(), [(float(f[i]), float(h[i]), float(v[i]), float(got[i]), float(want[i])) for i in (over | got.isnan()).nonzero()[:5, 0]]
+
+
+# A whole sequence: h_t is a sum of the v_s (and h0), each times a product of gates, and every operation of the kernels but 1 - U (below) adds or
+# multiplies such terms, so that the error of a term is its own relative one: delta_l + 3 eps for each gate on its way (an operation for the
+# gate, one for the sum), and the joins of stretches, of a wave's rows, a chunk's waves, a group's chunks (15 at most), a section's groups
+# (15) and a state's start: 64 eps in all (a section more is 32768 steps more, whose own 3 eps each pay for it).  The product P of a
+# stretch's gates may be taken as 1 - U with U = sum of u_l times the product before it, U <= 1/2: off by eps + U times U's relative error,
+# no more than delta + eps a step.  So with m_t as above
+#     d_t = a_t (d_{t-1} + (delta_t + 3 eps) m_{t-1}) + u_t |v_t| (delta_t + 3 eps),    |h_t - exact| <= d_t + 64 eps m_t
+# and the same from the end for dh.  The products behind them: y = h sigmoid(o), dv = dh u, df = dh (h_{t-1} - v) a u, do = dy h so (1 - so), add
+# their gates' deltas and an eps an operation (of t h - t v, t = a u, by the magnitudes).  1.01 for what is quadratic, TINY M for gates that
+# read as 0.
+def local_scan(z, h0=None, output_gate=True, lengths=None, seg_start=None, dy=None, dh_last=None):
+    """(exact results, their bounds), float64 on the CPU step by step: dicts of y, h_last and, where dy is given, dz and dh0."""
+    z = z.detach().double().cpu().numpy()
+    B, T, n = z.shape
+    C = n // (3 if output_gate else 2)
+    n_live = np.full(B, T) if lengths is None else lengths.cpu().long().clamp(0, T).numpy()
+    live = np.arange(T) < n_live[:, None]
+    begins = np.zeros((B, T), bool) if seg_start is None else seg_start.cpu().long().numpy() == np.arange(T)
+    begins &= live
+    z = np.where(live[..., None], z, 0.0)
+    f, v = z[..., :C], z[..., C:2 * C]
+    delta = lambda x: (1.5 * np.abs(x) + 8) * EPS  # noqa: E731
+    sig = lambda x: 1 / (1 + np.exp(np.minimum(-x, 700)))  # noqa: E731
+    a, u = sig(f), sig(-f)
+    K = delta(f) + 3 * EPS
+    h = np.zeros((B, C)) if h0 is None else h0.detach().double().cpu().numpy().copy()
+    M = max(np.abs(v).max(), np.abs(h).max())
+    keep = np.where(live[..., None], np.where(begins[..., None], 0.0, a), 1.0)
+    new, loss = np.where(live[..., None], u * v, 0.0), np.where(live[..., None], K, 0.0)
+    hs, ms, ds = np.empty((T + 1, B, C)), np.empty((T + 1, B, C)), np.empty((T + 1, B, C))
+    hs[0], ms[0], ds[0] = h, np.abs(h), 0
+    for t in range(T):
+        k, l, w = keep[:, t], loss[:, t], new[:, t]
+        hs[t + 1] = k * hs[t] + w
+        ms[t + 1] = k * ms[t] + np.abs(w)
+        ds[t + 1] = k * (ds[t] + l * ms[t]) + np.abs(w) * l
+    hs, ms, eh = (x.transpose(1, 0, 2) for x in (hs, ms, 1.01 * (ds + 64 * EPS * ms) + 8 * TINY * M))
+    o = z[..., 2 * C:] if output_gate else None
+    so, do = (sig(o), delta(o)) if output_gate else (np.ones((B, T, C)), np.zeros((B, T, C)))
+    L = live[..., None]
+    want = dict(y=np.where(L, hs[:, 1:] * so, 0), h_last=hs[:, -1])
+    bound = dict(y=np.where(L, so * (eh[:, 1:] + (do + 2 * EPS) * ms[:, 1:]), 0), h_last=eh[:, -1])
+    if dy is not None:
+        dy = np.where(L, dy.double().cpu().numpy(), 0)
+        r = np.zeros((B, C)) if dh_last is None else dh_last.double().cpu().numpy()
+        mr, dr = np.abs(r), np.zeros((B, C))
+        S = max(np.abs(dy).max(), mr.max())
+        g, dh, mb, db = dy * so, np.empty((B, T, C)), np.empty((B, T, C)), np.empty((B, T, C))
+        for t in reversed(range(T)):
+            k, l, gt = keep[:, t], loss[:, t], g[:, t]
+            dh[:, t] = gt + r
+            mb[:, t] = np.abs(gt) + mr
+            db[:, t] = (do[:, t] + 2 * EPS) * np.abs(gt) + dr
+            r, mr, dr = k * dh[:, t], k * mb[:, t], k * (db[:, t] + l * mb[:, t])
+        eb = 1.01 * (db + 64 * EPS * mb) + 8 * TINY * S
+        before, mbe, ebe = (np.where(begins[..., None], 0, x[:, :-1]) for x in (hs, ms, eh))
+        t, K2 = a * u, 2 * delta(f) + 6 * EPS
+        dz = [dh * (before - v) * t, dh * u]
+        bz = [t * (eb * (mbe + np.abs(v)) + mb * (ebe + K2 * (mbe + np.abs(v)))), u * (eb + K * mb)]
+        if output_gate:
+            so1 = so * sig(-o)
+            dz.append(dy * hs[:, 1:] * so1)
+            bz.append(np.abs(dy) * so1 * (eh[:, 1:] + (2 * do + 6 * EPS) * ms[:, 1:]))
+        want.update(dz=np.concatenate([np.where(L, x, 0) for x in dz], -1), dh0=r)
+        bound.update(dz=np.concatenate([np.where(L, 1.01 * x + 8 * TINY * M * S, 0) for x in bz], -1), dh0=1.01 * (dr + 64 * EPS * mr) + 8 * TINY * S)
+    return tuple({k: torch.from_numpy(np.ascontiguousarray(x)) for k, x in d.items()} for d in (want, bound))
+
+
+def check_local(got, local, only=None):
+    """Every number within its own bound and the rounding to its type."""
+    want, bound = local
+    for k in want:
+        if got.get(k) is None or (only and k not in only):
+            continue
+        x, w, b = got[k].detach(), want[k], bound[k]
+        info = torch.finfo(x.dtype)
+        over = (x.double().cpu() - w).abs() / (b + info.eps / 2 * (w.abs() + b) + info.smallest_normal * info.eps / 2)
+        assert x.shape == w.shape and not x.isnan().any(), k
+        assert float(over.max()) <= 1.0, f"{k}: {float(over.max()):.3g} times its bound at {np.unravel_index(int(over.argmax()), over.shape)}"

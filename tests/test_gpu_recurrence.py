@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from tests._ops import DTYPES, check_blend, check_scan, gate_ends, near, oracle_scan
+from tests._ops import DTYPES, check_blend, check_local, check_scan, gate_ends, local_scan, near, oracle_scan
 from wavenet_vocoder_amd.recurrence import gated_recurrence, gated_recurrence_step
 
 pytestmark = pytest.mark.gpu
@@ -516,3 +516,91 @@ def test_step_with_gates_at_both_ends(dtype, gates):
     y = gated_recurrence_step(z, state, output_gate=gates == 3)
     check_blend(state[0], f, h, v)
     assert torch.equal(y, (state * (0.5 if gates == 3 else 1.0)).to(y.dtype))
+
+
+LOCAL_SHAPES = [(1, 1, 4), (2, 9, 3), (3, 130, 40), (2, 1000, 20), (2, 1000, 70), (1, 3000, 24), (1, 3000, 67)]
+
+
+@pytest.mark.parametrize("kind", ["full", "lengths", "both"])
+@pytest.mark.parametrize("what", ["h0", "dh_last", "v", "dy", "all"])
+@pytest.mark.parametrize("shape", LOCAL_SHAPES, ids=lambda s: "x".join(map(str, s)))
+def test_large_values_leave_what_the_gates_leave(shape, what, kind):
+    """A state, gradient, input or gradient of an output 1e6 times the others: what is left of it after its gates, no more."""
+    B, T, C = shape
+    z, h0, dy, dh = inputs(B, T, C, 3, torch.float32, seed=T + C)
+    z[..., :C] = (z[..., :C] - 2.0) / 1.5           # gates about 1/2
+    if what in ("h0", "all"):
+        h0 *= 1e6
+    if what in ("dh_last", "all"):
+        dh *= 1e6
+    if what in ("v", "all"):
+        z[:, T // 3, C:2 * C] *= 1e6
+    if what in ("dy", "all"):
+        dy[:, T // 2] *= 1e6
+    m = maps(kind, B, T, seed=T)
+    check_local(run(z, h0, dy, dh, 3, m), local_scan(z, h0, True, dy=dy, dh_last=dh, **m))
+
+
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+@pytest.mark.parametrize("f", [-80.0, -20.0, -16.0, -12.0, -10.0, -6.0, -1.0, 0.0, 1.0, 6.0, 10.0])
+@pytest.mark.parametrize("shape", [(2, 1, 8), (2, 2, 40), (1, 5, 130), (2, 300, 20), (2, 300, 70)], ids=lambda s: "x".join(map(str, s)))
+def test_gates_hold_their_precision_at_both_ends(shape, f, dtype):
+    """Every output of gates around f, dh0 of gates that forget among them: (2^-24 |f|) of itself, not of 1."""
+    B, T, C = shape
+    z, h0, dy, dh = inputs(B, T, C, 3, torch.float32, seed=7)
+    z[..., :C] = f + 0.1 * z[..., :C]
+    z = z.to(DTYPES[dtype])
+    dy = dy.to(DTYPES[dtype])
+    check_local(run(z, h0, dy, dh, 3, {}), local_scan(z, h0, True, dy=dy, dh_last=dh))
+
+
+@pytest.mark.parametrize("T", [3, 200, 700, 3000])
+@pytest.mark.parametrize("C", [12, 70])
+def test_infinite_gates_replace_and_keep(C, T):
+    """f = -inf: the state is v, whatever it was.  f = inf: the state stays."""
+    z, h0, dy, dh = inputs(2, T, C, 2, torch.float32, seed=10)
+    h0 *= 1e8
+    z[..., :C] = -float("inf")
+    got = run(z, h0, dy, dh, 2, {})
+    assert torch.equal(got["y"].cpu(), z[..., C:]) and torch.equal(got["h_last"].cpu(), z[:, -1, C:]) and not got["dh0"].any()
+    assert torch.equal(got["dz"][..., C:].cpu()[:, :-1], dy[:, :-1])
+    z[:, :, :C] = float("inf")
+    z[:, T // 2, :C] = -float("inf")
+    got = run(z, h0, dy, dh, 2, {})
+    want = h0[:, None].repeat(1, T, 1)
+    want[:, T // 2:] = z[:, T // 2, None, C:]
+    assert torch.equal(got["y"].cpu(), want) and torch.equal(got["h_last"].cpu(), want[:, -1])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("T", [4, 200, 700, 3000])
+@pytest.mark.parametrize("C", [12, 70])
+def test_values_at_the_type_s_ends(C, T, dtype):
+    """v, h0 and dh_last of both signs next to the largest number: a convex combination of them is none larger."""
+    z, h0, dy, dh = inputs(2, T, C, 2, torch.float32, seed=10)
+    sign = torch.where(torch.arange(T) % 2 == 0, 1.0, -1.0)[:, None]
+    z[..., :C] = (z[..., :C] - 2.0) / 1.5
+    z[..., C:] = 3e38 * sign
+    z = z.to(DTYPES[dtype])
+    h0 = torch.full_like(h0, -3e38)
+    dy *= 1e-20
+    dh = torch.full_like(dh, 1e-20)
+    check_local(run(z, h0, dy.to(z.dtype), dh, 2, {}), local_scan(z, h0, False, dy=dy.to(z.dtype), dh_last=dh))
+
+
+@pytest.mark.parametrize("T", [4, 200, 700, 3000])
+@pytest.mark.parametrize("C", [12, 70])
+def test_an_infinite_state_is_handed_on(C, T):
+    """Empty rows, and what stands behind a length, hand on what they are given, whatever it is: forward the state, backward its gradient."""
+    z, h0, dy, dh = inputs(3, T, C, 3, torch.float32, seed=14)
+    inf = float("inf")
+    for x in (h0, dh):
+        x[0, ::2], x[0, 1::3] = inf, -inf
+    n = torch.tensor([0, T // 2, T - 1], dtype=torch.int32)
+    z[1, T // 2 - 1, C:2 * C] = inf                 # the last live step's input: the state behind it is infinite, or
+    z[1, T // 2 - 1, :C] = 0.0
+    dh[2] = inf                                     # the gradient that arrives at row 2's end
+    got = run(z, h0, dy, dh, 3, dict(lengths=n))
+    assert torch.equal(got["h_last"][0].cpu(), h0[0]) and torch.equal(got["dh0"][0].cpu(), dh[0])
+    assert (got["h_last"][1] == inf).all()
+    assert torch.equal(got["dz"][2, T - 2, C:2 * C].cpu(), torch.full((C,), inf)) and not got["y"][0].any()

@@ -27,6 +27,13 @@ __device__ __forceinline__ float wnv_gate(float x, float& slope) {
     slope = er * r;
     return x >= 0.f ? r : er;
 }
+// sigmoid(f), and u = 1 - sigmoid(f) = sigmoid(-f), each to its own precision.
+__device__ __forceinline__ float wnv_gates(float f, float& u) {
+    const float e = __builtin_amdgcn_exp2f(fabsf(f) * -1.44269504088896340736f);
+    const float more = __builtin_amdgcn_rcpf(1.0f + e), less = e * more;
+    u = f > 0.f ? less : more;
+    return f > 0.f ? more : less;
+}
 // sigmoid(f) h + (1 - sigmoid(f)) v.  Of the two weights the smaller, sigmoid(-|f|), is known to its own precision, and the other is 1 less
 // that: a state that a gate remembers for n steps is not off by n roundings of a weight next to 1, and one that it forgets leaves what
 // the formula leaves of it, not 2^-24 of what it was.  Nothing overflows that the result does not.  f = inf gives h, f = -inf gives v

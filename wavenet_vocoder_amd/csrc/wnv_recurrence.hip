@@ -1,11 +1,12 @@
 // wnv_recurrence.hip -- the gated linear recurrence: a scan over (B, T, C), its backward pass, and one step with the state in place.
 //
 //   z = (f | v | o) along the channels,  u = 1 - sigmoid(f)
-//   h_t = sigmoid(f_t) h_{t-1} + (1 - sigmoid(f_t)) v_t = h_{t-1} + u_t (v_t - h_{t-1})          y_t = h_t sigmoid(o_t)   (no o: y = h)
+//   h_t = a_t h_{t-1} + u_t v_t,  a = sigmoid(f)          y_t = h_t sigmoid(o_t)   (no o: y = h)
 //
-// The second form of h_t is what runs: a gate that remembers long has sigmoid(f) next to 1, where 32 bits leave it 6e-8 off, and a
-// state that sums over 1 / u steps then is 6e-8 / u off; u itself is held to its own precision.  (An infinite v leaves v - h without
-// a value a step later: the rest of its utterance is NaN.)
+// a and u are each held to their own precision.  A gate that forgets leaves a h of the state, and h + u (v - h) would leave 2^-24 of h; a gate
+// that remembers long has a next to 1, where 32 bits leave it 6e-8 off, and a state that goes through 1 / u such steps is 6e-8 / u off.  So
+// steps are a h + u v only within a stretch of 8 of them, and what a stretch keeps of the state is 1 - U, with U summed up from its u, where
+// that is the more exact of the two.  (An infinite v or state is infinite or NaN for the rest of its utterance.)
 // h_{t-1} reads as zero at a step that begins an utterance of a packed slot (seg_start[b][t] == t).  Behind lengths[b] the state is
 // handed on, y and the gradients are zero, and z is not looked at.
 #include <hip/hip_runtime.h>
@@ -14,6 +15,8 @@
 
 #include "wnv_hostutil.h"
 #include "wnv_num.h"
+
+#pragma clang fp contract(off)          // what is fused is written as fmaf: one kernel's arithmetic is another's
 
 namespace {
 
@@ -36,40 +39,52 @@ struct RecArgs {
 };
 
 // ---- maps of the state --------------------------------------------------------------------------------------------------------
-// A stretch of steps maps the state before it to the state behind it: h -> h + (b - u h), with 1 - u the product of its gates; u < 0
-// says that the state behind it is b whatever stood before, which only happens where utterances begin (SEG; without the test a join
-// is 4 operations in place of 8, and the kernels a fifth shorter).  The backward pass maps what flows back by the same form.
-struct Map { float u, b; };
+// A stretch of steps maps the state before it to the state behind it: h -> p h + b, with p the product of its gates; u = 1 - p is carried
+// next to it (sums of products of gates, nothing is taken from anything), and p is 1 - u where u <= 1/2.  p < 0 says that the state behind
+// is b whatever stood before, which only happens where utterances begin (SEG).  A stretch without steps hands any h on as it is, an
+// infinite one too.  The backward pass maps what flows back by the same form.
+struct Map { float p, u, b; };
+constexpr Map NOTHING{1.f, 0.f, 0.f};
 
 template <bool SEG> __device__ __forceinline__ float apply(Map m, float h) {
-    const float r = h + fmaf(-m.u, h, m.b);
-    return SEG && m.u < 0.f ? m.b : r;
+    const float r = fmaf(m.p, h, m.b);
+    return SEG && m.p < 0.f ? m.b : r;
 }
 template <bool SEG> __device__ __forceinline__ Map join(Map first, Map then) {
     Map r;
-    r.u = fmaf(-first.u, then.u, first.u + then.u);
-    if (SEG && (then.u < 0.f || first.u < 0.f)) r.u = -1.f;
+    r.p = first.p * then.p;
+    r.u = fmaf(first.p, then.u, first.u);
     r.b = apply<SEG>(then, first.b);
+    if (SEG && (then.p < 0.f || first.p < 0.f)) r.p = -1.f;
     return r;
 }
 
-// A map is handed to the other workgroups as one 8-byte store that carries its own "valid": the workspace is filled with ones, and u
-// is never that pattern (a NaN is rewritten to the usual one).  No fence is needed: nothing else is read on the strength of it.
+// A map is handed to the other workgroups as one 8-byte store that carries its own "valid": b, and p where it is at most 1/2, else -u (2:
+// an utterance begins).  The workspace is filled with ones, and no map has that pattern (a NaN is rewritten to the usual one).  No fence
+// is needed: nothing else is read on the strength of it.
 constexpr unsigned EMPTY = 0xffffffffu;
-__device__ __forceinline__ void publish(unsigned long long* slot, Map m) {
-    const unsigned u = m.u != m.u ? 0x7fc00000u : __float_as_uint(m.u);
-    __hip_atomic_store(slot, ((unsigned long long)__float_as_uint(m.b) << 32) | u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+template <bool SEG> __device__ __forceinline__ void publish(unsigned long long* slot, Map m) {
+    float k = m.u <= 0.5f ? -m.u : m.p;
+    if (SEG && m.p < 0.f) k = 2.f;
+    const unsigned w = k != k ? 0x7fc00000u : __float_as_uint(k);
+    __hip_atomic_store(slot, ((unsigned long long)__float_as_uint(m.b) << 32) | w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 __device__ __forceinline__ unsigned long long peek(const unsigned long long* slot) {
     return __hip_atomic_load(slot, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ __forceinline__ Map unpacked(unsigned long long v) { return {__uint_as_float((unsigned)v), __uint_as_float((unsigned)(v >> 32))}; }
+template <bool SEG> __device__ __forceinline__ Map unpacked(unsigned long long v) {
+    const float k = __uint_as_float((unsigned)v), rest = 1.f - fabsf(k), b = __uint_as_float((unsigned)(v >> 32));
+    const bool u = (int)(unsigned)v < 0;            // the sign, of a zero too
+    Map m{u ? rest : k, u ? -k : rest, b};
+    if (SEG && k > 1.f) m.p = -1.f;
+    return m;
+}
 
 // Waits until the first n (uniform, N at most) of the slots that lie W apart hold maps, and hands them to `take` in their order.
 // The wait ends: a workgroup draws its chunk from a counter, so the chunks before that of one that runs have all been started, and
 // the lowest of them waits for nobody.  Should a slot stay empty for some seconds all the same, its map is NaN: the launch ends, and
 // says so in its results.
-template <int N, typename F> __device__ __forceinline__ void take_maps(const unsigned long long* slots, int W, int n, F take) {
+template <int N, bool SEG, typename F> __device__ __forceinline__ void take_maps(const unsigned long long* slots, int W, int n, F take) {
     unsigned long long v[N];
     for (int tries = 0;; ++tries) {
         bool holds = true;
@@ -84,7 +99,7 @@ template <int N, typename F> __device__ __forceinline__ void take_maps(const uns
     }
 #pragma unroll
     for (int i = 0; i < N; ++i)
-        if (i < n) take(unpacked(v[i]));        // the empty pattern itself is a NaN
+        if (i < n) take(unpacked<SEG>(v[i]));   // the empty pattern itself is a NaN
 }
 
 // How a chunk learns the state before it, without a chain through all chunks and in one order of arithmetic whatever the timing:
@@ -109,11 +124,11 @@ __device__ __forceinline__ Slots slots_at(unsigned long long* all, int row, int 
 template <int W, bool SEG> __device__ __forceinline__ Map map_in_group(const Slots& s, int k, int chunks, Map own) {
     const int at = k % GROUP;
     const bool more = k + 1 < chunks, last = at == GROUP - 1;
-    if (more && !last) publish(s.chunk + (long long)k * W, own);
-    Map all{0.f, 0.f};
+    if (more && !last) publish<SEG>(s.chunk + (long long)k * W, own);
+    Map all = NOTHING;
     for (int i = 0; i < at; i += GROUP / 2)         // 8 at a time: 15 at once cost 14 registers more, and a wave per SIMD with them
-        take_maps<GROUP / 2>(s.chunk + (long long)(k - at + i) * W, W, min(at - i, GROUP / 2), [&](Map m) { all = join<SEG>(all, m); });
-    if (more && last && k / GROUP % GROUP != GROUP - 1) publish(s.group + (long long)(k / GROUP) * W, join<SEG>(all, own));
+        take_maps<GROUP / 2, SEG>(s.chunk + (long long)(k - at + i) * W, W, min(at - i, GROUP / 2), [&](Map m) { all = join<SEG>(all, m); });
+    if (more && last && k / GROUP % GROUP != GROUP - 1) publish<SEG>(s.group + (long long)(k / GROUP) * W, join<SEG>(all, own));
     return all;
 }
 // The state before the group of chunk k as far as the first 8 groups of its section lead, `first` before chunk 0, and the map of
@@ -121,14 +136,14 @@ template <int W, bool SEG> __device__ __forceinline__ Map map_in_group(const Slo
 template <int W, bool SEG> __device__ __forceinline__ float state_before_groups(const Slots& s, int k, float first) {
     const int section = k / (GROUP * GROUP), g0 = section * GROUP, n = min(k / GROUP - g0, GROUP / 2);
     float h = first;
-    if (section) take_maps<1>(s.section + (long long)(section - 1) * W, W, 1, [&](Map m) { h = m.b; });
-    take_maps<GROUP / 2>(s.group + (long long)g0 * W, W, n, [&](Map m) { h = apply<SEG>(m, h); });
+    if (section) take_maps<1, SEG>(s.section + (long long)(section - 1) * W, W, 1, [&](Map m) { h = m.b; });
+    take_maps<GROUP / 2, SEG>(s.group + (long long)g0 * W, W, n, [&](Map m) { h = apply<SEG>(m, h); });
     return h;
 }
 template <int W, bool SEG> __device__ __forceinline__ Map map_of_groups(const Slots& s, int k) {
     const int g0 = k / (GROUP * GROUP) * GROUP + GROUP / 2, n = k / GROUP - g0;
-    Map all{0.f, 0.f};
-    take_maps<GROUP / 2 - 1>(s.group + (long long)g0 * W, W, n, [&](Map m) { all = join<SEG>(all, m); });
+    Map all = NOTHING;
+    take_maps<GROUP / 2 - 1, SEG>(s.group + (long long)g0 * W, W, n, [&](Map m) { all = join<SEG>(all, m); });
     return all;
 }
 __device__ __forceinline__ bool ends_section(int k, int chunks) { return (k + 1) % (GROUP * GROUP) == 0 && k + 1 < chunks; }
@@ -186,29 +201,69 @@ template <typename E, int V, bool STREAM> __device__ __forceinline__ void store(
 // The maps of a wave's rows joined in time (BACK: the last row first): of all of them, and of those before the own row.
 template <int LANES, bool BACK, bool SEG> __device__ __forceinline__ void join_rows(Map x, Map& all, Map& before) {
     if constexpr (LANES == 16) {        // four rows: two exchanges of registers, no LDS
-        const auto u = __builtin_amdgcn_permlane16_swap(__float_as_uint(x.u), __float_as_uint(x.u), false, false);     // rows 0 0 2 2 | 1 1 3 3
+        const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(x.p), __float_as_uint(x.p), false, false);     // rows 0 0 2 2 | 1 1 3 3
+        const auto u = __builtin_amdgcn_permlane16_swap(__float_as_uint(x.u), __float_as_uint(x.u), false, false);
         const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x.b), __float_as_uint(x.b), false, false);
-        const Map even{__uint_as_float(u[0]), __uint_as_float(b[0])}, odd{__uint_as_float(u[1]), __uint_as_float(b[1])};
+        const Map even{__uint_as_float(p[0]), __uint_as_float(u[0]), __uint_as_float(b[0])};
+        const Map odd{__uint_as_float(p[1]), __uint_as_float(u[1]), __uint_as_float(b[1])};
         const Map pair = BACK ? join<SEG>(odd, even) : join<SEG>(even, odd);
-        const auto pu = __builtin_amdgcn_permlane32_swap(__float_as_uint(pair.u), __float_as_uint(pair.u), false, false);  // rows 0 1 0 1 | 2 3 2 3
+        const auto pp = __builtin_amdgcn_permlane32_swap(__float_as_uint(pair.p), __float_as_uint(pair.p), false, false);  // rows 0 1 0 1 | 2 3 2 3
+        const auto pu = __builtin_amdgcn_permlane32_swap(__float_as_uint(pair.u), __float_as_uint(pair.u), false, false);
         const auto pb = __builtin_amdgcn_permlane32_swap(__float_as_uint(pair.b), __float_as_uint(pair.b), false, false);
-        const Map low{__uint_as_float(pu[0]), __uint_as_float(pb[0])}, high{__uint_as_float(pu[1]), __uint_as_float(pb[1])};
+        const Map low{__uint_as_float(pp[0]), __uint_as_float(pu[0]), __uint_as_float(pb[0])};
+        const Map high{__uint_as_float(pp[1]), __uint_as_float(pu[1]), __uint_as_float(pb[1])};
         const int row = (threadIdx.x / LANES) & 3;
         all = BACK ? join<SEG>(high, low) : join<SEG>(low, high);
-        before = (row & 1) != BACK ? (BACK ? odd : even) : Map{0.f, 0.f};
+        before = (row & 1) != BACK ? (BACK ? odd : even) : NOTHING;
         if ((row >> 1) != BACK) before = join<SEG>(BACK ? high : low, before);
     } else {                            // each row joined to the one 1, 2, 4, ... rows before it
+        const auto moved = [](Map m, int d) {
+            return BACK ? Map{__shfl_down(m.p, d), __shfl_down(m.u, d), __shfl_down(m.b, d)}
+                        : Map{__shfl_up(m.p, d), __shfl_up(m.u, d), __shfl_up(m.b, d)};
+        };
         const int row = BACK ? 63 / LANES - threadIdx.x % 64 / LANES : threadIdx.x % 64 / LANES;
 #pragma unroll
         for (int d = LANES; d < 64; d *= 2) {
-            const Map other{BACK ? __shfl_down(x.u, d) : __shfl_up(x.u, d), BACK ? __shfl_down(x.b, d) : __shfl_up(x.b, d)};
+            const Map other = moved(x, d);
             if (row >= d / LANES) x = join<SEG>(other, x);
         }
         const int last = (BACK ? 0 : 64 - LANES) + threadIdx.x % LANES;
-        all = {__shfl(x.u, last), __shfl(x.b, last)};
-        before = {BACK ? __shfl_down(x.u, LANES) : __shfl_up(x.u, LANES), BACK ? __shfl_down(x.b, LANES) : __shfl_up(x.b, LANES)};
-        if (row == 0) before = {0.f, 0.f};
+        all = {__shfl(x.p, last), __shfl(x.u, last), __shfl(x.b, last)};
+        before = moved(x, LANES);
+        if (row == 0) before = NOTHING;
     }
+}
+
+// What a forward pass keeps of its stretch's steps for the second run over them.  float32: a and u v.  16-bit types: the smaller of a and u,
+// negative where that is u, next to v as it came; 16 registers less, which are a fourth wave per SIMD (bf16 8 x 24064 x 512: 172 us for
+// 178), and the arithmetic of wnv_blend.
+template <typename E, int V> struct Steps {
+    float keep[L][V], put[L][V];
+    __device__ __forceinline__ void hold(int l, int i, float a, float, float uv) { keep[l][i] = a; put[l][i] = uv; }
+    __device__ __forceinline__ float run(int l, int i, float h, float) const { return fmaf(keep[l][i], h, put[l][i]); }
+};
+template <typename E, int V> struct PackedSteps {
+    float less[L][V];
+    __device__ __forceinline__ void hold(int l, int i, float a, float u, float) { less[l][i] = u < a ? -u : a; }
+    __device__ __forceinline__ float run(int l, int i, float h, float v) const {
+        const bool keeps = (int)__float_as_uint(less[l][i]) < 0;
+        const float more = keeps ? h : v, rest = keeps ? v : h, w = fabsf(less[l][i]);
+        return fmaf(w, rest, fmaf(-w, more, more));
+    }
+};
+template <int V> struct Steps<wnv_bf16, V> : PackedSteps<wnv_bf16, V> {};
+template <int V> struct Steps<wnv_f16, V> : PackedSteps<wnv_f16, V> {};
+
+// A stretch's map step by step, and at its end.
+template <bool SEG> __device__ __forceinline__ void step(Map& m, float keep, float u, float put, bool begins) {
+    if (SEG && begins) m.b = 0.f;
+    m.b = fmaf(keep, m.b, put);
+    m.u = fmaf(u, m.p, m.u);
+    m.p *= keep;
+}
+template <bool SEG> __device__ __forceinline__ void finish(Map& m, int begins) {
+    if (m.u <= 0.5f) m.p = 1.f - m.u;
+    if (SEG && begins) m.p = -1.f;
 }
 
 struct Place { int b, tile, chunk, row; };
@@ -269,7 +324,7 @@ template <int LANES, bool SEG> __device__ __forceinline__ int begins_in(const En
 // its registers.  z is read once.  Chunks that are live to their end (FULL) run without a test at every step: the steps' exponentials
 // and reciprocals then overlap (bf16 8 x 24064 x 512 forward: 164 us, with the tests 185).
 template <typename E, int G, int V, int LANES, int WAVES, bool SEG, bool STREAM>
-__global__ void __launch_bounds__(64 * WAVES, WAVES > 4 ? 2 : SEG && sizeof(E) == 2 ? 4 : 3) wnv_recurrence_fwd(RecArgs a) {
+__global__ void __launch_bounds__(64 * WAVES, WAVES > 4 ? 2 : sizeof(E) == 2 ? 4 : 3) wnv_recurrence_fwd(RecArgs a) {
     constexpr int W = LANES * V, STEPS = Shape<LANES, WAVES>::STEPS;
     __shared__ Map totals[WAVES][W], prev[W], groups[W];
     __shared__ float base[W];
@@ -284,7 +339,7 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES > 4 ? 2 : SEG && sizeof(E) =
     const uint32_t from = (uint32_t)(tid / LANES * L * a.zt + c) * (uint32_t)sizeof(E);
 
     Vec<E, V> f[L], v[L], o[L];
-    float u[L][V];
+    Steps<E, V> steps;
     Map m[V], before[V];
     int begins = 0;
     const auto reduce = [&](auto full) {
@@ -298,28 +353,39 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES > 4 ? 2 : SEG && sizeof(E) =
             }
         begins = begins_in<LANES, SEG>(entries, live);
 #pragma unroll
-        for (int i = 0; i < V; ++i) m[i] = {0.f, 0.f};
+        for (int i = 0; i < V; ++i) m[i] = NOTHING;
 #pragma unroll
         for (int l = 0; l < L; ++l)
             if (FULL || l < live) {
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    u[l][i] = wnv_gate(-f[l].get(i));
-                    if (SEG && begins >> l & 1) m[i].b = 0.f;
-                    m[i].u = fmaf(-u[l][i], m[i].u, m[i].u + u[l][i]);
-                    m[i].b = fmaf(u[l][i], v[l].get(i) - m[i].b, m[i].b);
+                    float u;
+                    const float keep = wnv_gates(f[l].get(i), u), put = u * v[l].get(i);
+                    steps.hold(l, i, keep, u, put);
+                    step<false>(m[i], keep, u, put, false);
                 }
             }
     };
     if (whole) reduce(std::true_type{});
     else reduce(std::false_type{});
+    const bool any = SEG && __any(begins);
+    const auto rows = [&](auto seg) {
+        constexpr bool S = decltype(seg)::value;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        if (SEG && begins) m[i].u = -1.f;
-        Map all;
-        join_rows<LANES, false, SEG>(m[i], all, before[i]);
-        if (tid % 64 < LANES) totals[wave][at + i] = all;
-    }
+        for (int i = 0; i < V; ++i) {
+            if (S && begins) {          // the state of its last utterance, from nothing
+#pragma unroll
+                for (int l = 0; l < L; ++l)
+                    if (l < live) m[i].b = steps.run(l, i, begins >> l & 1 ? 0.f : m[i].b, v[l].get(i));
+            }
+            finish<S>(m[i], begins);
+            Map all;
+            join_rows<LANES, false, S>(m[i], all, before[i]);
+            if (tid % 64 < LANES) totals[wave][at + i] = all;
+        }
+    };
+    if (any) rows(std::integral_constant<bool, SEG>{});
+    else rows(std::false_type{});
     __syncthreads();
     const int ch = tid % 64;
     if (wave < 3 && ch < W) {
@@ -347,14 +413,14 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES > 4 ? 2 : SEG && sizeof(E) =
         if (tid >= 64 * WAVES - LANES) {                   // the chunk's last stretch: the state behind it
             const float last = apply<SEG>(m[i], h[i]);
             if (ends_section(p.chunk, a.chunks))
-                publish(slots_at(a.slots, p.row, a.chunks, W, at + i).section + (long long)(p.chunk / (GROUP * GROUP)) * W, {-1.f, last});
+                publish<SEG>(slots_at(a.slots, p.row, a.chunks, W, at + i).section + (long long)(p.chunk / (GROUP * GROUP)) * W, {0.f, 1.f, last});
             if (p.chunk + 1 == a.chunks) a.h_last[(long long)p.b * a.C + c + i] = last;
         }
     }
     E* y = (E*)a.y + ((long long)p.b * a.T + (long long)p.chunk * STEPS) * a.C;
     const uint32_t to = (uint32_t)(tid / LANES * L * a.C + c) * (uint32_t)sizeof(E);
-    const auto run = [&](auto full) {
-        constexpr bool FULL = decltype(full)::value;
+    const auto run = [&](auto full, auto seg) {
+        constexpr bool FULL = decltype(full)::value, S = decltype(seg)::value;
 #pragma unroll
         for (int l = 0; l < L; ++l)
             if (FULL || t0 + l < a.T) {
@@ -363,8 +429,8 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES > 4 ? 2 : SEG && sizeof(E) =
                 for (int i = 0; i < V; ++i) {
                     float q = 0.f;
                     if (FULL || l < live) {
-                        if (SEG && begins >> l & 1) h[i] = 0.f;
-                        h[i] = fmaf(u[l][i], v[l].get(i) - h[i], h[i]);
+                        if (S && begins >> l & 1) h[i] = 0.f;
+                        h[i] = steps.run(l, i, h[i], v[l].get(i));
                         q = h[i];
                         if (G == 3) q *= wnv_gate(o[l].get(i));
                     }
@@ -373,12 +439,13 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES > 4 ? 2 : SEG && sizeof(E) =
                 store<E, V, STREAM>(y + (long long)l * a.C, to, out);
             }
     };
-    if (whole) run(std::true_type{});
-    else run(std::false_type{});
+    if (whole && !any) run(std::true_type{}, std::false_type{});
+    else if (SEG && whole) run(std::true_type{}, std::integral_constant<bool, SEG>{});
+    else run(std::false_type{}, std::integral_constant<bool, SEG>{});
 }
 
-// g_t = dy_t sigmoid(o_t);  dh_t = g_t + (what step t+1 hands back);  hands back r = dh_t - u_t dh_t, nothing over a beginning
-// df = dh (h_{t-1} - v) sigmoid(f) u;  dv = dh u;  do = dy h sigmoid(o) (1 - sigmoid(o))
+// g_t = dy_t sigmoid(o_t);  dh_t = g_t + (what step t+1 hands back);  hands back r = a_t dh_t, nothing over a beginning
+// df = dh (h_{t-1} - v) a u;  dv = dh u;  do = dy h sigmoid(o) (1 - sigmoid(o))
 // The chunks run from the last to the first, r is found the way the forward pass finds h; h itself starts from the state that the
 // forward pass saved before each chunk and is run through again.
 template <typename E, int G, int V, int LANES, int WAVES, bool SEG, bool STREAM>
@@ -400,7 +467,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) wnv_recurrence_bwd(RecArgs a) {
 
     Vec<E, V> f[L], v[L], o[L], d[L];
     Vec<float, V> saved;
-    float u[L][V], uk[L][V], g[L][V], q[L][V];          // u sigmoid(f); dy sigmoid(o); dy sigmoid(o) (1 - sigmoid(o))
+    float keep[L][V], u[L][V], g[L][V], q[L][V];        // a, u; dy sigmoid(o); dy sigmoid(o) (1 - sigmoid(o))
     Map m[V], r[V];
     int begins = 0;
     const auto reduce = [&](auto full) {
@@ -416,16 +483,14 @@ __global__ void __launch_bounds__(64 * WAVES, 2) wnv_recurrence_bwd(RecArgs a) {
         saved = load<float, V, false>(a.saved + ((long long)p.row * a.chunks + p.chunk) * W, at * 4);
         begins = begins_in<LANES, SEG>(entries, live);
 #pragma unroll
-        for (int i = 0; i < V; ++i) m[i] = r[i] = {0.f, 0.f};
+        for (int i = 0; i < V; ++i) m[i] = r[i] = NOTHING;
 #pragma unroll
         for (int l = 0; l < L; ++l)
             if (FULL || l < live) {
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    u[l][i] = wnv_gate(-f[l].get(i), uk[l][i]);
-                    if (SEG && begins >> l & 1) m[i].b = 0.f;
-                    m[i].u = fmaf(-u[l][i], m[i].u, m[i].u + u[l][i]);
-                    m[i].b = fmaf(u[l][i], v[l].get(i) - m[i].b, m[i].b);
+                    keep[l][i] = wnv_gates(f[l].get(i), u[l][i]);
+                    step<SEG>(m[i], keep[l][i], u[l][i], u[l][i] * v[l].get(i), begins >> l & 1);
                     g[l][i] = a.dy ? d[l].get(i) : 0.f;
                     if (G == 3) {
                         const float so = wnv_gate(o[l].get(i), q[l][i]);
@@ -440,7 +505,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) wnv_recurrence_bwd(RecArgs a) {
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     const float dh = g[l][i] + r[i].b;
-                    r[i].b = SEG && begins >> l & 1 ? 0.f : fmaf(-u[l][i], dh, dh);
+                    r[i].b = SEG && begins >> l & 1 ? 0.f : keep[l][i] * dh;
                 }
             }
     };
@@ -449,7 +514,8 @@ __global__ void __launch_bounds__(64 * WAVES, 2) wnv_recurrence_bwd(RecArgs a) {
     Map h_before[V], r_before[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        if (SEG && begins) m[i].u = -1.f;
+        finish<SEG>(m[i], begins);
+        r[i].p = m[i].p;
         r[i].u = m[i].u;
         Map all, all_back;
         join_rows<LANES, false, SEG>(m[i], all, h_before[i]);
@@ -485,7 +551,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) wnv_recurrence_bwd(RecArgs a) {
         if (tid < LANES) {                              // the chunk's first stretch: what flows out of it
             const float out = apply<SEG>(r[i], x[i]);
             if (ends_section(order, a.chunks))
-                publish(slots_at(a.slots, p.row, a.chunks, W, at + i).section + (long long)(order / (GROUP * GROUP)) * W, {-1.f, out});
+                publish<SEG>(slots_at(a.slots, p.row, a.chunks, W, at + i).section + (long long)(order / (GROUP * GROUP)) * W, {0.f, 1.f, out});
             if (p.chunk == 0 && a.dh0) a.dh0[(long long)p.b * a.C + c + i] = out;
         }
     }
@@ -493,14 +559,14 @@ __global__ void __launch_bounds__(64 * WAVES, 2) wnv_recurrence_bwd(RecArgs a) {
     const uint32_t to = (uint32_t)(tid / LANES * L * G * a.C + c) * (uint32_t)sizeof(E);
     const auto run = [&](auto full) {
         constexpr bool FULL = decltype(full)::value;
-        float before[L][V];
+        float behind[L][V];
 #pragma unroll
         for (int l = 0; l < L; ++l)
             if (FULL || l < live) {
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    before[l][i] = SEG && begins >> l & 1 ? 0.f : h[i];
-                    h[i] = fmaf(u[l][i], v[l].get(i) - before[l][i], before[l][i]);
+                    const float before = SEG && begins >> l & 1 ? 0.f : l ? behind[l - 1][i] : h[i];
+                    behind[l][i] = fmaf(keep[l][i], before, u[l][i] * v[l].get(i));
                 }
             }
 #pragma unroll
@@ -511,11 +577,12 @@ __global__ void __launch_bounds__(64 * WAVES, 2) wnv_recurrence_bwd(RecArgs a) {
                 for (int i = 0; i < V; ++i) {
                     float xf = 0.f, xv = 0.f, xo = 0.f;
                     if (FULL || l < live) {
-                        const float w = v[l].get(i) - before[l][i], dh = g[l][i] + x[i];
-                        xf = -dh * w * uk[l][i];
+                        const float before = SEG && begins >> l & 1 ? 0.f : l ? behind[l - 1][i] : h[i];
+                        const float slope = keep[l][i] * u[l][i], dh = g[l][i] + x[i];
+                        xf = dh * fmaf(slope, before, -(slope * v[l].get(i)));      // the difference itself may overflow
                         xv = dh * u[l][i];
-                        if (G == 3) xo = q[l][i] * fmaf(u[l][i], w, before[l][i]);
-                        x[i] = SEG && begins >> l & 1 ? 0.f : fmaf(-u[l][i], dh, dh);
+                        if (G == 3) xo = q[l][i] * behind[l][i];
+                        x[i] = SEG && begins >> l & 1 ? 0.f : keep[l][i] * dh;
                     }
                     df[i] = xf;
                     dv[i] = xv;
