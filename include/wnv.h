@@ -353,8 +353,9 @@ WNV_API wnv_status wnv_logmel(wnv_mel_handle h, const wnv_logmel_args* args);
  * The maps live in device memory and are not range-checked further: any value of seg_start other than t just does not begin one.
  * Infinite gates are their limits (f = inf keeps the state, f = -inf replaces it, o = -inf gives 0); an infinite v makes the rest of
  * its utterance NaN.
- * No atomics on data: the same call gives the same bits.  Everything a call needs beyond its arguments is in `workspace`, which the
- * call writes before it reads: calls that may run at the same time (other streams, graphs replayed side by side) each have their own. */
+ * No atomics on data: the same call gives the same bits, and a row's bits do not depend on the rows beside it.
+ * Everything a call needs beyond its arguments is in `workspace`, which the call writes before it reads: calls that may run at the same
+ * time (other streams, graphs replayed side by side) each have their own. */
 typedef enum wnv_dtype { WNV_F32 = 0, WNV_BF16 = 1, WNV_F16 = 2 } wnv_dtype;
 struct wnv_recurrence_args {
     int32_t B, C;

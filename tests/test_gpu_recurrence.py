@@ -604,3 +604,20 @@ def test_an_infinite_state_is_handed_on(C, T):
     assert torch.equal(got["h_last"][0].cpu(), h0[0]) and torch.equal(got["dh0"][0].cpu(), dh[0])
     assert (got["h_last"][1] == inf).all()
     assert torch.equal(got["dz"][2, T - 2, C:2 * C].cpu(), torch.full((C,), inf)) and not got["y"][0].any()
+
+
+@pytest.mark.parametrize("kind", ["full", "both"])
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+@pytest.mark.parametrize("shape", [(90, 300, 100), (30, 300, 300), (9, 512, 700), (60, 1000, 40), (40, 700, 130), (20, 1024, 256), (80, 513, 67), (200, 129, 130),
+                                   (100, 1000, 30), (600, 700, 8), (700, 1024, 3), (100, 900, 32), (5000, 513, 1)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_a_rows_bits_do_not_depend_on_its_batch_at_any_length(shape, dtype, kind):
+    """Sequences that a small batch runs in one workgroup and a large one in several, whose joins are the same."""
+    B, T, C = shape
+    z, h0, dy, dh = inputs(B, T, C, 3, DTYPES[dtype], seed=3)
+    m = maps(kind, B, T, seed=5)
+    all_ = run(z, h0, dy, dh, 3, m)
+    for b, n in ((0, 1), (B // 2, 2), (B - 1, 1)):
+        part = run(z[b:b + n], h0[b:b + n], dy[b:b + n], dh[b:b + n], 3, {k: v[b:b + n] for k, v in m.items()})
+        for k in all_:
+            assert torch.equal(part[k], all_[k][b:b + n]), (k, b)

@@ -22,6 +22,7 @@ namespace {
 
 struct RecArgs {
     int B, C, T, tiles, chunks;     // tiles of the channels, chunks of the time
+    int part_bits;                  // a part is 1 << part_bits blocks
     long long zb, zt;               // batch and time stride of z, in elements
     long long h0b;
     const void* z;
@@ -29,7 +30,7 @@ struct RecArgs {
     const int *lengths, *seg_start;
     void* y;
     float* h_last;
-    float* saved;                   // [row][chunk][tile width]: the state before the chunk's first step
+    float* saved;                   // [row][chunk][part][tile width]: the state before the part's first step
     unsigned long long* slots;      // workspace: of each row of tiles a counter, then its maps
     const void* dy;
     long long dyb, dyt;
@@ -71,6 +72,12 @@ template <bool SEG> __device__ __forceinline__ void publish(unsigned long long* 
 }
 __device__ __forceinline__ unsigned long long peek(const unsigned long long* slot) {
     return __hip_atomic_load(slot, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// A map as it comes out of a slot.
+template <bool SEG> __device__ __forceinline__ Map handed_on(Map m) {
+    if (m.u <= 0.5f) m.p = SEG && m.p < 0.f ? m.p : 1.f - m.u;
+    else m.u = 1.f - m.p;
+    return m;
 }
 template <bool SEG> __device__ __forceinline__ Map unpacked(unsigned long long v) {
     const float k = __uint_as_float((unsigned)v), rest = 1.f - fabsf(k), b = __uint_as_float((unsigned)(v >> 32));
@@ -156,9 +163,14 @@ __device__ __forceinline__ bool ends_section(int k, int chunks) { return (k + 1)
 // and 3 workgroups backward took 356 us for 316.  The last lane of a tile that ends in no multiple of V starts earlier and shares
 // channels with its neighbour (both compute and write the same); V = 1 is for rows narrower than 4.  Narrow tiles take stretches of 4
 // lanes, 16 to a wave.
-constexpr int L = 8;
+//
+// Which cut runs goes by the amount of data too, and does not show in the results: 4 stretches are a quad, 4 quads a block of 128 steps, 1 block
+// or, of rows up to 32 channels, 4 are a part.  The four of a quad and of a block are joined two and two, blocks within their part and
+// parts one after the other, whether a workgroup holds one part, and the parts are chunks that hand each other their maps, or all of them.
+constexpr int L = 8, BLOCK = 16 * L;
 template <int LANES, int WAVES> struct Shape {
-    static constexpr int ROWS = 64 / LANES, WAVE_STEPS = ROWS * L, STEPS = WAVES * WAVE_STEPS;
+    static constexpr int STEPS = WAVES * (64 / LANES) * L;
+    static constexpr int QUADS = STEPS / (4 * L), BLOCKS = QUADS / 4;
 };
 
 // V elements as they stand in memory, packed in as few registers; addresses are a uniform base and 32 bits of a lane's own.
@@ -190,7 +202,12 @@ template <typename E, int V, bool STREAM> __device__ __forceinline__ void store(
     typedef typename Raw<V * sizeof(E)>::T R;
     E e[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) e[i] = wnv_down<E>(x[i]);
+    for (int i = 0; i < V; ++i) {
+        float f = x[i];
+        // a float32 product is rounded before it becomes f16, in every kernel: the compiler makes one mixed instruction of the two in some
+        if (__is_same(E, wnv_f16)) asm("" : "+v"(f));
+        e[i] = wnv_down<E>(f);
+    }
     R r;
     __builtin_memcpy(&r, e, sizeof r);
     R* p = (R*)((char*)base + bytes);
@@ -198,42 +215,34 @@ template <typename E, int V, bool STREAM> __device__ __forceinline__ void store(
     else *p = r;
 }
 
-// The maps of a wave's rows joined in time (BACK: the last row first): of all of them, and of those before the own row.
-template <int LANES, bool BACK, bool SEG> __device__ __forceinline__ void join_rows(Map x, Map& all, Map& before) {
-    if constexpr (LANES == 16) {        // four rows: two exchanges of registers, no LDS
-        const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(x.p), __float_as_uint(x.p), false, false);     // rows 0 0 2 2 | 1 1 3 3
-        const auto u = __builtin_amdgcn_permlane16_swap(__float_as_uint(x.u), __float_as_uint(x.u), false, false);
-        const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x.b), __float_as_uint(x.b), false, false);
-        const Map even{__uint_as_float(p[0]), __uint_as_float(u[0]), __uint_as_float(b[0])};
-        const Map odd{__uint_as_float(p[1]), __uint_as_float(u[1]), __uint_as_float(b[1])};
-        const Map pair = BACK ? join<SEG>(odd, even) : join<SEG>(even, odd);
-        const auto pp = __builtin_amdgcn_permlane32_swap(__float_as_uint(pair.p), __float_as_uint(pair.p), false, false);  // rows 0 1 0 1 | 2 3 2 3
-        const auto pu = __builtin_amdgcn_permlane32_swap(__float_as_uint(pair.u), __float_as_uint(pair.u), false, false);
-        const auto pb = __builtin_amdgcn_permlane32_swap(__float_as_uint(pair.b), __float_as_uint(pair.b), false, false);
-        const Map low{__uint_as_float(pp[0]), __uint_as_float(pu[0]), __uint_as_float(pb[0])};
-        const Map high{__uint_as_float(pp[1]), __uint_as_float(pu[1]), __uint_as_float(pb[1])};
-        const int row = (threadIdx.x / LANES) & 3;
-        all = BACK ? join<SEG>(high, low) : join<SEG>(low, high);
-        before = (row & 1) != BACK ? (BACK ? odd : even) : NOTHING;
-        if ((row >> 1) != BACK) before = join<SEG>(BACK ? high : low, before);
-    } else {                            // each row joined to the one 1, 2, 4, ... rows before it
-        const auto moved = [](Map m, int d) {
-            return BACK ? Map{__shfl_down(m.p, d), __shfl_down(m.u, d), __shfl_down(m.b, d)}
-                        : Map{__shfl_up(m.p, d), __shfl_up(m.u, d), __shfl_up(m.b, d)};
-        };
-        const int row = BACK ? 63 / LANES - threadIdx.x % 64 / LANES : threadIdx.x % 64 / LANES;
-#pragma unroll
-        for (int d = LANES; d < 64; d *= 2) {
-            const Map other = moved(x, d);
-            if (row >= d / LANES) x = join<SEG>(other, x);
-        }
-        const int last = (BACK ? 0 : 64 - LANES) + threadIdx.x % LANES;
-        all = {__shfl(x.p, last), __shfl(x.u, last), __shfl(x.b, last)};
-        before = moved(x, LANES);
-        if (row == 0) before = NOTHING;
+// The maps of a quad's four stretches joined in time (BACK: the last one first): of all of them, and of those before the own one.
+template <int LANES> __device__ __forceinline__ void exchange(float x, int stride, float& low, float& high) {     // of two stretches that lie `stride` apart
+    if constexpr (LANES == 16) {        // two exchanges of registers, no LDS
+        const uint32_t w = __float_as_uint(x);
+        const auto r = stride == 1 ? __builtin_amdgcn_permlane16_swap(w, w, false, false) : __builtin_amdgcn_permlane32_swap(w, w, false, false);
+        low = __uint_as_float(r[0]);
+        high = __uint_as_float(r[1]);
+    } else {
+        const float other = __shfl_xor(x, stride * LANES);
+        const bool second = threadIdx.x / LANES & stride;
+        low = second ? other : x;
+        high = second ? x : other;
     }
 }
-
+template <int LANES> __device__ __forceinline__ void exchange(Map x, int stride, Map& low, Map& high) {
+    exchange<LANES>(x.p, stride, low.p, high.p);
+    exchange<LANES>(x.u, stride, low.u, high.u);
+    exchange<LANES>(x.b, stride, low.b, high.b);
+}
+template <int LANES, bool BACK, bool SEG> __device__ __forceinline__ void join_quad(Map x, Map& all, Map& before) {
+    Map even, odd, low, high;
+    exchange<LANES>(x, 1, even, odd);
+    exchange<LANES>(BACK ? join<SEG>(odd, even) : join<SEG>(even, odd), 2, low, high);
+    const int row = threadIdx.x / LANES & 3;
+    all = BACK ? join<SEG>(high, low) : join<SEG>(low, high);
+    before = (row & 1) != BACK ? (BACK ? odd : even) : NOTHING;
+    if ((row >> 1) != BACK) before = join<SEG>(BACK ? high : low, before);
+}
 // What a forward pass keeps of its stretch's steps for the second run over them.  float32: a and u v.  16-bit types: the smaller of a and u,
 // negative where that is u, next to v as it came; 16 registers less, which are a fourth wave per SIMD (bf16 8 x 24064 x 512: 172 us for
 // 178), and the arithmetic of wnv_blend.
@@ -291,6 +300,47 @@ template <bool BACK> __device__ __forceinline__ bool draw_place(const RecArgs& a
     return true;
 }
 
+template <bool BACK, bool SEG, int QUADS, int W> __device__ __forceinline__ Map block_of(const Map (&quads)[QUADS][W], int k, int ch) {
+    const Map a = quads[4 * k][ch], b = quads[4 * k + 1][ch], c = quads[4 * k + 2][ch], d = quads[4 * k + 3][ch];
+    return BACK ? join<SEG>(join<SEG>(d, c), join<SEG>(b, a)) : join<SEG>(join<SEG>(a, b), join<SEG>(c, d));
+}
+// The maps of a workgroup's quads joined to its chunk's, which the others get, to its blocks' where it has several, and to `prev`: of the
+// parts before each of its own; one channel.
+template <int W, int QUADS, bool BACK, bool SEG>
+__device__ __forceinline__ void join_blocks(const RecArgs& a, const Slots& slots, int order, int ch, const Map (&quads)[QUADS][W], Map (&blocks)[QUADS / 4][W],
+                                            Map (&prev)[QUADS / 4][W]) {
+    constexpr int BLOCKS = QUADS / 4;
+    const int last = (1 << a.part_bits) - 1, parts = BLOCKS >> a.part_bits;
+    Map all = NOTHING, own = NOTHING;
+#pragma unroll
+    for (int k = 0; k < BLOCKS; ++k) {
+        const int mine = BACK ? BLOCKS - 1 - k : k;
+        const Map block = block_of<BACK, SEG>(quads, mine, ch);
+        if (BLOCKS == 1) {
+            own = block;
+        } else {
+            blocks[mine][ch] = block;
+            own = k & last ? join<SEG>(own, block) : block;
+            if (parts > 1) {            // the only chunk
+                if ((k & last) == 0) prev[mine >> a.part_bits][ch] = all;
+                if ((k & last) == last) all = join<SEG>(all, handed_on<SEG>(own));
+            }
+        }
+    }
+    if (BLOCKS == 1 || parts == 1) prev[0][ch] = map_in_group<W, SEG>(slots, order, a.chunks, own);
+}
+// The state before a quad from that before its part, one channel.
+template <int W, int QUADS, bool BACK, bool SEG>
+__device__ __forceinline__ float state_before_quad(const RecArgs& a, const Map (&quads)[QUADS][W], const Map (&blocks)[QUADS / 4][W], int quad, int ch, float h) {
+    const int q = BACK ? QUADS - 1 - quad : quad, block = q / 4;
+    if (QUADS > 4)
+        for (int k = block >> a.part_bits << a.part_bits; k < block; ++k) h = apply<SEG>(blocks[BACK ? QUADS / 4 - 1 - k : k][ch], h);
+    const auto at = [&](int i) { return quads[BACK ? QUADS - 1 - 4 * block - i : 4 * block + i][ch]; };
+    Map before = NOTHING;
+    for (int i = 0; i < q % 4; ++i) before = join<SEG>(before, at(i));
+    return apply<SEG>(before, h);
+}
+
 // The number of a row's live steps.
 __device__ __forceinline__ int live_to(const RecArgs& a, int b) { return a.lengths ? max(0, min(a.lengths[b], a.T)) : a.T; }
 // The wave's entries of the map in one or two loads (asked for ahead of the data), a lane each; a stretch takes its 8 bits of a ballot.
@@ -325,10 +375,12 @@ template <int LANES, bool SEG> __device__ __forceinline__ int begins_in(const En
 // and reciprocals then overlap (bf16 8 x 24064 x 512 forward: 164 us, with the tests 185).
 template <typename E, int G, int V, int LANES, int WAVES, bool SEG, bool STREAM>
 __global__ void __launch_bounds__(64 * WAVES, WAVES > 4 ? 2 : sizeof(E) == 2 ? 4 : 3) wnv_recurrence_fwd(RecArgs a) {
-    constexpr int W = LANES * V, STEPS = Shape<LANES, WAVES>::STEPS;
-    __shared__ Map totals[WAVES][W], prev[W], groups[W];
+    typedef Shape<LANES, WAVES> S;
+    constexpr int W = LANES * V, STEPS = S::STEPS;
+    __shared__ Map quads[S::QUADS][W], blocks[S::BLOCKS][W], prev[S::BLOCKS][W], groups[W];
     __shared__ float base[W];
     const int tid = threadIdx.x, lane = tid % LANES, wave = tid / 64, at = lane * V;
+    const int quad = tid / (4 * LANES), part = quad / 4 >> a.part_bits, parts = S::BLOCKS >> a.part_bits;
     Place p;
     if (!draw_place<false>(a, W, p)) return;
     const int c = min(p.tile * W + at, a.C - V), n = live_to(a, p.b);
@@ -370,18 +422,18 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES > 4 ? 2 : sizeof(E) == 2 ? 4
     else reduce(std::false_type{});
     const bool any = SEG && __any(begins);
     const auto rows = [&](auto seg) {
-        constexpr bool S = decltype(seg)::value;
+        constexpr bool AT = decltype(seg)::value;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            if (S && begins) {          // the state of its last utterance, from nothing
+            if (AT && begins) {          // the state of its last utterance, from nothing
 #pragma unroll
                 for (int l = 0; l < L; ++l)
                     if (l < live) m[i].b = steps.run(l, i, begins >> l & 1 ? 0.f : m[i].b, v[l].get(i));
             }
-            finish<S>(m[i], begins);
+            finish<AT>(m[i], begins);
             Map all;
-            join_rows<LANES, false, S>(m[i], all, before[i]);
-            if (tid % 64 < LANES) totals[wave][at + i] = all;
+            join_quad<LANES, false, AT>(m[i], all, before[i]);
+            if (tid % (4 * LANES) < LANES) quads[quad][at + i] = all;
         }
     };
     if (any) rows(std::integral_constant<bool, SEG>{});
@@ -391,10 +443,7 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES > 4 ? 2 : sizeof(E) == 2 ? 4
     if (wave < 3 && ch < W) {
         const Slots slots = slots_at(a.slots, p.row, a.chunks, W, ch);
         if (wave == 0) {
-            Map all = totals[0][ch];
-#pragma unroll
-            for (int w = 1; w < WAVES; ++w) all = join<SEG>(all, totals[w][ch]);
-            prev[ch] = map_in_group<W, SEG>(slots, p.chunk, a.chunks, all);
+            join_blocks<W, S::QUADS, false, SEG>(a, slots, p.chunk, ch, quads, blocks, prev);
         } else if (wave == 1) {
             base[ch] = state_before_groups<W, SEG>(slots, p.chunk, a.h0 ? a.h0[p.b * a.h0b + min(p.tile * W + ch / V * V, a.C - V) + ch % V] : 0.f);
         } else {
@@ -404,13 +453,15 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES > 4 ? 2 : sizeof(E) == 2 ? 4
     __syncthreads();
 
     float h[V];
+    const int last_quad = parts > 1 ? (((a.T - 1) / BLOCK >> a.part_bits) + 1 << a.part_bits) * 4 - 1 : S::QUADS - 1;      // of the last part that is there
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        h[i] = apply<SEG>(prev[at + i], apply<SEG>(groups[at + i], base[at + i]));
-        if (a.saved && tid < LANES) a.saved[((long long)p.row * a.chunks + p.chunk) * W + at + i] = h[i];
-        for (int w = 0; w < wave; ++w) h[i] = apply<SEG>(totals[w][at + i], h[i]);
+        h[i] = apply<SEG>(prev[part][at + i], apply<SEG>(groups[at + i], base[at + i]));
+        if (a.saved && quad == part << a.part_bits + 2 && tid % (4 * LANES) < LANES)
+            a.saved[(((long long)p.row * a.chunks + p.chunk) * parts + part) * W + at + i] = h[i];
+        h[i] = state_before_quad<W, S::QUADS, false, SEG>(a, quads, blocks, quad, at + i, h[i]);
         h[i] = apply<SEG>(before[i], h[i]);
-        if (tid >= 64 * WAVES - LANES) {                   // the chunk's last stretch: the state behind it
+        if (quad == last_quad && tid % (4 * LANES) >= 3 * LANES) {      // its last stretch: the state behind it
             const float last = apply<SEG>(m[i], h[i]);
             if (ends_section(p.chunk, a.chunks))
                 publish<SEG>(slots_at(a.slots, p.row, a.chunks, W, at + i).section + (long long)(p.chunk / (GROUP * GROUP)) * W, {0.f, 1.f, last});
@@ -420,7 +471,7 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES > 4 ? 2 : sizeof(E) == 2 ? 4
     E* y = (E*)a.y + ((long long)p.b * a.T + (long long)p.chunk * STEPS) * a.C;
     const uint32_t to = (uint32_t)(tid / LANES * L * a.C + c) * (uint32_t)sizeof(E);
     const auto run = [&](auto full, auto seg) {
-        constexpr bool FULL = decltype(full)::value, S = decltype(seg)::value;
+        constexpr bool FULL = decltype(full)::value, AT = decltype(seg)::value;
 #pragma unroll
         for (int l = 0; l < L; ++l)
             if (FULL || t0 + l < a.T) {
@@ -429,7 +480,7 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES > 4 ? 2 : sizeof(E) == 2 ? 4
                 for (int i = 0; i < V; ++i) {
                     float q = 0.f;
                     if (FULL || l < live) {
-                        if (S && begins >> l & 1) h[i] = 0.f;
+                        if (AT && begins >> l & 1) h[i] = 0.f;
                         h[i] = steps.run(l, i, h[i], v[l].get(i));
                         q = h[i];
                         if (G == 3) q *= wnv_gate(o[l].get(i));
@@ -450,10 +501,12 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES > 4 ? 2 : sizeof(E) == 2 ? 4
 // forward pass saved before each chunk and is run through again.
 template <typename E, int G, int V, int LANES, int WAVES, bool SEG, bool STREAM>
 __global__ void __launch_bounds__(64 * WAVES, 2) wnv_recurrence_bwd(RecArgs a) {
-    constexpr int W = LANES * V, STEPS = Shape<LANES, WAVES>::STEPS;
-    __shared__ Map ahead[WAVES][W], back[WAVES][W], prev[W], groups[W];         // of h and of r
+    typedef Shape<LANES, WAVES> S;
+    constexpr int W = LANES * V, STEPS = S::STEPS;
+    __shared__ Map ahead[S::QUADS][W], back[S::QUADS][W], ahead_blocks[S::BLOCKS][W], back_blocks[S::BLOCKS][W], prev[S::BLOCKS][W], groups[W];      // of h and of r
     __shared__ float base[W];
     const int tid = threadIdx.x, lane = tid % LANES, wave = tid / 64, at = lane * V;
+    const int quad = tid / (4 * LANES), part = quad / 4 >> a.part_bits, parts = S::BLOCKS >> a.part_bits;
     Place p;
     if (!draw_place<true>(a, W, p)) return;
     const int order = a.chunks - 1 - p.chunk, c = min(p.tile * W + at, a.C - V), n = live_to(a, p.b);
@@ -480,7 +533,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) wnv_recurrence_bwd(RecArgs a) {
                 if (G == 3) o[l] = load<E, V, STREAM>(z + l * a.zt + 2 * a.C, from);
                 if (a.dy) d[l] = load<E, V, STREAM>(dy + l * a.dyt, dfrom);
             }
-        saved = load<float, V, false>(a.saved + ((long long)p.row * a.chunks + p.chunk) * W, at * 4);
+        saved = load<float, V, false>(a.saved + ((long long)p.row * a.chunks + p.chunk) * parts * W, (part * W + at) * 4);
         begins = begins_in<LANES, SEG>(entries, live);
 #pragma unroll
         for (int i = 0; i < V; ++i) m[i] = r[i] = NOTHING;
@@ -518,23 +571,23 @@ __global__ void __launch_bounds__(64 * WAVES, 2) wnv_recurrence_bwd(RecArgs a) {
         r[i].p = m[i].p;
         r[i].u = m[i].u;
         Map all, all_back;
-        join_rows<LANES, false, SEG>(m[i], all, h_before[i]);
-        join_rows<LANES, true, SEG>(r[i], all_back, r_before[i]);
-        if (tid % 64 < LANES) ahead[wave][at + i] = all, back[wave][at + i] = all_back;
+        join_quad<LANES, false, SEG>(m[i], all, h_before[i]);
+        join_quad<LANES, true, SEG>(r[i], all_back, r_before[i]);
+        if (tid % (4 * LANES) < LANES) ahead[quad][at + i] = all, back[quad][at + i] = all_back;
     }
     __syncthreads();
     const int ch = tid % 64;
-    if (wave < 3 && ch < W) {
+    if (wave < (S::BLOCKS > 1 ? 4 : 3) && ch < W) {
         const Slots slots = slots_at(a.slots, p.row, a.chunks, W, ch);
         if (wave == 0) {
-            Map all = back[WAVES - 1][ch];
-#pragma unroll
-            for (int w = WAVES - 2; w >= 0; --w) all = join<SEG>(all, back[w][ch]);
-            prev[ch] = map_in_group<W, SEG>(slots, order, a.chunks, all);
+            join_blocks<W, S::QUADS, true, SEG>(a, slots, order, ch, back, back_blocks, prev);
         } else if (wave == 1) {
             base[ch] = state_before_groups<W, SEG>(slots, order, a.dh_last ? a.dh_last[(long long)p.b * a.C + min(p.tile * W + ch / V * V, a.C - V) + ch % V] : 0.f);
-        } else {
+        } else if (wave == 2) {
             groups[ch] = map_of_groups<W, SEG>(slots, order);
+        } else {
+#pragma unroll
+            for (int k = 0; k < S::BLOCKS; ++k) ahead_blocks[k][ch] = block_of<false, SEG>(ahead, k, ch);
         }
     }
     __syncthreads();
@@ -543,9 +596,9 @@ __global__ void __launch_bounds__(64 * WAVES, 2) wnv_recurrence_bwd(RecArgs a) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         h[i] = saved.get(i);
-        x[i] = apply<SEG>(prev[at + i], apply<SEG>(groups[at + i], base[at + i]));
-        for (int w = 0; w < wave; ++w) h[i] = apply<SEG>(ahead[w][at + i], h[i]);
-        for (int w = WAVES - 1; w > wave; --w) x[i] = apply<SEG>(back[w][at + i], x[i]);
+        x[i] = apply<SEG>(prev[part][at + i], apply<SEG>(groups[at + i], base[at + i]));
+        h[i] = state_before_quad<W, S::QUADS, false, SEG>(a, ahead, ahead_blocks, quad, at + i, h[i]);
+        x[i] = state_before_quad<W, S::QUADS, true, SEG>(a, back, back_blocks, quad, at + i, x[i]);
         h[i] = apply<SEG>(h_before[i], h[i]);
         x[i] = apply<SEG>(r_before[i], x[i]);
         if (tid < LANES) {                              // the chunk's first stretch: what flows out of it
@@ -651,7 +704,7 @@ wnv_status launched(const char* who) {
 // tiles of 8 waves and 21 in wide ones, both passes 66 and 58; 64 x 512 x 512 both passes 179 and 134).
 constexpr int NARROW_CHANNELS = 32, LITTLE_CHANNELS = 256;
 constexpr int64_t LITTLE = 2 << 20;
-struct Cut { int V, lanes, waves, W, tiles, chunks; };
+struct Cut { int V, lanes, waves, W, tiles, chunks, part_bits, parts; };
 Cut cut_of(int64_t B, int64_t T, int C) {
     constexpr int WIDE = Shape<16, 4>::STEPS, NARROW = Shape<4, 4>::STEPS;
     Cut c;
@@ -665,6 +718,8 @@ Cut cut_of(int64_t B, int64_t T, int C) {
     c.W = c.lanes * c.V;
     c.tiles = (C + c.W - 1) / c.W;
     c.chunks = (int)((T + steps - 1) / steps);
+    c.part_bits = C <= NARROW_CHANNELS ? 2 : 0;
+    c.parts = steps / BLOCK >> c.part_bits;
     return c;
 }
 
@@ -684,7 +739,7 @@ int64_t slot_bytes(int64_t B, const Cut& c) { return c.chunks > 1 ? B * c.tiles 
 // The kernel's arguments; the workspace is filled on the way.
 wnv_status prepare(const char* who, const wnv_recurrence_args* a, const Cut& c, RecArgs& k) {
     k.B = a->B; k.C = a->C; k.T = (int)a->T;
-    k.tiles = c.tiles; k.chunks = c.chunks;
+    k.tiles = c.tiles; k.chunks = c.chunks; k.part_bits = c.part_bits;
     k.zb = a->z_batch_stride; k.zt = a->T > 1 ? a->z_time_stride : 0; k.h0b = a->h0_batch_stride;
     k.z = a->z; k.h0 = a->h0; k.lengths = a->lengths; k.seg_start = a->seg_start;
     k.y = a->y; k.h_last = a->h_last; k.saved = (float*)a->saved; k.slots = (unsigned long long*)a->workspace;
@@ -739,7 +794,7 @@ template <typename E> void launch(bool back, const wnv_recurrence_args* a, const
 extern "C" int64_t wnv_recurrence_saved_bytes(int32_t B, int64_t T, int32_t C, int32_t gates, int32_t dtype) {
     if (check_shape("wnv_recurrence_saved_bytes", 0, B, T, C, gates, dtype) != WNV_OK) return -1;
     const Cut c = cut_of(B, T, C);
-    return (int64_t)B * c.tiles * c.chunks * c.W * 4;
+    return (int64_t)B * c.tiles * c.chunks * c.parts * c.W * 4;
 }
 
 extern "C" int64_t wnv_recurrence_workspace_bytes(int32_t B, int64_t T, int32_t C, int32_t gates, int32_t dtype) {
