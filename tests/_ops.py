@@ -172,8 +172,16 @@ def check_blend(got, f, h, v):
 # and the same from the end for dh.  The products behind them: y = h sigmoid(o), dv = dh u, df = dh (h_{t-1} - v) a u, do = dy h so (1 - so), add
 # their gates' deltas and an eps an operation (of t h - t v, t = a u, by the magnitudes).  1.01 for what is quadratic, TINY M for gates that
 # read as 0.
-def local_scan(z, h0=None, output_gate=True, lengths=None, seg_start=None, dy=None, dh_last=None):
+#
+# Long sequences of gates that remember (`long`) need less than delta a step.  A stretch keeps P = 1 - U of the state: off by eps of itself for
+# the subtraction and, U being a sum of its 8 u with at most 16 roundings each, by U (delta + 16 eps); a block of 128 steps, which takes its
+# P from 1 - U again, multiplies 16 such P by 15 products: within 31 eps, and U (delta + 30 eps) with the 14 roundings of its sums.  That is
+# eps / 4 a step and u (delta + 30 eps); the joins of chunks, groups and sections behind it are fewer than one in 128 steps.  P >= 1/2 there:
+# twice that, relative to P, so a step loses no more than 2 u (delta + 30 eps) + eps / 2, or delta + 3 eps as above.  The constant is 128 eps:
+# within its own stretch a state has gone through up to 8 steps of a h + u v, 5 eps each.
+def local_scan(z, h0=None, output_gate=True, lengths=None, seg_start=None, dy=None, dh_last=None, long=False):
     """(exact results, their bounds), float64 on the CPU step by step: dicts of y, h_last and, where dy is given, dz and dh0."""
+    FIXED = (128 if long else 64) * EPS
     z = z.detach().double().cpu().numpy()
     B, T, n = z.shape
     C = n // (3 if output_gate else 2)
@@ -190,15 +198,16 @@ def local_scan(z, h0=None, output_gate=True, lengths=None, seg_start=None, dy=No
     h = np.zeros((B, C)) if h0 is None else h0.detach().double().cpu().numpy().copy()
     M = max(np.abs(v).max(), np.abs(h).max())
     keep = np.where(live[..., None], np.where(begins[..., None], 0.0, a), 1.0)
-    new, loss = np.where(live[..., None], u * v, 0.0), np.where(live[..., None], K, 0.0)
+    new, own = np.where(live[..., None], u * v, 0.0), np.where(live[..., None], K, 0.0)
+    loss = np.where(live[..., None], np.minimum(K, 2 * u * (delta(f) + 30 * EPS) + EPS / 2), 0.0) if long else own
     hs, ms, ds = np.empty((T + 1, B, C)), np.empty((T + 1, B, C)), np.empty((T + 1, B, C))
     hs[0], ms[0], ds[0] = h, np.abs(h), 0
     for t in range(T):
-        k, l, w = keep[:, t], loss[:, t], new[:, t]
+        k, l, w, o = keep[:, t], loss[:, t], new[:, t], own[:, t]
         hs[t + 1] = k * hs[t] + w
         ms[t + 1] = k * ms[t] + np.abs(w)
-        ds[t + 1] = k * (ds[t] + l * ms[t]) + np.abs(w) * l
-    hs, ms, eh = (x.transpose(1, 0, 2) for x in (hs, ms, 1.01 * (ds + 64 * EPS * ms) + 8 * TINY * M))
+        ds[t + 1] = k * (ds[t] + l * ms[t]) + np.abs(w) * o
+    hs, ms, eh = (x.transpose(1, 0, 2) for x in (hs, ms, 1.01 * (ds + FIXED * ms) + 8 * TINY * M))
     o = z[..., 2 * C:] if output_gate else None
     so, do = (sig(o), delta(o)) if output_gate else (np.ones((B, T, C)), np.zeros((B, T, C)))
     L = live[..., None]
@@ -216,7 +225,7 @@ def local_scan(z, h0=None, output_gate=True, lengths=None, seg_start=None, dy=No
             mb[:, t] = np.abs(gt) + mr
             db[:, t] = (do[:, t] + 2 * EPS) * np.abs(gt) + dr
             r, mr, dr = k * dh[:, t], k * mb[:, t], k * (db[:, t] + l * mb[:, t])
-        eb = 1.01 * (db + 64 * EPS * mb) + 8 * TINY * S
+        eb = 1.01 * (db + FIXED * mb) + 8 * TINY * S
         before, mbe, ebe = (np.where(begins[..., None], 0, x[:, :-1]) for x in (hs, ms, eh))
         t, K2 = a * u, 2 * delta(f) + 6 * EPS
         dz = [dh * (before - v) * t, dh * u]
@@ -226,7 +235,7 @@ def local_scan(z, h0=None, output_gate=True, lengths=None, seg_start=None, dy=No
             dz.append(dy * hs[:, 1:] * so1)
             bz.append(np.abs(dy) * so1 * (eh[:, 1:] + (2 * do + 6 * EPS) * ms[:, 1:]))
         want.update(dz=np.concatenate([np.where(L, x, 0) for x in dz], -1), dh0=r)
-        bound.update(dz=np.concatenate([np.where(L, 1.01 * x + 8 * TINY * M * S, 0) for x in bz], -1), dh0=1.01 * (dr + 64 * EPS * mr) + 8 * TINY * S)
+        bound.update(dz=np.concatenate([np.where(L, 1.01 * x + 8 * TINY * M * S, 0) for x in bz], -1), dh0=1.01 * (dr + FIXED * mr) + 8 * TINY * S)
     return tuple({k: torch.from_numpy(np.ascontiguousarray(x)) for k, x in d.items()} for d in (want, bound))
 
 

@@ -621,3 +621,28 @@ def test_a_rows_bits_do_not_depend_on_its_batch_at_any_length(shape, dtype, kind
         part = run(z[b:b + n], h0[b:b + n], dy[b:b + n], dh[b:b + n], 3, {k: v[b:b + n] for k, v in m.items()})
         for k in all_:
             assert torch.equal(part[k], all_[k][b:b + n]), (k, b)
+
+
+# Chunks of 128 steps (512 of rows up to 32 channels), groups of 16 chunks, sections of 16 groups: from chunk 144 on a chunk takes the maps of its
+# section's groups 8 and up, from chunk 256 on a state that a section handed out, from 512 on one that had another's before it.
+LONG = [(1, 20000, 33), (2, 33000, 40), (1, 70000, 36), (1, 80000, 20), (2, 135000, 5), (1, 270000, 2)]
+
+
+@pytest.mark.parametrize("kind", ["full", "ends"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("shape", LONG, ids=lambda s: "x".join(map(str, s)))
+def test_long_sequences_against_the_definition(shape, dtype, kind):
+    """Every level of the hand-over between chunks, with gates that remember 8000 steps, so that each is seen far behind it."""
+    B, T, C = shape
+    z, h0, dy, dh = inputs(B, T, C, 2, torch.float32, seed=T)
+    z[..., :C] = 9.0 + 0.1 * z[..., :C]
+    z[..., C:] += 1.0
+    z, dy = z.to(DTYPES[dtype]), dy.to(DTYPES[dtype])
+    h0, dh = 30 * h0, 30 * dh
+    m = {}
+    if kind == "ends":                  # a length inside the last chunks, utterances that begin on both sides of the hand-overs
+        start = torch.full((B, T), -1, dtype=torch.int32)
+        for at in (T // 3, T // 2 + 1, T - 700):
+            start[:, at:] = at
+        m = dict(lengths=torch.full((B,), T - 300, dtype=torch.int32), seg_start=start)
+    check_local(run(z, h0, dy, dh, 2, m), local_scan(z, h0, False, dy=dy, dh_last=dh, long=True, **m))
