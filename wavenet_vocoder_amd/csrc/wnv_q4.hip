@@ -351,9 +351,11 @@ __global__ void __launch_bounds__(NT == 1 ? 1024 : 512) wnv_q4_rows(Q4Dev q, Q4C
 
 // Which form runs (us a launch in a graph, both sides measured):
 //  * x through LDS if its rows fit (two workgroups a CU then) and it pays: float32, whose three parts become columns of one product
-//    (1 x 8192 x 8192: 11.6, from L2 23.4; 8 x 512 x 3 512 with the step: 4.4 and 5.4) -- at most 5 rows a workgroup --, and 16-bit
-//    types if a wave has several blocks of inputs to wait for (1 x 8192 x 8192 bf16: 11.1 and 13.2; 8 x 1616 x 512, one block a wave:
-//    4.6 and 3.9).
+//    (1 x 8192 x 8192: 11.6, from L2 23.4; 8 x 512 x 3 512 with the step: 4.4 and 5.4) -- at most 5 rows a workgroup, so that many rows
+//    read the weights more often: as long as that is no more than two workgroups a CU (through LDS and from L2, 512 of them: 5 x 2048 x 8192
+//    6.7 and 7.4, 16 x 2048 x 2048 6.7 and 7.2; more: 6 x 2048 x 8192 9.9 and 7.5, 64 x 2048 x 2048 17.5 and 9.1, 64 x 512 x 8192 16.8 and
+//    9.7), and with the step always (24 x 2048 x 3 2048 13.6 and 16.1, 64 x 2048 x 3 2048 27.7 and 28.6) --, and 16-bit types if a wave
+//    has several blocks of inputs to wait for (1 x 8192 x 8192 bf16: 11.1 and 13.2; 8 x 1616 x 512, one block a wave: 4.6 and 3.9).
 //  * else two tiles a wave, which halves what is read of x, as soon as single tiles would be more workgroups than CUs (bf16
 //    64 x 4096 x 4096: 15.5 and 19.6, 48 x 2048 x 2048: 5.3 and 6.6; with fewer, 16 x 2048 x 2048: 5.0 and 4.4), and 8 waves of
 //    two slices, whose registers have room for it (64 x 8192 x 8192: bf16 40 and 47 with 16 waves, float32 83 and 106).
@@ -374,7 +376,9 @@ template <typename E, int GATES> void launch(const Q4Dev& q, const Q4Call& a, hi
     const int slices = GATES == 0 ? 16 : GATES == 2 ? 8 : 4;    // a workgroup is 16 waves at most, 12 with three gates
     const int split = std::min(slices, q.kb), most = 16 / PARTS;
     const size_t staged = (size_t)PARTS * std::min(a.B, most) * (16 * q.kb + 1) * 16;
-    if (staged <= STAGE_MOST && (PARTS == 3 || (a.B <= 16 && q.kb > split))) return launch<E, 1, GATES, true>(q, a, split, split, most, staged, s);
+    const int64_t passes = (a.B + most - 1) / most;
+    const bool pays = PARTS == 3 ? GATES || q.gates * q.tiles * passes <= 2 * CUS : a.B <= 16 && q.kb > split;
+    if (staged <= STAGE_MOST && pays) return launch<E, 1, GATES, true>(q, a, split, split, most, staged, s);
     if constexpr (!GATES) {
         if ((int64_t)q.gates * q.tiles * ((a.B + 15) / 16) > CUS) return launch<E, 2, GATES, false>(q, a, split, std::min(split, 8), 16, 0, s);
     }
