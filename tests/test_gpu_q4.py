@@ -275,3 +275,24 @@ def test_recurrence_step_with_gates_at_both_ends(dtype, gates, B):
     for row in state:
         check_blend(row, f, h, v)
     assert torch.equal(y, (state * (0.5 if gates == 3 else 1.0)).to(y.dtype))
+
+
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+@pytest.mark.parametrize("group", [32, 128])
+@pytest.mark.parametrize("shape", [(1, 300, 40), (4, 128, 16), (40, 257, 33), (5, 2100, 20)], ids=lambda s: "x".join(map(str, s)))
+def test_finite_inputs_of_any_size(shape, group, dtype):
+    """Rows next to the largest number of their type: what is summed on the way overflows where the result does, not before it."""
+    B, cin, cout = shape
+    codes, scales, zp = random_q4(cout, cin, group, 3)
+    scales = (scales.float() * 2.0 ** -10).to(torch.bfloat16)
+    q = Q4Linear(cin, cout, "cuda", group_size=group)
+    q.set_codes(codes.cuda(), scales.cuda(), zp.cuda())
+    g = torch.Generator().manual_seed(B)
+    sign = torch.where(torch.rand(B, cin, generator=g) < 0.5, -1.0, 1.0)
+    x = (sign * (0.5 + 0.5 * torch.rand(B, cin, generator=g)) * float(torch.finfo(DTYPES[dtype]).max)).to(DTYPES[dtype])
+    x[0] = x[0].abs()
+    parts = (codes, scales, zp, None)
+    want = exact(x, parts, group)
+    assert torch.isfinite(x).all()
+    assert float(want.abs().max()) < float(torch.finfo(DTYPES[dtype]).max)
+    check(q.step(x.cuda()), x, parts, group)

@@ -3,9 +3,10 @@
 //
 // The matrix instruction does the dot products, with the weights as its rows and up to 16 rows of x as its columns, so that a code
 // costs a shift and an and-or per pair, and not an operation per code and row of x: a 16-bit float 16 + code is a mask and a constant
-// away from the code (bf16: 0x4180 | code << 3, f16: 0x4c00 | code << 6), exact, and a second instruction with -(16 + zero) in every
-// place takes the offset out again: the sum of x (code - zero) over a group, in float32, which the group's scale then joins to the
-// rest.  float32 x is cut into three bf16 parts that add up to it exactly; they share the weights.
+// away from the code (f16: 0x4c00 | code << 6; bf16, times 2^-12: 0x3b80 | code << 3), exact, and a second instruction with -(16 + zero) in
+// every place takes the offset out again: the sum of x (code - zero) over a group, in float32, which the group's scale then joins to the
+// rest.  float32 x is cut into three bf16 parts that add up to it exactly; they share the weights.  (The 2^-12 is taken out at the end: 128
+// products of up to 31 x stay below 2^12 x, which may be the type's largest number.)
 //
 // Weights are laid out once, in tiles of 16 rows x 128 inputs: lane l of a wave holds row l % 16 and, in word j of its 16 bytes, the
 // inputs 32 j + 8 (l / 16) ... + 7 of the tile -- what a 16 x 16 x 32 matrix instruction wants of a lane.  Inputs 2p and 2p + 1 of a
@@ -135,8 +136,8 @@ typedef u32x4 u32x4_any __attribute__((aligned(1)));
 
 // What the kernels need to know of x's type: the 16-bit float that its products run in, and how many parts of that make one x.
 template <typename E> struct Q4Type;
-template <> struct Q4Type<wnv_bf16> { static constexpr int PARTS = 1, AT = 3; static constexpr uint32_t ONE = 0x4180u; };
-template <> struct Q4Type<wnv_f16> { static constexpr int PARTS = 1, AT = 6; static constexpr uint32_t ONE = 0x4c00u; };
+template <> struct Q4Type<wnv_bf16> { static constexpr int PARTS = 1, AT = 3; static constexpr uint32_t ONE = 0x3b80u; static constexpr float UP = 4096.f; };
+template <> struct Q4Type<wnv_f16> { static constexpr int PARTS = 1, AT = 6; static constexpr uint32_t ONE = 0x4c00u; static constexpr float UP = 1.f; };
 template <> struct Q4Type<float> : Q4Type<wnv_bf16> { static constexpr int PARTS = 3; };
 
 template <typename E> __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
@@ -146,7 +147,7 @@ template <typename E> __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f3
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// The 8 codes of a word as 16 + code, in the order of x's memory.
+// The 8 codes of a word as 16 + code (over UP), in the order of x's memory.
 template <typename E> __device__ __forceinline__ u32x4 codes_up(uint32_t w) {
     constexpr int AT = Q4Type<E>::AT;
     constexpr uint32_t MASK = 0x000f000fu << AT, ONE = Q4Type<E>::ONE * 0x10001u;
@@ -158,7 +159,7 @@ template <typename E> __device__ __forceinline__ u32x4 codes_up(uint32_t w) {
     }
     return r;
 }
-template <typename E> __device__ __forceinline__ u32x4 offset_of(uint32_t zero) {        // -(16 + zero), 8 times
+template <typename E> __device__ __forceinline__ u32x4 offset_of(uint32_t zero) {        // -(16 + zero) (over UP), 8 times
     const uint32_t h = (zero << Q4Type<E>::AT) | Q4Type<E>::ONE | 0x8000u, w = h | h << 16;
     return u32x4{w, w, w, w};
 }
@@ -328,7 +329,7 @@ __global__ void __launch_bounds__(NT == 1 ? 1024 : 512) wnv_q4_rows(Q4Dev q, Q4C
                 const float* one = part + at + (g * split + w) * (NT * SUMS * 256);
                 sum += PARTS == 3 ? one[0] + one[apart] + one[2 * apart] : one[0];
             }
-            z[g] = sum + q.bias[(tile + g * q.tiles) * 16 + n];
+            z[g] = fmaf(sum, Q4Type<E>::UP, q.bias[(tile + g * q.tiles) * 16 + n]);
         }
         if (!GATES) {
             ((E*)a.y)[((long long)row * q.gates + gate) * q.rows + channel] = wnv_down<E>(z[0]);
