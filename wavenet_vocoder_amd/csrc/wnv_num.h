@@ -14,20 +14,21 @@ template <typename E> __device__ __forceinline__ float wnv_up(E x) { return (flo
 // one rounding to nearest even, of a value computed in 32 bits
 template <typename E> __device__ __forceinline__ E wnv_down(float x) { return (E)x; }
 
-// sigmoid(x) = 1 / (1 + exp(-x)), by the hardware's base-2 exponential and reciprocal (an ulp each): to a few ulps of itself at both
-// ends, so that 1 - sigmoid(f), taken as sigmoid(-f), is as exact next to 0 as sigmoid(f) (1 - sigmoid(f) would leave it 2^-24
-// absolute: at f = 9, 5e-4 of it).  exp overflows to infinity, whose reciprocal is the right 0; a NaN passes.
+// sigmoid(x) = 1 / (1 + exp(-x)), by the hardware's base-2 exponential and reciprocal, an ulp each.  x log2(e) is rounded to 24 bits before
+// that, so that next to 0 the result is within (1.5 |x| + 8) 2^-24 of itself: 11 ulps at x = -9, 64 at -80, and below 2^-126 it may
+// read as 0.  1 - sigmoid(f), taken as sigmoid(-f), is that exact too (1 - sigmoid(f) would leave it 2^-24 absolute: at f = 9, 5e-4 of it).
+// exp overflows to infinity, whose reciprocal is the right 0; a NaN passes.
 __device__ __forceinline__ float wnv_gate(float x) {
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -1.44269504088896340736f));
 }
-// The same, and sigmoid(x) (1 - sigmoid(x)) = e / (1 + e)^2 with e = exp(-|x|) <= 1: exact at both ends too, no overflow.
+// The same, and sigmoid(x) (1 - sigmoid(x)) = e / (1 + e)^2 with e = exp(-|x|) <= 1: as exact, at both ends, no overflow.
 __device__ __forceinline__ float wnv_gate(float x, float& slope) {
     const float e = __builtin_amdgcn_exp2f(fabsf(x) * -1.44269504088896340736f);
     const float r = __builtin_amdgcn_rcpf(1.0f + e), er = e * r;
     slope = er * r;
     return x >= 0.f ? r : er;
 }
-// sigmoid(f), and u = 1 - sigmoid(f) = sigmoid(-f), each to its own precision.
+// sigmoid(f), and u = 1 - sigmoid(f) = sigmoid(-f), each as exact as above.
 __device__ __forceinline__ float wnv_gates(float f, float& u) {
     const float e = __builtin_amdgcn_exp2f(fabsf(f) * -1.44269504088896340736f);
     const float more = __builtin_amdgcn_rcpf(1.0f + e), less = e * more;
