@@ -351,11 +351,14 @@ WNV_API wnv_status wnv_logmel(wnv_mel_handle h, const wnv_logmel_args* args);
  * of a padded batch end at lengths[b]: behind it z is not looked at, y and the gradients are zero and the state is handed on, so
  * h_last is the state behind the last real step (h0 for an empty row).  lengths are taken as min(max(lengths[b], 0), T).
  * The maps live in device memory and are not range-checked further: any value of seg_start other than t just does not begin one.
- * Infinite gates are their limits (f = inf keeps the state, f = -inf replaces it, o = -inf gives 0); an infinite v makes the rest of
- * its utterance NaN.
+ * Infinite gates are their limits (f = inf keeps the state, f = -inf replaces it, o = -inf gives 0), of finite states and inputs; an
+ * infinite v or h0 leaves the rest of its utterance infinite or NaN, and is handed on as it is where there is nothing left to do.
+ * sigmoid(f) and 1 - sigmoid(f) are each within (1.5 |f| + 8) 2^-24 of themselves; below 2^-126 they may read as 0.
  * No atomics on data: the same call gives the same bits, and a row's bits do not depend on the rows beside it.
  * Everything a call needs beyond its arguments is in `workspace`, which the call writes before it reads: calls that may run at the same
- * time (other streams, graphs replayed side by side) each have their own. */
+ * time (other streams, graphs replayed side by side) each have their own.  Parts of a sequence wait for each other on the device, for
+ * parts that have started only; should one of them not answer for some seconds all the same, the kernel ends, and what depends on
+ * that part is NaN.  The status is that of the launch: it does not tell. */
 typedef enum wnv_dtype { WNV_F32 = 0, WNV_BF16 = 1, WNV_F16 = 2 } wnv_dtype;
 struct wnv_recurrence_args {
     int32_t B, C;
@@ -395,14 +398,16 @@ WNV_API wnv_status wnv_recurrence_step(int32_t device, const void* z, int64_t z_
  *     W[n][k] = scale[n][k / group] (code[n][k] - zero[n][k / group]),    group 32, 64 or 128 inputs, the last one may be short.
  * Scales are bf16; x and y have the call's dtype, sums are float32.  gates > 1: the outputs are that many gates of cout / gates
  * channels, as the recurrence above takes them.  Setting weights waits for the device; after that a handle is only read, from any
- * number of streams at once.  An infinite or NaN input makes the outputs of its own row NaN. */
+ * number of streams at once.  Finite inputs of any size are summed without overflow; float32 and bf16 ones below 2^-100 may lose
+ * digits.  An infinite or NaN input makes the outputs of its own row NaN. */
 typedef struct wnv_q4* wnv_q4_handle;
 WNV_API wnv_status wnv_q4_create(int32_t cin, int32_t cout, int32_t gates, int32_t group, int32_t device, wnv_q4_handle* out);
 /* All device memory: codes (cout, cin) one per byte, scales bf16 (cout, ceil(cin / group)), zeros the same shape or NULL (8),
- * bias float32 (cout) or NULL.  A code or zero point over 15: WNV_ERR_INVALID_ARG. */
+ * bias float32 (cout) or NULL.  A code or zero point over 15: WNV_ERR_INVALID_ARG, and the handle has no weights until they are set. */
 WNV_API wnv_status wnv_q4_set_codes(wnv_q4_handle h, const uint8_t* codes, const void* scales, const uint8_t* zeros, const float* bias,
                             void* stream);
-/* weight device float32 (cout, cin), rounded here: asymmetric, a 15th of each group's range (widened to hold 0) as its scale. */
+/* weight device float32 (cout, cin), rounded here: asymmetric, a 15th of each group's range (widened to hold 0) as its scale.  A weight
+ * that is not finite or over 3e38: WNV_ERR_INVALID_ARG, as above. */
 WNV_API wnv_status wnv_q4_set_weights(wnv_q4_handle h, const float* weight, const float* bias, void* stream);
 WNV_API wnv_status wnv_q4_dequantise(wnv_q4_handle h, float* weight, void* stream);      /* device float32 (cout, cin) = W */
 WNV_API wnv_status wnv_q4_step(wnv_q4_handle h, const void* x, int64_t x_row_stride, void* y, int32_t B, int32_t dtype, void* stream);

@@ -448,7 +448,7 @@ static wnv_status q4_pack(wnv_q4* h, const uint8_t* codes, const wnv_bf16* scale
     int found = 0;
     HIP_TRY(hipMemcpyAsync(&found, bad, sizeof found, hipMemcpyDeviceToHost, s));
     HIP_TRY(hipStreamSynchronize(s));
-    if (found) return fail(WNV_ERR_INVALID_ARG, "wnv_q4: a code or zero point is over 15, or a weight is not finite");
+    if (found) return fail(WNV_ERR_INVALID_ARG, "wnv_q4: a code or zero point is over 15, or a weight is not finite or over 3e38");
     h->loaded = true;
     return WNV_OK;
 }

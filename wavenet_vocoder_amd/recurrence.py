@@ -149,7 +149,8 @@ def gated_recurrence(z: torch.Tensor, h0: Optional[torch.Tensor] = None, *, outp
     is not looked at, y and the gradients are zero, and the state is handed on (an empty row's is ``h0``).  ``seg_start`` (B, T): the
     map of a packed slot (``wnv_generate_args``) -- the state reads as zero at each step t with ``seg_start[b, t] == t``; a negative
     entry is an utterance begun before this call, which goes on from ``h0``.  Differentiable (once, not in forward mode) in z and h0.
-    Runs on the current stream of z's device and is capturable; the same call gives the same bits, and a row's do not depend on its batch."""
+    Runs on the current stream of z's device and is capturable; the same call gives the same bits, and a row's do not depend on its batch.
+    Parts of a long sequence wait for each other on the device; should one not answer for seconds, what depends on it is NaN."""
     refuse_tangents("gated_recurrence", z, h0)
     require_gpu_tensor(z, "z")
     _dtype(z)
