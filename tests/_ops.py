@@ -3,11 +3,12 @@
 Bounds, M = max(|v|, |h0|), S = max|dh|, u = 1 - sigmoid(f), eps = 2^-24 (half a step of float32):
   * a gate is off by at most delta = (1.5 |f| + 8) eps of itself, next to 0 and next to 1: the exponent f log2(e) is rounded (|f| eps at
     most, 1.5 with the change of base), exp2 and the reciprocal are within an ulp, and three more operations follow;
-  * h is a convex combination of the v and h0, so |h| <= M.  h_t = h + u (v - h) rounds three times (3 eps 2 M at most) and carries
-    u delta 2 M of the gate; an older error shrinks by 1 - u per step: at most 1 / u_min or T of them live at a time.  Maps of whole
-    stretches h -> h + (B - U h) round as often again when they are joined.  So |h - exact| <= k M with
-    k = 2 delta + 12 eps min(T, 1 / u_min) + 12 eps;
-  * dh_t = s, what goes back is s - u s: the same recursion with S in place of M, |dh - exact| <= k S;
+  * h is a convex combination of the v and h0, so |h| <= M.  A step a h + u v rounds twice (2 eps M) and carries delta of a h and of u v, of
+    which an older share shrinks by 1 - u per step: at most N = 1 / u_min or T of them live at a time, 2 eps M N for the roundings and
+    2 delta M for the gates, whose shares u v add up to M and whose shares a h are held as 1 - U over stretches.  The joins of stretches,
+    quads, blocks, chunks, groups and sections round a state no more than 40 times on its way, a few eps of M each; where N < 8, next to
+    nothing of it is left behind the first of them, and else 40 < 10 N.  So |h - exact| <= k M with k = 2 delta + 12 eps N + 12 eps;
+  * dh_t = s, what goes back is a s: the same recursion with S in place of M, |dh - exact| <= k S;
   * df = dh (h_{t-1} - v) sigmoid(f) u: k S 2 M + S k M + S 2 M (2 delta + 4 eps), times sigmoid(f) u <= 1/4: within k S M;
     dv = dh u: (k + delta + eps) S <= 2 k S;  do = dy h sigmoid(o)(1 - sigmoid(o)): (k M + M (2 delta + 4 eps)) |dy| / 4 <= k M |dy|.
   * the result's own type rounds by finfo.eps / 2 of the value (half a step of the smallest number near zero)."""
