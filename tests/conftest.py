@@ -14,8 +14,15 @@ def pytest_configure(config):
 
 def pytest_collection_modifyitems(config, items):
     """A gpu-marked test on a box without a GPU is an error of selection, not a skip-to-green:
-    only deselect it when the user did not ask for gpu tests explicitly."""
+    only deselect it when the user did not ask for gpu tests explicitly.
+
+    Where the built reference is missing, the GPU tests that run it fail; they come last then, so that a run that stops at its first
+    failure has run everything else."""
     import torch
+
+    from oracle import reference
+    if not reference.available():
+        items.sort(key=lambda item: item.path.name in ("test_gpu_graft_reference.py", "test_gpu_vs_reference.py"))
     if torch.cuda.is_available():
         return
     markexpr = config.getoption("-m") or ""
