@@ -305,9 +305,9 @@ template <bool BACK, bool SEG, int QUADS, int W> __device__ __forceinline__ Map 
     return BACK ? join<SEG>(join<SEG>(d, c), join<SEG>(b, a)) : join<SEG>(join<SEG>(a, b), join<SEG>(c, d));
 }
 // The maps of a workgroup's quads joined to its chunk's, which the others get, to its blocks' where it has several, and to `prev`: of the
-// parts before each of its own; one channel.
+// parts before each of its own; one channel.  Returns the chunk's.
 template <int W, int QUADS, bool BACK, bool SEG>
-__device__ __forceinline__ void join_blocks(const RecArgs& a, const Slots& slots, int order, int ch, const Map (&quads)[QUADS][W], Map (&blocks)[QUADS / 4][W],
+__device__ __forceinline__ Map join_blocks(const RecArgs& a, const Slots& slots, int order, int ch, const Map (&quads)[QUADS][W], Map (&blocks)[QUADS / 4][W],
                                             Map (&prev)[QUADS / 4][W]) {
     constexpr int BLOCKS = QUADS / 4;
     const int last = (1 << a.part_bits) - 1, parts = BLOCKS >> a.part_bits;
@@ -328,17 +328,35 @@ __device__ __forceinline__ void join_blocks(const RecArgs& a, const Slots& slots
         }
     }
     if (BLOCKS == 1 || parts == 1) prev[0][ch] = map_in_group<W, SEG>(slots, order, a.chunks, own);
+    return own;
 }
-// The state before a quad from that before its part, one channel.
-template <int W, int QUADS, bool BACK, bool SEG>
-__device__ __forceinline__ float state_before_quad(const RecArgs& a, const Map (&quads)[QUADS][W], const Map (&blocks)[QUADS / 4][W], int quad, int ch, float h) {
-    const int q = BACK ? QUADS - 1 - quad : quad, block = q / 4;
+// The last chunk of a section hands out the state behind it as soon as it knows the one before it; one channel.
+template <int W, bool SEG>
+__device__ __forceinline__ void hand_out_section(const RecArgs& a, int row, int order, int ch, Map chunk, Map prev, Map groups, float base) {
+    const float behind = apply<SEG>(chunk, apply<SEG>(prev, apply<SEG>(groups, base)));
+    publish<SEG>(slots_at(a.slots, row, a.chunks, W, ch).section + (long long)(order / (GROUP * GROUP)) * W, {0.f, 1.f, behind});
+}
+// The state before a quad from that before its part, a lane's channels from ch on.  The quads' maps are all asked for before the first is used
+// (2 x 300 x 128 float32 forward 8.1 us; one after the other 8.7).
+template <int W, int V, int QUADS, bool BACK, bool SEG>
+__device__ __forceinline__ void state_before_quad(const RecArgs& a, const Map (&quads)[QUADS][W], const Map (&blocks)[QUADS / 4][W], int quad, int ch, float (&h)[V]) {
+    const int q = BACK ? QUADS - 1 - quad : quad, block = q / 4, in = q % 4;
     if (QUADS > 4)
-        for (int k = block >> a.part_bits << a.part_bits; k < block; ++k) h = apply<SEG>(blocks[BACK ? QUADS / 4 - 1 - k : k][ch], h);
-    const auto at = [&](int i) { return quads[BACK ? QUADS - 1 - 4 * block - i : 4 * block + i][ch]; };
-    Map before = NOTHING;
-    for (int i = 0; i < q % 4; ++i) before = join<SEG>(before, at(i));
-    return apply<SEG>(before, h);
+        for (int k = block >> a.part_bits << a.part_bits; k < block; ++k)
+#pragma unroll
+            for (int c = 0; c < V; ++c) h[c] = apply<SEG>(blocks[BACK ? QUADS / 4 - 1 - k : k][ch + c], h[c]);
+    Map three[3][V];
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+#pragma unroll
+        for (int c = 0; c < V; ++c) three[i][c] = quads[BACK ? QUADS - 1 - 4 * block - i : 4 * block + i][ch + c];
+#pragma unroll
+    for (int c = 0; c < V; ++c) {
+        Map before = NOTHING;
+#pragma unroll
+        for (int i = 0; i < 3; ++i) before = join<SEG>(before, in > i ? three[i][c] : NOTHING);
+        h[c] = apply<SEG>(before, h[c]);
+    }
 }
 
 // The number of a row's live steps.
@@ -377,7 +395,7 @@ template <typename E, int G, int V, int LANES, int WAVES, bool SEG, bool STREAM>
 __global__ void __launch_bounds__(64 * WAVES, WAVES > 4 ? 2 : sizeof(E) == 2 ? 4 : 3) wnv_recurrence_fwd(RecArgs a) {
     typedef Shape<LANES, WAVES> S;
     constexpr int W = LANES * V, STEPS = S::STEPS;
-    __shared__ Map quads[S::QUADS][W], blocks[S::BLOCKS][W], prev[S::BLOCKS][W], groups[W];
+    __shared__ Map quads[S::QUADS][W], blocks[S::BLOCKS][W], prev[S::BLOCKS][W], chunk[W], groups[W];
     __shared__ float base[W];
     const int tid = threadIdx.x, lane = tid % LANES, wave = tid / 64, at = lane * V;
     const int quad = tid / (4 * LANES), part = quad / 4 >> a.part_bits, parts = S::BLOCKS >> a.part_bits;
@@ -443,7 +461,7 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES > 4 ? 2 : sizeof(E) == 2 ? 4
     if (wave < 3 && ch < W) {
         const Slots slots = slots_at(a.slots, p.row, a.chunks, W, ch);
         if (wave == 0) {
-            join_blocks<W, S::QUADS, false, SEG>(a, slots, p.chunk, ch, quads, blocks, prev);
+            chunk[ch] = join_blocks<W, S::QUADS, false, SEG>(a, slots, p.chunk, ch, quads, blocks, prev);
         } else if (wave == 1) {
             base[ch] = state_before_groups<W, SEG>(slots, p.chunk, a.h0 ? a.h0[p.b * a.h0b + min(p.tile * W + ch / V * V, a.C - V) + ch % V] : 0.f);
         } else {
@@ -452,6 +470,7 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES > 4 ? 2 : sizeof(E) == 2 ? 4
     }
     __syncthreads();
 
+    if (ends_section(p.chunk, a.chunks) && tid < W) hand_out_section<W, SEG>(a, p.row, p.chunk, tid, chunk[tid], prev[0][tid], groups[tid], base[tid]);
     float h[V];
     const int last_quad = parts > 1 ? (((a.T - 1) / BLOCK >> a.part_bits) + 1 << a.part_bits) * 4 - 1 : S::QUADS - 1;      // of the last part that is there
 #pragma unroll
@@ -459,14 +478,11 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES > 4 ? 2 : sizeof(E) == 2 ? 4
         h[i] = apply<SEG>(prev[part][at + i], apply<SEG>(groups[at + i], base[at + i]));
         if (a.saved && quad == part << a.part_bits + 2 && tid % (4 * LANES) < LANES)
             a.saved[(((long long)p.row * a.chunks + p.chunk) * parts + part) * W + at + i] = h[i];
-        h[i] = state_before_quad<W, S::QUADS, false, SEG>(a, quads, blocks, quad, at + i, h[i]);
+    }
+    state_before_quad<W, V, S::QUADS, false, SEG>(a, quads, blocks, quad, at, h);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
         h[i] = apply<SEG>(before[i], h[i]);
-        if (quad == last_quad && tid % (4 * LANES) >= 3 * LANES) {      // its last stretch: the state behind it
-            const float last = apply<SEG>(m[i], h[i]);
-            if (ends_section(p.chunk, a.chunks))
-                publish<SEG>(slots_at(a.slots, p.row, a.chunks, W, at + i).section + (long long)(p.chunk / (GROUP * GROUP)) * W, {0.f, 1.f, last});
-            if (p.chunk + 1 == a.chunks) a.h_last[(long long)p.b * a.C + c + i] = last;
-        }
     }
     E* y = (E*)a.y + ((long long)p.b * a.T + (long long)p.chunk * STEPS) * a.C;
     const uint32_t to = (uint32_t)(tid / LANES * L * a.C + c) * (uint32_t)sizeof(E);
@@ -493,6 +509,10 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES > 4 ? 2 : sizeof(E) == 2 ? 4
     if (whole && !any) run(std::true_type{}, std::false_type{});
     else if (SEG && whole) run(std::true_type{}, std::integral_constant<bool, SEG>{});
     else run(std::false_type{}, std::integral_constant<bool, SEG>{});
+    if (p.chunk + 1 == a.chunks && quad == last_quad && tid % (4 * LANES) >= 3 * LANES) {       // its last stretch: the state behind it
+#pragma unroll
+        for (int i = 0; i < V; ++i) a.h_last[(long long)p.b * a.C + c + i] = h[i];
+    }
 }
 
 // g_t = dy_t sigmoid(o_t);  dh_t = g_t + (what step t+1 hands back);  hands back r = a_t dh_t, nothing over a beginning
@@ -503,7 +523,7 @@ template <typename E, int G, int V, int LANES, int WAVES, bool SEG, bool STREAM>
 __global__ void __launch_bounds__(64 * WAVES, 2) wnv_recurrence_bwd(RecArgs a) {
     typedef Shape<LANES, WAVES> S;
     constexpr int W = LANES * V, STEPS = S::STEPS;
-    __shared__ Map ahead[S::QUADS][W], back[S::QUADS][W], ahead_blocks[S::BLOCKS][W], back_blocks[S::BLOCKS][W], prev[S::BLOCKS][W], groups[W];      // of h and of r
+    __shared__ Map ahead[S::QUADS][W], back[S::QUADS][W], ahead_blocks[S::BLOCKS][W], back_blocks[S::BLOCKS][W], prev[S::BLOCKS][W], chunk[W], groups[W];    // of h and of r
     __shared__ float base[W];
     const int tid = threadIdx.x, lane = tid % LANES, wave = tid / 64, at = lane * V;
     const int quad = tid / (4 * LANES), part = quad / 4 >> a.part_bits, parts = S::BLOCKS >> a.part_bits;
@@ -580,7 +600,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) wnv_recurrence_bwd(RecArgs a) {
     if (wave < (S::BLOCKS > 1 ? 4 : 3) && ch < W) {
         const Slots slots = slots_at(a.slots, p.row, a.chunks, W, ch);
         if (wave == 0) {
-            join_blocks<W, S::QUADS, true, SEG>(a, slots, order, ch, back, back_blocks, prev);
+            chunk[ch] = join_blocks<W, S::QUADS, true, SEG>(a, slots, order, ch, back, back_blocks, prev);
         } else if (wave == 1) {
             base[ch] = state_before_groups<W, SEG>(slots, order, a.dh_last ? a.dh_last[(long long)p.b * a.C + min(p.tile * W + ch / V * V, a.C - V) + ch % V] : 0.f);
         } else if (wave == 2) {
@@ -592,21 +612,19 @@ __global__ void __launch_bounds__(64 * WAVES, 2) wnv_recurrence_bwd(RecArgs a) {
     }
     __syncthreads();
 
+    if (ends_section(order, a.chunks) && tid < W) hand_out_section<W, SEG>(a, p.row, order, tid, chunk[tid], prev[0][tid], groups[tid], base[tid]);
     float h[V], x[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         h[i] = saved.get(i);
         x[i] = apply<SEG>(prev[part][at + i], apply<SEG>(groups[at + i], base[at + i]));
-        h[i] = state_before_quad<W, S::QUADS, false, SEG>(a, ahead, ahead_blocks, quad, at + i, h[i]);
-        x[i] = state_before_quad<W, S::QUADS, true, SEG>(a, back, back_blocks, quad, at + i, x[i]);
+    }
+    state_before_quad<W, V, S::QUADS, false, SEG>(a, ahead, ahead_blocks, quad, at, h);
+    state_before_quad<W, V, S::QUADS, true, SEG>(a, back, back_blocks, quad, at, x);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
         h[i] = apply<SEG>(h_before[i], h[i]);
         x[i] = apply<SEG>(r_before[i], x[i]);
-        if (tid < LANES) {                              // the chunk's first stretch: what flows out of it
-            const float out = apply<SEG>(r[i], x[i]);
-            if (ends_section(order, a.chunks))
-                publish<SEG>(slots_at(a.slots, p.row, a.chunks, W, at + i).section + (long long)(order / (GROUP * GROUP)) * W, {0.f, 1.f, out});
-            if (p.chunk == 0 && a.dh0) a.dh0[(long long)p.b * a.C + c + i] = out;
-        }
     }
     E* dz = (E*)a.dz + ((long long)p.b * a.T + (long long)p.chunk * STEPS) * (G * (long long)a.C);
     const uint32_t to = (uint32_t)(tid / LANES * L * G * a.C + c) * (uint32_t)sizeof(E);
@@ -649,6 +667,10 @@ __global__ void __launch_bounds__(64 * WAVES, 2) wnv_recurrence_bwd(RecArgs a) {
     };
     if (whole) run(std::true_type{});
     else run(std::false_type{});
+    if (p.chunk == 0 && a.dh0 && tid < LANES) {         // the first stretch: what flows out of it
+#pragma unroll
+        for (int i = 0; i < V; ++i) a.dh0[(long long)p.b * a.C + c + i] = x[i];
+    }
 }
 
 __global__ void __launch_bounds__(256) wnv_recurrence_fill(uint4* p, long long n) {
