@@ -28,12 +28,11 @@ def require_gpu_tensor(t: torch.Tensor, what: str) -> None:
 
 
 def refuse_tangents(what: str, *tensors: Optional[torch.Tensor]) -> None:
-    """Dual tensors of forward-mode differentiation do not require grad, and the kernels know nothing of their tangents.  (Within a dual
-    level only: the level is looked up first, since the calls are a few microseconds long.)"""
-    if getattr(forward_ad, "_current_level", 0) >= 0:
-        for t in tensors:
-            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
-                raise RuntimeError(f"{what} has no forward-mode derivative")
+    """Dual tensors of forward-mode differentiation do not require grad, and the kernels know nothing of their tangents.  Called within a dual
+    level only, which the callers look up themselves: they are a few microseconds long."""
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{what} has no forward-mode derivative")
 
 
 def make_config(*, out_channels, layers, stacks, residual_channels, gate_channels, skip_out_channels,
@@ -510,7 +509,8 @@ class Q4Linear:
 
     def _rows(self, x: torch.Tensor):
         """x as the kernels take it, its number of rows and its type."""
-        refuse_tangents("a 4-bit product", x)
+        if getattr(forward_ad, "_current_level", 0) >= 0:
+            refuse_tangents("a 4-bit product", x)
         shape = x.shape
         code = self._DTYPES.get(x.dtype)
         if (code is None or x.get_device() != self._index or len(shape) != 2 or shape[1] != self.cin or shape[0] == 0
@@ -529,7 +529,8 @@ class Q4Linear:
 
     def recurrence_step(self, x: torch.Tensor, state: torch.Tensor) -> torch.Tensor:
         """x (B, cin), ``state`` (B, channels) float32 contiguous, updated in place -> y (B, channels) of x's type."""
-        refuse_tangents("Q4Linear.recurrence_step", state)
+        if getattr(forward_ad, "_current_level", 0) >= 0:
+            refuse_tangents("a 4-bit product", state)
         x, B, code = self._rows(x)
         if state.shape != (B, self.channels):
             raise ValueError(f"state is {tuple(state.shape)}, expected {(B, self.channels)}")

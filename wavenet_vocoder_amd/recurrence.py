@@ -14,6 +14,7 @@ from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 from torch.autograd.graph import increment_version
 
@@ -151,7 +152,8 @@ def gated_recurrence(z: torch.Tensor, h0: Optional[torch.Tensor] = None, *, outp
     entry is an utterance begun before this call, which goes on from ``h0``.  Differentiable (once, not in forward mode) in z and h0.
     Runs on the current stream of z's device and is capturable; the same call gives the same bits, and a row's do not depend on its batch.
     Parts of a long sequence wait for each other on the device; should one not answer for seconds, what depends on it is NaN."""
-    refuse_tangents("gated_recurrence", z, h0)
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        refuse_tangents("gated_recurrence", z, h0)
     require_gpu_tensor(z, "z")
     _dtype(z)
     if z.dim() != 3:
@@ -174,10 +176,20 @@ def gated_recurrence(z: torch.Tensor, h0: Optional[torch.Tensor] = None, *, outp
     return y, h_last
 
 
+_step = None
+
+
+def _load_step():
+    global _step
+    _step = _lib.lib().wnv_recurrence_step
+    return _step
+
+
 def gated_recurrence_step(z: torch.Tensor, state: torch.Tensor, *, output_gate: bool = True) -> torch.Tensor:
     """One step: z (B, 3 C) (``output_gate=False``: (B, 2 C)), ``state`` (B, C) float32 contiguous, updated in place -> y (B, C) of z's
     type.  Not differentiable: the training form is ``gated_recurrence``."""
-    refuse_tangents("gated_recurrence_step", z, state)
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        refuse_tangents("gated_recurrence_step", z, state)
     shape, sshape, gates, dev = z.shape, state.shape, 3 if output_gate else 2, z.get_device()
     code = _DTYPES.get(z.dtype)
     if (code is None or dev < 0 or len(shape) != 2 or len(sshape) != 2 or sshape[0] != shape[0] or sshape[1] * gates != shape[1]
@@ -188,7 +200,7 @@ def gated_recurrence_step(z: torch.Tensor, state: torch.Tensor, *, output_gate: 
     z = _rows(z)
     y = z.new_empty(sshape)
     increment_version(state)            # a graph that saved the state has to see that it changed
-    st = _lib.lib().wnv_recurrence_step(dev, z.data_ptr(), z.stride(0), state.data_ptr(), y.data_ptr(), B, n, gates, code, _raw_stream(dev))
+    st = (_step or _load_step())(dev, z.data_ptr(), z.stride(0), state.data_ptr(), y.data_ptr(), B, n, gates, code, _raw_stream(dev))
     if st:
         check(st)
     return y
