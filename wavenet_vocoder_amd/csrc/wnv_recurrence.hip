@@ -350,12 +350,23 @@ __device__ __forceinline__ void state_before_quad(const RecArgs& a, const Map (&
     for (int i = 0; i < 3; ++i)
 #pragma unroll
         for (int c = 0; c < V; ++c) three[i][c] = quads[BACK ? QUADS - 1 - 4 * block - i : 4 * block + i][ch + c];
+    if (QUADS == 4) {                   // a quad is a wave: one branch for all of it
+        if (in == 0) return;
 #pragma unroll
-    for (int c = 0; c < V; ++c) {
-        Map before = NOTHING;
+        for (int c = 0; c < V; ++c) {
+            Map before = three[0][c];
+            if (in > 1) before = join<SEG>(before, three[1][c]);
+            if (in > 2) before = join<SEG>(before, three[2][c]);
+            h[c] = apply<SEG>(before, h[c]);
+        }
+    } else {
 #pragma unroll
-        for (int i = 0; i < 3; ++i) before = join<SEG>(before, in > i ? three[i][c] : NOTHING);
-        h[c] = apply<SEG>(before, h[c]);
+        for (int c = 0; c < V; ++c) {
+            Map before = NOTHING;
+#pragma unroll
+            for (int i = 0; i < 3; ++i) before = join<SEG>(before, in > i ? three[i][c] : NOTHING);
+            h[c] = apply<SEG>(before, h[c]);
+        }
     }
 }
 
@@ -397,8 +408,8 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES > 4 ? 2 : sizeof(E) == 2 ? 4
     constexpr int W = LANES * V, STEPS = S::STEPS;
     __shared__ Map quads[S::QUADS][W], blocks[S::BLOCKS][W], prev[S::BLOCKS][W], chunk[W], groups[W];
     __shared__ float base[W];
-    const int tid = threadIdx.x, lane = tid % LANES, wave = tid / 64, at = lane * V;
-    const int quad = tid / (4 * LANES), part = quad / 4 >> a.part_bits, parts = S::BLOCKS >> a.part_bits;
+    const int tid = threadIdx.x, lane = tid % LANES, wave = __builtin_amdgcn_readfirstlane(tid / 64), at = lane * V;
+    const int quad = LANES == 16 ? __builtin_amdgcn_readfirstlane(tid / 64) : tid / (4 * LANES), part = quad / 4 >> a.part_bits, parts = S::BLOCKS >> a.part_bits;
     Place p;
     if (!draw_place<false>(a, W, p)) return;
     const int c = min(p.tile * W + at, a.C - V), n = live_to(a, p.b);
@@ -525,8 +536,8 @@ __global__ void __launch_bounds__(64 * WAVES, 2) wnv_recurrence_bwd(RecArgs a) {
     constexpr int W = LANES * V, STEPS = S::STEPS;
     __shared__ Map ahead[S::QUADS][W], back[S::QUADS][W], ahead_blocks[S::BLOCKS][W], back_blocks[S::BLOCKS][W], prev[S::BLOCKS][W], chunk[W], groups[W];    // of h and of r
     __shared__ float base[W];
-    const int tid = threadIdx.x, lane = tid % LANES, wave = tid / 64, at = lane * V;
-    const int quad = tid / (4 * LANES), part = quad / 4 >> a.part_bits, parts = S::BLOCKS >> a.part_bits;
+    const int tid = threadIdx.x, lane = tid % LANES, wave = __builtin_amdgcn_readfirstlane(tid / 64), at = lane * V;
+    const int quad = LANES == 16 ? __builtin_amdgcn_readfirstlane(tid / 64) : tid / (4 * LANES), part = quad / 4 >> a.part_bits, parts = S::BLOCKS >> a.part_bits;
     Place p;
     if (!draw_place<true>(a, W, p)) return;
     const int order = a.chunks - 1 - p.chunk, c = min(p.tile * W + at, a.C - V), n = live_to(a, p.b);
