@@ -158,9 +158,9 @@ __device__ __forceinline__ bool ends_section(int k, int chunks) { return (k + 1)
 // ---- the shape of a workgroup -------------------------------------------------------------------------------------------------
 // 4 (or 8) waves of 4 stretches of L steps; a stretch is 16 lanes, a row of the wave, along the channels.  A lane holds V = 4 channels, so
 // that a tile is 64 channels wide: 128 bytes of a 16-bit type, 256 of float32 (8 channels a lane and 4 steps, for rows of 256 bytes
-// of a 16-bit type too, took 213 us for 185 forward and 506 for 316 backward, bf16 8 x 24064 x 512: more maps to join per step).
-// Registers decide how many workgroups share a CU: 3 forward and 2 backward, each with 32 steps x channels a thread; half the steps
-// and 3 workgroups backward took 356 us for 316.  The last lane of a tile that ends in no multiple of V starts earlier and shares
+// of a 16-bit type too, took 213 us forward when this took 185, and 506 backward for 316, bf16 8 x 24064 x 512: more maps to join per step).
+// Registers decide how many workgroups share a CU: 3 forward (4 of 16-bit types) and 2 backward, each with 32 steps x channels a thread;
+// half the steps and 3 workgroups backward took 356 us when this took 316.  The last lane of a tile that ends in no multiple of V starts earlier and shares
 // channels with its neighbour (both compute and write the same); V = 1 is for rows narrower than 4.  Narrow tiles take stretches of 4
 // lanes, 16 to a wave.
 //
@@ -183,10 +183,10 @@ template <typename E, int V> struct Vec {
         return (float)__builtin_bit_cast(wnv_f16, (uint16_t)(w[i / 2] >> (16 * (i & 1))));
     }
 };
-// STREAM: past the caches, for data that no cache holds until its next use anyway (8 x 24064 x 512 forward: float32 271 us and 298
-// without, bf16 166 and 175).  What fits the last-level cache is better left to it (1 x 24064 x 128 float32: 15.7 with, 14.2 without),
-// and rows that are no multiple of 128 bytes have to be: their neighbours share a line, which the cache puts together (16 x 24064 x 100
-// float32 backward: 343 with, 250 without).
+// STREAM: past the caches, for data that no cache holds until its next use anyway (8 x 24064 x 512, with and without: float32 forward 285 and
+// 301 us, backward 496 and 523; bf16 169 and 181, 290 and 312).  Rows that are no multiple of 128 bytes are left to the caches: their
+// neighbours share a line, which the cache puts together (16 x 24064 x 100 float32: forward 195 with and 168 without, backward 376 and
+// 307), and what fits the last level may be there for its next user.
 template <int BYTES> struct Raw { typedef uint32_t T __attribute__((ext_vector_type(BYTES / 4), aligned(1))); };
 template <> struct Raw<2> { typedef uint16_t T __attribute__((aligned(1))); };
 template <> struct Raw<4> { typedef uint32_t T __attribute__((aligned(1))); };
@@ -244,8 +244,8 @@ template <int LANES, bool BACK, bool SEG> __device__ __forceinline__ void join_q
     if ((row >> 1) != BACK) before = join<SEG>(BACK ? high : low, before);
 }
 // What a forward pass keeps of its stretch's steps for the second run over them.  float32: a and u v.  16-bit types: the smaller of a and u,
-// negative where that is u, next to v as it came; 16 registers less, which are a fourth wave per SIMD (bf16 8 x 24064 x 512: 172 us for
-// 178), and the arithmetic of wnv_blend.
+// negative where that is u, next to v as it came; 16 registers less, which are a fourth wave per SIMD (bf16 8 x 24064 x 512: 171 us, with
+// a and u v in three waves 178), and the arithmetic of wnv_blend.
 template <typename E, int V> struct Steps {
     float keep[L][V], put[L][V];
     __device__ __forceinline__ void hold(int l, int i, float a, float, float uv) { keep[l][i] = a; put[l][i] = uv; }
@@ -401,7 +401,11 @@ template <int LANES, bool SEG> __device__ __forceinline__ int begins_in(const En
 // One chunk of one tile.  Each thread reduces its stretch to a map, the wave joins its rows', wave 0 the chunk's and its group's while
 // waves 1 and 2 find the state before the group; then each thread knows the state before its stretch and runs over it again, out of
 // its registers.  z is read once.  Chunks that are live to their end (FULL) run without a test at every step: the steps' exponentials
-// and reciprocals then overlap (bf16 8 x 24064 x 512 forward: 164 us, with the tests 185).
+// and reciprocals then overlap (8 x 24064 x 512: bf16 forward 169 us, with the tests 187, backward 290 and 330; float32, which waits for
+// memory, 285 and 282).  In a packed slot most waves hold no beginning, and run as in any other row.
+//
+// What bounds it at 8 x 24064 x 512: float32 memory, 270 us for 1.58 GB, with the vector units issuing 30% of the time.  bf16 the vector units,
+// 73% of the time in packed slots -- four transcendentals an element, at a quarter of the rate --, 171 us for 0.79 GB.
 template <typename E, int G, int V, int LANES, int WAVES, bool SEG, bool STREAM>
 __global__ void __launch_bounds__(64 * WAVES, WAVES > 4 ? 2 : sizeof(E) == 2 ? 4 : 3) wnv_recurrence_fwd(RecArgs a) {
     typedef Shape<LANES, WAVES> S;
@@ -727,14 +731,13 @@ wnv_status launched(const char* who) {
 
 // How B x T x C is cut.  Tiles are 64 channels and chunks 128 steps, or narrow ones of 16 channels (4 with V = 1) and 512 steps:
 //  * where rows are narrow, lanes along the channels are idle, and with them go a quarter of the chunks to wait for (forward and
-//    backward of 16 x 24064, us, narrow tiles and wide ones: float32 C = 20 97 and 121, C = 40 198 and 170; bf16 C = 32 85 and 112,
-//    C = 48 134 and 133);
+//    backward of 16 x 24064, us, narrow tiles and wide ones: float32 C = 20 99 and 126, C = 40 191 and 172; bf16 C = 32 87 and 121,
+//    C = 48 119 and 135);
 //  * where there is little data and that makes one chunk of several, which needs neither a filled workspace nor a wait: the host's
-//    time falls by a launch and an allocation (2 x 300 x 128 float32 forward 9.3 us a call and 13.7, 2 x 400 x 512 9.4 and 12.7).
-// Of narrow tiles two chunks become one of 8 waves, for the same reason (2 x 700 x 128 float32 forward 9.6 us a call and 12.9, both
-// passes 91 and 103).
-// More data is the GPU's time, and is read faster in whole lines by more workgroups (64 x 700 x 128 float32 forward 26 us in narrow
-// tiles of 8 waves and 21 in wide ones, both passes 66 and 58; 64 x 512 x 512 both passes 179 and 134).
+//    time falls by a launch and an allocation (2 x 300 x 128 float32 forward 10.1 us a call and 14.2, 2 x 400 x 512 10.3 and 14.6).
+// Of narrow tiles two chunks become one of 8 waves, for the same reason (2 x 700 x 128 float32 forward 10.2 us a call and 14.6).
+// More data is the GPU's time, and is read faster in whole lines by more workgroups (64 x 700 x 128 float32 forward 31 us in narrow
+// tiles of 8 waves and 27 in wide ones, backward 43 and 42; 64 x 512 x 512 backward 119 and 97).
 constexpr int NARROW_CHANNELS = 32, LITTLE_CHANNELS = 256;
 constexpr int64_t LITTLE = 2 << 20;
 struct Cut { int V, lanes, waves, W, tiles, chunks, part_bits, parts; };
